@@ -56,6 +56,11 @@ extern "C" {
 #define RBG_BIGNN_CONV_ONLY      0u  /* exactly BiGNNConv.forward */
 #define RBG_BIGNN_LEAKY_NORM     1u  /* + LeakyReLU(slope) + row L2-normalize (NGCF.forward's per-layer tail) */
 
+/* element types of the operators over large item vocabularies (everything else is fp32) */
+#define RBG_F32  0
+#define RBG_BF16 1
+#define RBG_F16  2
+
 #define RBG_MAX_FUSED_LAYERS     8   /* K up to this is fused into K launches; larger K still works (unfused mean) */
 
 typedef struct rbg_graph rbg_graph;
@@ -681,6 +686,82 @@ int rbg_ipc_wait(const void *flags, int n, uint64_t value, int timeout_ms, int *
 /* out[t] = scale * (srcs[0][t] + srcs[1][t] + ...), added left to right: the layer mean of lightgcn.py:80-81 over
  * separately held layer outputs (the sharded propagation) in one launch.  n_srcs <= RBG_MAX_FUSED_LAYERS + 1. */
 int rbg_mean_f32(const float *const *srcs, int n_srcs, int64_t n_floats, float scale, float *out, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * operators over large item vocabularies: a table's rows and their gradient, losses on whole rows of logits, scores from an
+ * 8-bit table.  `dtype` is RBG_F32, RBG_BF16 or RBG_F16; arithmetic is in 32 bits, an output is rounded once, to nearest even.
+ * Leading dimensions count elements (bytes for codes).  Ids and targets are DEVICE int64; one outside its range reads nothing and
+ * adds to nothing (-1 is the usual "none").  Sums run in an order that sizes and alignments alone decide: results are bit-stable.
+ * A workspace belongs to the call until its work on `stream` has ended: calls that may overlap (two streams, two captured graphs
+ * replayed side by side) need one each.  No call allocates or synchronizes; every call can be captured.
+ * ------------------------------------------------------------------------------------------- */
+
+/* out[i, :] = scale * table[ids[i], :]   (zeros where ids[i] is outside [0, n_rows)).  Rows of d elements; ldt, ldo >= d.
+ * The row gather of lightgcn.py:60-68,128 for any element type; out must not overlap table. */
+int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dtype, const int64_t *ids, int64_t n, float scale, void *out,
+                  int64_t ldo, void *stream);
+
+/* Its gradient: out[v, :] = scale * sum over the places i with ids[i] = v, ascending, of grad[i, :]; zeros for rows nothing refers to and
+ * for row padding_idx (negative: none).  out is [n_rows, d] contiguous and written whole; out_dtype is dtype or RBG_F32.  The places
+ * are sorted by row (no float atomics).  n < 2^31 - 2^16, n_rows < 2^31 - 1, d <= 2^20.  `workspace`: rbg_embedding_grad_workspace(n, n_rows, d) bytes, 16-byte aligned. */
+int rbg_embedding_grad_workspace(int64_t n, int64_t n_rows, int d, int64_t *bytes);
+int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *ids, int64_t n, int64_t n_rows, int d, float scale,
+                       int64_t padding_idx, void *out, int out_dtype, void *workspace, void *stream);
+
+/* Distillation from a teacher's top list.  Row b has V student logits z (row stride ldz) and k entries (idx, val) of the teacher,
+ * [n, k] contiguous — what rbg_full_sort_topk_f32 writes.  Entries with idx outside [0, V) are none, whatever val holds.
+ *   p = softmax(val / T) over the row's entries;  log q = log softmax(z / T) over all V;   loss[b] = T^2 sum_j p_j (log p_j - log q_j)
+ *   grad[b, :] = row_w[b] dloss[b] / dz = row_w[b] T (q - p)        (row_w NULL: 1;  entries of equal idx add up)
+ * A row without entries (none, or all val -inf), or whose logits are all -inf, has loss 0 and gradient 0.  Other infinities and
+ * NaN follow the formula.  grad NULL: the loss alone.  stats (or NULL) [n, 2] receives what the backward form needs.
+ * 1 <= k <= 256, 1e-15 <= T <= 1e15.  grad may be z itself (same stride).  `workspace`: rbg_distill_topk_workspace(n, V) bytes, 16-byte aligned. */
+int rbg_distill_topk_workspace(int64_t n, int64_t V, int64_t *bytes);
+int rbg_distill_topk(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V, const int64_t *idx, const float *val, int k, float T,
+                     const float *row_w, float *loss, float *stats, void *grad, int64_t ldg, void *workspace, void *stream);
+int rbg_distill_topk_backward(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V, const int64_t *idx, const float *val, int k,
+                              float T, const float *stats, const float *row_w, void *grad, int64_t ldg, void *stream);
+
+/* logp[m] = z[m, targets[m]] - log sum_j exp z[m, j]; 0 for a row without a target in [0, V) or whose logits are all -inf.
+ * backward: grad[m, :] = row_g[m] (onehot(targets[m]) - softmax(z[m, :])), zeros for such rows.  stats [m, 2] as above (or NULL).
+ * `workspace`: rbg_token_logp_workspace(m, V) bytes, 16-byte aligned. */
+int rbg_token_logp_workspace(int64_t m, int64_t V, int64_t *bytes);
+int rbg_token_logp(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, const int64_t *targets, float *logp, float *stats,
+                   void *workspace, void *stream);
+int rbg_token_logp_backward(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, const int64_t *targets, const float *stats,
+                            const float *row_g, void *grad, int64_t ldg, void *stream);
+
+/* Preference loss on pairs of packed sequences (the reference's BPR, lightgcn.py:93-100, is its case of one token, one shared row
+ * and no reference model).  Sequence s is the tokens [offsets[s], offsets[s + 1]) (DEVICE int64 [2 pairs + 1], ascending; an empty one
+ * sums to 0); sequence 2 i is pair i's preferred one, 2 i + 1 the other; ref[s] is the reference model's sum.
+ *   margin[i] = beta ((sum logp of 2 i - ref[2 i]) - (sum logp of 2 i + 1 - ref[2 i + 1]))
+ *   loss[i]   = -(1 - smoothing) log sigmoid(margin[i]) - smoothing log sigmoid(-margin[i])          0 <= smoothing <= 1
+ * The sums are held in 64 bits: a margin is a small difference of large sums.
+ * backward: grad_logp [m] from margin and the gradients g_loss, g_margin [pairs] (either may be NULL); zeros outside the sequences.
+ * Offsets outside [0, m] are clamped. */
+int rbg_preference_loss(const float *logp, int64_t m, const int64_t *offsets, int64_t pairs, const float *ref, float beta, float smoothing,
+                        float *loss, float *margin, void *stream);
+int rbg_preference_loss_backward(const float *margin, int64_t m, const int64_t *offsets, int64_t pairs, float beta, float smoothing,
+                                 const float *g_loss, const float *g_margin, float *grad_logp, void *stream);
+
+/* The same from the logits themselves, value and gradient in one call: logp as rbg_token_logp, kept in 64 bits;
+ * grad[m, :] = d(sum_i pair_w[i] loss[i]) / dz (pair_w NULL: 1).  grad may be z itself (same stride).
+ * `workspace`: rbg_preference_grad_workspace(m, V) bytes, 16-byte aligned. */
+int rbg_preference_grad_workspace(int64_t m, int64_t V, int64_t *bytes);
+int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, const int64_t *targets, const int64_t *offsets,
+                        int64_t pairs, const float *ref, float beta, float smoothing, const float *pair_w, float *loss, float *margin,
+                        void *grad, int64_t ldg, void *workspace, void *stream);
+
+/* Rows in 8 bits with a scale each: scale[r] = fl32(max |x[r, :]| / 127), codes[r, j] = x[r, j] / scale[r], rounded to nearest even and
+ * kept in [-127, 127]; zeros in columns [K, ldc).  A row whose scale would be below 2^-126 has scale 0 and codes 0; one that
+ * holds an infinity or NaN has scale NaN and codes 0.  ldc % 16 == 0, codes 16-byte aligned. */
+int rbg_quantize_rows_i8(const void *x, int64_t ldx, int dtype, int64_t n, int64_t K, int8_t *codes, int64_t ldc, float *scale, void *stream);
+
+/* The scores of rbg_score_f32 from rows in 8 bits: S[b, j] = su[b] si[j] sum_k qu[b, k] qi[j, k], the sum exact in 32-bit integers
+ * (1 <= K <= 131071).  qu [B, ldu]: ldu % 128 == 0, columns [K, ldu) zero (what rbg_quantize_rows_i8 writes); qi [n, ldi]:
+ * ldi % 16 == 0, any value in columns [K, K rounded up to 16), which have to be there for the last row too.  qu, qi 16-byte aligned.
+ * S [B, lds] of out_dtype, rounded once from 32 bits. */
+int rbg_score_i8(const int8_t *qu, int64_t ldu, const float *su, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n,
+                 int64_t K, void *S, int64_t lds, int out_dtype, void *stream);
 
 #ifdef __cplusplus
 }

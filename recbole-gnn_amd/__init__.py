@@ -5,12 +5,14 @@ The package directory name carries a hyphen; import it as ``recbole_gnn_amd`` (t
 the repository root) or with ``importlib.import_module("recbole-gnn_amd")``.
 Importing fails loudly if librbgnn.so (the HIP extension) has not been built; there is no CPU path.
 """
-from . import _lib, colsharded, driver, graph, hybrid, models, ops, sharded, sharded_train, synth, train  # noqa: F401
+from . import _lib, colsharded, driver, graph, hybrid, models, ops, sharded, sharded_train, synth, train, vocab  # noqa: F401
 from ._lib import LIB_PATH, RbgError  # noqa: F401
 from .graph import (GraphHandle, InteractionDataset, device_count, find_communities, get_option, get_tuning, norm_edges,  # noqa: F401
                     set_option, set_tuning)
 from .models import NCL, NGCF, SGL, GeneralGraphRecommender, LightGCN, SimGCL, XSimGCL  # noqa: F401
 from .ops import BiGNNConv, LightGCNConv, full_sort_topk, gather_rows, lightgcn_forward, score, spmm  # noqa: F401
+from .vocab import (distill_topk, distill_topk_grad, embedding, embedding_grad, preference_grad, preference_loss, quantize_rows,  # noqa: F401
+                    score_int8, token_logp)
 
 from .train import (FusedBPRAdam, FusedNCLAdam, FusedNGCFAdam, FusedSGLAdam, FusedSimGCLAdam, FusedXSimGCLAdam, GraphedStep,  # noqa: F401,E402
                     fused_stepper)

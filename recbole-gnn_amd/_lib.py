@@ -15,6 +15,7 @@ GRAPH_DEFAULT, GRAPH_KEEP_HOST, GRAPH_BUILD_ON_HOST, GRAPH_NATURAL_ORDER, GRAPH_
 FWD_DEFAULT, FWD_KEEP_LAST_LAYER, FWD_LAYERS_SCRATCH = 0, 1, 2
 BIGNN_CONV_ONLY, BIGNN_LEAKY_NORM = 0, 1
 MAX_FUSED_LAYERS = 8
+F32, BF16, F16 = 0, 1, 2  # element types of the operators over large item vocabularies
 
 c_i64, c_i32, c_u32, c_int, c_f32, c_vp = (ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32, ctypes.c_int,
                                            ctypes.c_float, ctypes.c_void_p)
@@ -114,6 +115,22 @@ SIGNATURES = {
     "rbg_lse_rows_f32": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_f32, c_f32, c_vp, c_vp, c_vp]),
     "rbg_lse_rows_backward_f32": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_f32, c_f32, c_vp, c_vp, c_vp,
                                           c_vp, c_vp, c_vp]),
+    "rbg_embedding": (c_int, [c_vp, c_i64, c_i64, c_int, c_int, c_vp, c_i64, c_f32, c_vp, c_i64, c_vp]),
+    "rbg_embedding_grad_workspace": (c_int, [c_i64, c_i64, c_int, P(c_i64)]),
+    "rbg_embedding_grad": (c_int, [c_vp, c_i64, c_int, c_vp, c_i64, c_i64, c_int, c_f32, c_i64, c_vp, c_int, c_vp, c_vp]),
+    "rbg_distill_topk_workspace": (c_int, [c_i64, c_i64, P(c_i64)]),
+    "rbg_distill_topk": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_f32, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp]),
+    "rbg_distill_topk_backward": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_f32, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "rbg_token_logp_workspace": (c_int, [c_i64, c_i64, P(c_i64)]),
+    "rbg_token_logp": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "rbg_token_logp_backward": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "rbg_preference_loss": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_f32, c_f32, c_vp, c_vp, c_vp]),
+    "rbg_preference_loss_backward": (c_int, [c_vp, c_i64, c_vp, c_i64, c_f32, c_f32, c_vp, c_vp, c_vp, c_vp]),
+    "rbg_preference_grad_workspace": (c_int, [c_i64, c_i64, P(c_i64)]),
+    "rbg_preference_grad": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_f32, c_f32, c_vp, c_vp, c_vp, c_vp, c_i64,
+                                    c_vp, c_vp]),
+    "rbg_quantize_rows_i8": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "rbg_score_i8": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_int, c_vp]),
 }
 
 

@@ -1,0 +1,530 @@
+// embed.hip — rows of a table looked up by id with a scale, and the table's gradient by sorted ids.
+//
+//   out[i] = s T[id_i]            dT[v] = s sum_{i : id_i = v, ascending i} G[i]
+//
+// The lookup is a gather: 8 bytes of id, a row read, a row written.
+// The gradient sorts the places by id (stably: equal ids keep their order) and then sums runs.  A lane-group of d / (16 bytes)
+// lanes walks a chunk of consecutive sorted places and writes every row whose run lies inside the chunk; a run that crosses a
+// chunk's border leaves 32-bit partial sums, one for the chunk's first run and one for its last, which a second launch adds
+// in chunk order.  No float atomics: the order of every sum is decided by the sizes alone.  The rows nothing refers to are
+// zeroed in the same launch by workgroups of their own, which find them by bisection in the sorted ids, so that every
+// row of the gradient is written once.
+//
+// The sort: up to kRankMax places, a place's rank is counted outright — the number of (id, place) pairs in front of it — from the
+// ids staged in LDS: N^2 compares, all independent, in one launch.  Above, least-significant-digit radix passes of
+// up to nine bits, three launches each (digit counts per tile, their prefix per digit, a stable scatter).
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "vocab_common.h"
+
+namespace rbg {
+
+// ---- lookup --------------------------------------------------------------------------------------------------------------
+
+// One thread per vector of VEC elements; `per_row` vectors in a row.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table, int64_t ldt, int64_t n_rows, const int64_t *__restrict__ ids,
+                                                     int64_t n, int per_row, float scale, T *__restrict__ out, int64_t ldo) {
+    const int64_t total = n * per_row, step = (int64_t)gridDim.x * 256;
+    for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < total; w += step) {
+        const int64_t i = w / per_row;
+        const int c = (int)(w - i * per_row) * VEC;
+        const int64_t id = ids[i];
+        Vec<T, VEC> v;
+        if (id >= 0 && id < n_rows) {
+            v = *reinterpret_cast<const Vec<T, VEC> *>(table + id * ldt + c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(scale * to_f32(v.v[e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(0.f);
+        }
+        *reinterpret_cast<Vec<T, VEC> *>(out + i * ldo + c) = v;
+    }
+}
+
+// ---- sort ----------------------------------------------------------------------------------------------------------------
+
+constexpr int kRankMax = 16384;  // places ranked by counting
+constexpr int kTile = 2048;      // places of a radix tile (256 threads x 8)
+constexpr int kMaxBits = 9;
+
+// A place's sort key: its row, or n_rows for one that adds to nothing (such places end behind every row).
+__device__ __forceinline__ uint32_t key_of(const int64_t *ids, int64_t i, int64_t n_rows, int64_t padding) {
+    const int64_t id = ids[i];
+    return id >= 0 && id < n_rows && id != padding ? (uint32_t)id : (uint32_t)n_rows;
+}
+
+// Rank by counting: a workgroup ranks 64 places; its 16 waves count over a sixteenth of the places each, out of LDS.
+__global__ __launch_bounds__(1024) void rank_kernel(const int64_t *__restrict__ ids, int n, int64_t n_rows, int64_t padding,
+                                                    uint32_t *__restrict__ keys, uint32_t *__restrict__ places, uint32_t *count) {
+    __shared__ __align__(16) uint32_t all[kRankMax];
+    __shared__ uint32_t before[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n4 = (n + 3) & ~3;
+    for (int j = threadIdx.x; j < n4; j += 1024) all[j] = j < n ? key_of(ids, j, n_rows, padding) : 0xffffffffu;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    const int i = blockIdx.x * 64 + lane;
+    const uint32_t mine = i < n ? all[i] : 0u;
+    // places in front of i: of equal ids those before it, i.e. key <= mine for j < i and key < mine from i on
+    const int per = ((n4 / 4 + 15) / 16) * 4, j0 = min(w * per, n4), j1 = min(j0 + per, n4);
+    uint32_t r = 0;
+    for (int j = j0; j < j1; j += 4) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(all + j);
+        r += k.x < mine || (k.x == mine && j < i);
+        r += k.y < mine || (k.y == mine && j + 1 < i);
+        r += k.z < mine || (k.z == mine && j + 2 < i);
+        r += k.w < mine || (k.w == mine && j + 3 < i);
+    }
+    before[w][lane] = r;
+    __syncthreads();
+    if (w == 0 && i < n) {
+        uint32_t rank = 0;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) rank += before[q][lane];
+        keys[rank] = mine;
+        places[rank] = (uint32_t)i;
+    }
+}
+
+// Radix pass, first launch: how often each digit occurs in each tile -> hist[digit][tile].  (ids: the first pass.)
+__global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, const uint32_t *keys, int64_t n, int64_t n_rows, int64_t padding,
+                                                          int shift, int bits, uint32_t *hist, uint32_t *count) {
+    __shared__ uint32_t h[1 << kMaxBits];
+    const int bins = 1 << bits;
+    for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)blockIdx.x * kTile;
+    for (int u = 0; u < kTile / 256; ++u) {
+        const int64_t i = i0 + u * 256 + threadIdx.x;
+        if (i < n) {
+            const uint32_t k = ids ? key_of(ids, i, n_rows, padding) : keys[i];
+            atomicAdd(&h[(k >> shift) & (bins - 1)], 1u);
+        }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += 256) hist[(int64_t)d * gridDim.x + blockIdx.x] = h[d];
+}
+
+// Second launch: one workgroup per digit turns its counts into their exclusive prefix over the tiles; total[digit].
+__global__ __launch_bounds__(256) void digit_prefix_kernel(uint32_t *hist, int tiles, uint32_t *total) {
+    __shared__ uint32_t part[4];
+    uint32_t *h = hist + (int64_t)blockIdx.x * tiles;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t run = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 256) {
+        const int t = t0 + threadIdx.x;
+        const uint32_t v = t < tiles ? h[t] : 0u;
+        uint32_t x = v;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 63) part[w] = x;
+        __syncthreads();
+        uint32_t base = run;
+        for (int q = 0; q < w; ++q) base += part[q];
+        if (t < tiles) h[t] = base + x - v;
+        run += part[0] + part[1] + part[2] + part[3];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) total[blockIdx.x] = run;
+}
+
+// Third launch: every place moves to (places of smaller digits) + (of its digit in earlier tiles) + (of its digit before it here).
+__global__ __launch_bounds__(256) void digit_scatter_kernel(const int64_t *ids, const uint32_t *keys, const uint32_t *places, int64_t n,
+                                                            int64_t n_rows, int64_t padding, int shift, int bits, const uint32_t *hist,
+                                                            const uint32_t *total, uint32_t *keys_out, uint32_t *places_out) {
+    __shared__ uint32_t at[4][1 << kMaxBits];  // places of a digit in each wave's quarter, then where the next one goes
+    __shared__ uint32_t part[4];
+    const int bins = 1 << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int d = threadIdx.x; d < 4 * (1 << kMaxBits); d += 256) (&at[0][0])[d] = 0;
+    __syncthreads();
+    constexpr int R = kTile / 256;
+    const int64_t i0 = (int64_t)blockIdx.x * kTile + w * (kTile / 4);
+    uint32_t key[R], rank[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int64_t i = i0 + u * 64 + lane;
+        const bool there = i < n;
+        key[u] = there ? (ids ? key_of(ids, i, n_rows, padding) : keys[i]) : 0u;
+        const uint32_t d = (key[u] >> shift) & (bins - 1);
+        unsigned long long same = __ballot(there);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long one = __ballot((d >> b) & 1u);
+            same &= (d >> b) & 1u ? one : ~one;
+        }
+        const int ahead = __popcll(same & ((1ull << lane) - 1ull));
+        volatile uint32_t *slot = &at[w][d];
+        const uint32_t old = *slot;       // (a wave's LDS accesses are served in the order it issues them)
+        rank[u] = old + ahead;
+        if (there && ahead == 0) *slot = old + __popcll(same);
+    }
+    __syncthreads();
+    // start of each digit: exclusive prefix of the totals, two digits per thread
+    const uint32_t a = 2 * threadIdx.x < (unsigned)bins ? total[2 * threadIdx.x] : 0u;
+    const uint32_t b = 2 * threadIdx.x + 1 < (unsigned)bins ? total[2 * threadIdx.x + 1] : 0u;
+    uint32_t x = a + b;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) part[w] = x;
+    __syncthreads();
+    uint32_t first = x - a - b;
+    for (int q = 0; q < w; ++q) first += part[q];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int d = 2 * threadIdx.x + k;
+        if (d < bins) {
+            uint32_t go = (k ? first + a : first) + hist[(int64_t)d * gridDim.x + blockIdx.x];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t c = at[q][d];
+                at[q][d] = go;
+                go += c;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int64_t i = i0 + u * 64 + lane;
+        if (i < n) {
+            const uint32_t to = at[w][(key[u] >> shift) & (bins - 1)] + rank[u];
+            keys_out[to] = key[u];
+            places_out[to] = places ? places[i] : (uint32_t)i;
+        }
+    }
+}
+
+// ---- sums of runs ------------------------------------------------------------------------------------------------------
+
+struct RunArgs {
+    const void *grad;
+    int64_t ldg;
+    int64_t n, n_rows;
+    int d, chunk;              // sorted places per chunk
+    int64_t chunks;
+    const uint32_t *keys, *places;
+    float scale;
+    void *out;
+    float *part;               // [chunks][2][d]: sums of the chunk's first run and of its last, where they cross a border
+    uint32_t *list, *count;    // chunks whose last run starts there and goes on
+    int64_t run_blocks;        // the launch's workgroups that sum; the rest zero rows
+};
+
+template <class T, int VEC>
+__device__ __forceinline__ void store_row(T *p, const float (&acc)[VEC], float scale) {
+    Vec<T, VEC> v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(scale * acc[e]);
+    *reinterpret_cast<Vec<T, VEC> *>(p) = v;
+}
+
+// First place of the sorted list whose key is not below v.
+__device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t n, uint32_t v) {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (keys[mid] < v) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// G lanes x VEC elements cover a piece of a row (blockIdx.y: which piece); 256 / G chunks per workgroup.
+template <class TI, class TO, int VEC, int G>
+__global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
+    constexpr int U = 8;  // rows in flight per lane-group
+    const int sub = threadIdx.x % G, grp = threadIdx.x / G;
+    const int col = (blockIdx.y * G + sub) * VEC;
+    const bool on = col < a.d;
+    TO *out = (TO *)a.out;
+    if (blockIdx.x >= a.run_blocks) {  // zero rows: a lane-group takes the rows of its stripe that no place refers to
+        const int64_t b = blockIdx.x - a.run_blocks;
+        const int64_t r0 = b * 256;
+        const int64_t r = r0 + threadIdx.x;
+        __shared__ uint32_t empty[256];
+        bool none = false;
+        if (r < a.n_rows) {
+            const int64_t at = first_not_below(a.keys, a.n, (uint32_t)r);
+            none = at >= a.n || a.keys[at] != (uint32_t)r;
+        }
+        empty[threadIdx.x] = none;
+        __syncthreads();
+        const float zero[VEC] = {};
+        if (on)
+            for (int q = grp; q < 256; q += 256 / G)
+                if (empty[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f);
+        return;
+    }
+    const int64_t c = (int64_t)blockIdx.x * (256 / G) + grp;
+    if (c >= a.chunks) return;
+    const int64_t p0 = c * a.chunk, p1 = min(p0 + a.chunk, a.n);
+    const TI *grad = (const TI *)a.grad;
+    const uint32_t none = (uint32_t)a.n_rows;
+    const uint32_t ahead = p0 > 0 ? a.keys[p0 - 1] : 0xffffffffu;  // (no key is 2^32 - 1)
+    const uint32_t behind = p1 < a.n ? a.keys[p1] : 0xffffffffu;
+    float acc[VEC] = {};
+    uint32_t run = a.keys[p0];
+    bool first = run == ahead;  // the current run began in an earlier chunk
+    for (int64_t p = p0; p < p1; p += U) {
+        uint32_t key[U];
+        Vec<TI, VEC> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            key[u] = p + u < p1 ? a.keys[p + u] : none;
+            if (key[u] != none && on) v[u] = *reinterpret_cast<const Vec<TI, VEC> *>(grad + (int64_t)a.places[p + u] * a.ldg + col);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p + u >= p1) break;
+            if (key[u] != run) {  // the run ends here
+                if (run != none && on) {
+                    if (first) {
+                        float *to = a.part + (2 * c) * a.d + col;
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) to[e] = acc[e];
+                    } else {
+                        store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale);
+                    }
+                }
+                run = key[u];
+                first = false;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+            }
+            if (run != none && on) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += to_f32(v[u].v[e]);
+            }
+        }
+    }
+    if (run == none) return;
+    const bool goes_on = run == behind;
+    if (!first && !goes_on) {
+        if (on) store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale);
+        return;
+    }
+    if (on) {
+        float *to = a.part + (2 * c + (first ? 0 : 1)) * a.d + col;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) to[e] = acc[e];
+    }
+    if (!first && sub == 0 && blockIdx.y == 0) a.list[atomicAdd(a.count, 1u)] = (uint32_t)c;  // (the list's order changes no sum)
+}
+
+// Runs over several chunks: the last sum of the chunk they start in, then the first sums of the chunks they reach into.
+template <class TO, int VEC, int G>
+__global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
+    constexpr int N = 256 / G;
+    __shared__ float sums[256 * VEC];
+    const int sub = threadIdx.x % G, grp = threadIdx.x / G;
+    const int col = (blockIdx.y * G + sub) * VEC;
+    const bool on = col < a.d;
+    const uint32_t todo = *a.count;
+    for (uint32_t t = blockIdx.x; t < todo; t += gridDim.x) {
+        const int64_t c = a.list[t];
+        const uint32_t key = a.keys[(c + 1) * a.chunk];
+        const int64_t end = first_not_below(a.keys, a.n, key + 1u);
+        const int64_t last = (end - 1) / a.chunk;  // the chunk it ends in
+        // parts c, c + 1, .., last: an equal piece for each lane-group, the pieces joined in order
+        const int64_t cnt = last - c + 1, per = (cnt + N - 1) / N;
+        const int64_t q0 = c + grp * per, q1 = min(q0 + per, last + 1);
+        float acc[VEC] = {};
+        if (on) {
+#pragma unroll 4
+            for (int64_t q = q0; q < q1; ++q) {
+                const float *from = a.part + (2 * q + (q == c ? 1 : 0)) * a.d + col;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += from[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sums[threadIdx.x * VEC + e] = acc[e];
+        __syncthreads();
+        if (grp == 0 && on) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+            for (int q = 0; q < N; ++q)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += sums[(q * G + sub) * VEC + e];
+            store_row<TO, VEC>((TO *)a.out + (int64_t)key * a.d + col, acc, a.scale);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+
+static int64_t round16e(int64_t b) { return (b + 15) & ~int64_t(15); }
+
+// Sorted places per chunk: enough chunks for eight waves per SIMD where the places allow it, 64 places at most (long runs leave few parts).
+static int chunk_of(int64_t n, int d) {
+    const int64_t want = n * std::max(1, d / 8) / (64 * 4096);
+    return want <= 8 ? 8 : want >= 64 ? 64 : (int)want / 8 * 8;
+}
+
+struct Layout {
+    int64_t keys, places, keys2, places2, hist, total, part, list, count, bytes;
+    int chunk, tiles;
+    int64_t chunks;
+};
+
+static Layout layout_of(int64_t n, int d) {
+    Layout l{};
+    l.chunk = chunk_of(n, d);
+    l.chunks = (n + l.chunk - 1) / l.chunk;
+    l.tiles = (int)((n + kTile - 1) / kTile);
+    int64_t at = 0;
+    auto take = [&](int64_t b) {
+        const int64_t r = at;
+        at += round16e(b);
+        return r;
+    };
+    l.count = take(16);
+    l.keys = take(4 * n), l.places = take(4 * n);
+    if (n > kRankMax) {
+        l.keys2 = take(4 * n), l.places2 = take(4 * n);
+        l.hist = take(4ll * (1 << kMaxBits) * l.tiles);
+        l.total = take(4 << kMaxBits);
+    }
+    l.list = take(4 * l.chunks);
+    l.part = take(4ll * 2 * l.chunks * d);
+    l.bytes = at;
+    return l;
+}
+
+template <class TI, class TO, int VEC, int G>
+static void launch_runs(const RunArgs &a0, hipStream_t s) {
+    RunArgs a = a0;
+    a.run_blocks = (a.chunks + 256 / G - 1) / (256 / G);
+    const unsigned pieces = (unsigned)((a.d + G * VEC - 1) / (G * VEC));
+    const int64_t zero_blocks = (a.n_rows + 255) / 256;
+    hipLaunchKernelGGL((run_sum_kernel<TI, TO, VEC, G>), dim3((unsigned)(a.run_blocks + zero_blocks), pieces), dim3(256), 0, s, a);
+    if (a.chunks > 1)
+        hipLaunchKernelGGL((run_join_kernel<TO, VEC, G>), dim3((unsigned)std::min<int64_t>(a.chunks, 1024), pieces), dim3(256), 0, s, a);
+}
+
+template <class TI, class TO>
+static int launch_runs_of(const RunArgs &a, bool wide, hipStream_t s) {
+    constexpr int VEC = 16 / (int)sizeof(TI);
+    const int lanes = wide ? a.d / VEC : a.d;
+    if (wide) {
+        if (lanes <= 4) launch_runs<TI, TO, VEC, 4>(a, s);
+        else if (lanes <= 8) launch_runs<TI, TO, VEC, 8>(a, s);
+        else if (lanes <= 16) launch_runs<TI, TO, VEC, 16>(a, s);
+        else if (lanes <= 32) launch_runs<TI, TO, VEC, 32>(a, s);
+        else launch_runs<TI, TO, VEC, 64>(a, s);
+    } else {
+        if (lanes <= 4) launch_runs<TI, TO, 1, 4>(a, s);
+        else if (lanes <= 16) launch_runs<TI, TO, 1, 16>(a, s);
+        else launch_runs<TI, TO, 1, 64>(a, s);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+static int check_places(int64_t n, int64_t n_rows, int d) {
+    if (n < 0 || n_rows < 0 || d <= 0) return fail(RBG_ESHAPE, "n = %lld, n_rows = %lld, d = %d", (long long)n, (long long)n_rows, d);
+    if (n >= 0x7fff0000ll || n_rows >= 0x7fffffffll || d > 1 << 20)
+        return fail(RBG_EUNSUPPORTED, "ids or rows beyond 2^31, or d beyond 2^20: n = %lld, n_rows = %lld, d = %d", (long long)n, (long long)n_rows, d);
+    return RBG_OK;
+}
+
+}  // namespace rbg
+
+using namespace rbg;
+
+extern "C" {
+
+int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dtype, const int64_t *ids, int64_t n, float scale, void *out,
+                  int64_t ldo, void *stream) {
+    clear_error();
+    if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
+    if (n < 0 || n_rows < 0 || d <= 0 || ldt < d || ldo < d)
+        return fail(RBG_ESHAPE, "n = %lld, n_rows = %lld, d = %d, ldt = %lld, ldo = %lld", (long long)n, (long long)n_rows, d, (long long)ldt, (long long)ldo);
+    if (n == 0) return RBG_OK;
+    if ((n_rows && !table) || !ids || !out) return fail(RBG_EINVAL, "NULL pointer");
+    const int size = elem_size(dtype);
+    if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) % size) return fail(RBG_EINVAL, "a table is not aligned to its type");
+    const bool wide = on_16(table) && on_16(out) && d * size % 16 == 0 && ldt * size % 16 == 0 && ldo * size % 16 == 0;
+    return with_elem(dtype, [&](auto t) {
+        typedef decltype(t) E;
+        constexpr int VEC = 16 / (int)sizeof(E);
+        const int per_row = wide ? d / VEC : d;
+        const unsigned grid = (unsigned)std::min<int64_t>((n * per_row + 255) / 256, 16384);
+        if (wide)
+            hipLaunchKernelGGL((lookup_kernel<E, VEC>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n,
+                               per_row, scale, (E *)out, ldo);
+        else
+            hipLaunchKernelGGL((lookup_kernel<E, 1>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n,
+                               per_row, scale, (E *)out, ldo);
+        RBG_HIP(hipGetLastError());
+        return (int)RBG_OK;
+    });
+}
+
+int rbg_embedding_grad_workspace(int64_t n, int64_t n_rows, int d, int64_t *bytes) {
+    clear_error();
+    if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
+    if (int rc = check_places(n, n_rows, d)) return rc;
+    *bytes = layout_of(n, d).bytes;
+    return RBG_OK;
+}
+
+int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *ids, int64_t n, int64_t n_rows, int d, float scale,
+                       int64_t padding_idx, void *out, int out_dtype, void *workspace, void *stream) {
+    clear_error();
+    if (!elem_ok(dtype) || (out_dtype != dtype && out_dtype != RBG_F32)) return fail(RBG_EINVAL, "dtype = %d, out_dtype = %d", dtype, out_dtype);
+    if (int rc = check_places(n, n_rows, d)) return rc;
+    if (ldg < d) return fail(RBG_ESHAPE, "d = %d, ldg = %lld", d, (long long)ldg);
+    if (n_rows == 0) return RBG_OK;
+    if ((n && (!grad || !ids)) || !out || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
+    const int size = elem_size(dtype), out_size = elem_size(out_dtype);
+    if (reinterpret_cast<uintptr_t>(grad) % size || reinterpret_cast<uintptr_t>(out) % out_size) return fail(RBG_EINVAL, "a tensor is not aligned to its type");
+    hipStream_t s = (hipStream_t)stream;
+    const Layout l = layout_of(n, d);
+    char *w = (char *)workspace;
+    uint32_t *count = (uint32_t *)(w + l.count);
+    uint32_t *keys = (uint32_t *)(w + l.keys), *places = (uint32_t *)(w + l.places);
+    if (n > 0 && n <= kRankMax) {
+        hipLaunchKernelGGL(rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+    } else if (n > 0) {
+        int bits = 1;
+        while (((int64_t)1 << bits) <= n_rows) ++bits;  // keys 0 .. n_rows
+        const int passes = (bits + kMaxBits - 1) / kMaxBits, width = (bits + passes - 1) / passes;
+        uint32_t *k2 = (uint32_t *)(w + l.keys2), *p2 = (uint32_t *)(w + l.places2);
+        uint32_t *hist = (uint32_t *)(w + l.hist), *total = (uint32_t *)(w + l.total);
+        const uint32_t *from_k = nullptr, *from_p = nullptr;
+        // the last pass ends in (keys, places)
+        uint32_t *to_k = passes & 1 ? keys : k2, *to_p = passes & 1 ? places : p2;
+        for (int q = 0; q < passes; ++q) {
+            const int64_t *src = q == 0 ? ids : nullptr;
+            hipLaunchKernelGGL(digit_count_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
+            hipLaunchKernelGGL(digit_prefix_kernel, dim3(1u << width), dim3(256), 0, s, hist, l.tiles, total);
+            hipLaunchKernelGGL(digit_scatter_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
+                               hist, total, to_k, to_p);
+            from_k = to_k, from_p = to_p;
+            to_k = to_k == keys ? k2 : keys, to_p = to_p == places ? p2 : places;
+        }
+    }
+    RBG_HIP(hipGetLastError());
+    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0};
+    const bool wide = on_16(grad) && reinterpret_cast<uintptr_t>(out) % (16 / size * out_size) == 0 && d * size % 16 == 0 && ldg * size % 16 == 0;
+    return with_elem(dtype, [&](auto t) {
+        typedef decltype(t) E;
+        return out_dtype == dtype ? launch_runs_of<E, E>(a, wide, s) : launch_runs_of<E, float>(a, wide, s);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,839 @@
+// logits.hip — losses on whole rows of logits: distillation from a teacher's top list, log-probabilities of targets, and the
+// preference loss on pairs of packed sequences, each with its gradient.
+//
+// Mathematics.  With m = max_j z_j, c = log2(e) / T and e_j = 2^((z_j - m) c), S = sum_j e_j, a row's softmax is q_j = e_j / S and
+// log q_j = (z_j - m) / T - ln S.  (z - m is formed before it is scaled: a row whose logits all hold the type's lowest value is a
+// uniform row, not a difference of overflows.)  (m, S) is all a gradient needs; a row of nothing but -inf has m = -inf, S = 0.
+// Every gradient here is a e_j plus a few sparse terms: the teacher's entries, or the target.
+//
+// What bounds it.  The rows are read from and written to HBM and nothing else is large: 16 bytes per lane and request, a row's
+// elements in front of and behind its 16-byte boundaries one by one (rows of an odd length start anywhere).  Value and gradient of
+// the distillation in one call keep the row in registers between the two: one read, one write.  The preference loss needs
+// every token of a pair before any gradient of it, so its rows are read twice.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "vocab_common.h"
+
+namespace rbg {
+
+constexpr int kMaxEntries = 256;  // of a teacher's list
+
+// A row of V elements as 16-byte chunks: `head` elements, then nb chunks, then the rest; x-th of the `extra` loose elements = at(x).
+template <class T>
+struct RowShape {
+    static constexpr int E = 16 / (int)sizeof(T);
+    int head, nb, extra, tail;
+    __device__ __forceinline__ RowShape(const T *p, int V) {
+        const int off = (int)((16u - (unsigned)(reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / (int)sizeof(T);
+        head = min(off, V);
+        nb = (V - head) / E;
+        tail = head + nb * E;
+        extra = head + (V - tail);
+    }
+    __device__ __forceinline__ int at(int x) const { return x < head ? x : tail + (x - head); }
+};
+
+struct MaxSum {
+    float m, s;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// (m, s) of two parts of a row.  A part of nothing but -inf is (-inf, 0); NaN stays in s.
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return {m, a.s + b.s};
+    return {m, a.s * exp2_fast((a.m - m) * c) + b.s * exp2_fast((b.m - m) * c)};
+}
+
+__device__ __forceinline__ MaxSum wave_join(MaxSum v, float c) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = join(v, MaxSum{__shfl_xor(v.m, o), __shfl_xor(v.s, o)}, c);
+    return v;
+}
+
+// Over a workgroup of TH threads; every thread gets the result.  `sh`: TH / 64 entries of LDS nobody else uses meanwhile.
+template <int TH>
+__device__ __forceinline__ MaxSum block_join(MaxSum v, float c, MaxSum *sh) {
+    v = wave_join(v, c);
+    if constexpr (TH > kWave) {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        if (lane == 0) sh[w] = v;
+        __syncthreads();
+        v = sh[0];
+#pragma unroll
+        for (int i = 1; i < TH / kWave; ++i) v = join(v, sh[i], c);
+    }
+    return v;
+}
+
+// The running (m, s) of one thread over U chunks at a time: one rescaling for U E elements.
+template <class T, int N>
+__device__ __forceinline__ void online(MaxSum &r, const float (&x)[N], float c) {
+    float m = r.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    const float mm = m == -INFINITY ? 0.f : m;
+    float s = r.s * exp2_fast((r.m - mm) * c);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += exp2_fast((x[i] - mm) * c);
+    r.m = m;
+    r.s = s;
+}
+
+// (m, s) of chunks [c0, c1) of a row, and of its loose elements when `loose`, over the threads of a workgroup.
+template <class T, int TH, int U>
+__device__ __forceinline__ MaxSum scan_row(const T *__restrict__ z, const RowShape<T> &sh, int c0, int c1, bool loose, float c) {
+    constexpr int E = RowShape<T>::E;
+    const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + sh.head);
+    MaxSum r{-INFINITY, 0.f};
+    int i = c0 + threadIdx.x;
+    for (; i + (U - 1) * TH < c1; i += U * TH) {
+        Vec<T, E> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = body[i + u * TH];
+        float x[U * E];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u * E + e] = to_f32(v[u].v[e]);
+        online<T>(r, x, c);
+    }
+    for (; i < c1; i += TH) {
+        const Vec<T, E> v = body[i];
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f32(v.v[e]);
+        online<T>(r, x, c);
+    }
+    if (loose && (int)threadIdx.x < sh.extra) {
+        const float x[1] = {to_f32(z[sh.at(threadIdx.x)])};
+        online<T>(r, x, c);
+    }
+    return r;
+}
+
+// g_j = a 2^((z_j - m) c) over chunks [c0, c1) (and the loose elements); element `hot` (or -1) gets `more` on top, before the rounding.
+// z and g may be the same row: an element is read and written by the same thread.
+template <class T, int TH, int U>
+__device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &sh, int c0, int c1, bool loose, float m, float c, float a,
+                                          int hot, float more) {
+    constexpr int E = RowShape<T>::E;
+    const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + sh.head);
+    Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
+    const bool wide = on_16_dev(out);
+    const int hb = hot - sh.head;
+    const int hc = hot >= sh.head && hot < sh.tail ? hb / E : -1, he = hb - hc * E;
+    for (int i0 = c0; i0 < c1; i0 += U * TH) {
+        Vec<T, E> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * TH + threadIdx.x;
+            if (i < c1) v[u] = body[i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * TH + threadIdx.x;
+            if (i >= c1) break;
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = a * exp2_fast((to_f32(v[u].v[e]) - m) * c);
+            if (i == hc) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] += e == he ? more : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u].v[e] = from_f32<T>(x[e]);
+            if (wide) {
+                out[i] = v[u];
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v[u].v[e];
+            }
+        }
+    }
+    if (loose && (int)threadIdx.x < sh.extra) {
+        const int j = sh.at(threadIdx.x);
+        float x = a * exp2_fast((to_f32(z[j]) - m) * c);
+        if (j == hot) x += more;
+        g[j] = from_f32<T>(x);
+    }
+}
+
+template <class T, int TH>
+__device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, int c1, bool loose) {
+    constexpr int E = RowShape<T>::E;
+    Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
+    const bool wide = on_16_dev(out);
+    Vec<T, E> v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(0.f);
+    for (int i = c0 + threadIdx.x; i < c1; i += TH) {
+        if (wide) {
+            out[i] = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v.v[e];
+        }
+    }
+    if (loose && (int)threadIdx.x < sh.extra) g[sh.at(threadIdx.x)] = from_f32<T>(0.f);
+}
+
+// Part s of S of a row's chunks.
+__device__ __forceinline__ void part_of(int nb, int s, int S, int &c0, int &c1) {
+    c0 = (int)((int64_t)nb * s / S);
+    c1 = (int)((int64_t)nb * (s + 1) / S);
+}
+
+// ---- distillation --------------------------------------------------------------------------------------------------------
+
+struct DistillArgs {
+    const void *z;
+    int64_t ldz;
+    int V, k;
+    const int64_t *idx;
+    const float *val;
+    float c, T;  // log2(e) / T
+    const float *row_w;
+    float *loss, *stats;
+    void *grad;
+    int64_t ldg;
+    MaxSum *part;  // [n][S] when a row is split
+    float *zt;     // [n][k] when a row is split: the entries' logits (the gradient may overwrite them)
+};
+
+struct Entries {
+    int idx[kMaxEntries];    // -1: none
+    float p[kMaxEntries];    // teacher's probability
+    float z[kMaxEntries];    // student's logit there
+    float any;               // 0: a row without entries
+    MaxSum red[16];
+};
+
+// Wave 0 fills the list: probabilities over the entries that are there.  Ends without a barrier.
+template <class T>
+__device__ __forceinline__ void load_entries(const DistillArgs &a, int64_t row, const T *z, const float *zt, Entries &sh) {
+    if (threadIdx.x >= kWave) return;
+    float v[kMaxEntries / kWave];
+    float tm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kMaxEntries / kWave; ++u) {
+        const int i = u * kWave + threadIdx.x;
+        v[u] = -INFINITY;
+        if (i < a.k) {
+            const int64_t j = a.idx[row * a.k + i];
+            const bool there = j >= 0 && j < a.V;
+            sh.idx[i] = there ? (int)j : -1;
+            sh.z[i] = there ? (zt ? zt[row * a.k + i] : to_f32(z[j])) : 0.f;
+            if (there) v[u] = a.val[row * a.k + i];
+            tm = fmaxf(tm, v[u]);
+        }
+    }
+    tm = wave_max(tm);
+    const float tmm = tm == -INFINITY ? 0.f : tm;
+    float s = 0.f;
+#pragma unroll
+    for (int u = 0; u < kMaxEntries / kWave; ++u) {
+        v[u] = exp2_fast((v[u] - tmm) * a.c);
+        s += v[u];
+    }
+    s = wave_sum(s);
+#pragma unroll
+    for (int u = 0; u < kMaxEntries / kWave; ++u) {
+        const int i = u * kWave + threadIdx.x;
+        if (i < a.k) sh.p[i] = s == 0.f ? 0.f : v[u] / s;
+    }
+    if (threadIdx.x == 0) sh.any = s;
+}
+
+__device__ __forceinline__ bool distill_empty(const Entries &sh, MaxSum st) { return sh.any == 0.f || (st.m == -INFINITY && st.s == 0.f); }
+
+// Wave 0: the row's loss from its list.  The teacher's log-probabilities are taken of the rounded p: p (log p - log q) is then the
+// divergence of the p that the gradient uses.
+__device__ __forceinline__ void entries_loss(const DistillArgs &a, int64_t row, const Entries &sh, MaxSum st) {
+    if (threadIdx.x >= kWave) return;
+    const float lns = logf(st.s), inv_t = 1.f / a.T;
+    float l = 0.f;
+    for (int i = threadIdx.x; i < a.k; i += kWave)
+        if (sh.idx[i] >= 0 && sh.p[i] != 0.f) l += sh.p[i] * (logf(sh.p[i]) - ((sh.z[i] - st.m) * inv_t - lns));
+    l = wave_sum(l);
+    if (threadIdx.x == 0) {
+        if (a.loss) a.loss[row] = distill_empty(sh, st) ? 0.f : a.T * a.T * l;
+        if (a.stats) a.stats[2 * row] = st.m, a.stats[2 * row + 1] = st.s;
+    }
+}
+
+// The entries' elements of the gradient, over what write_row stored there (a barrier lies between): w T (q - sum of p).  The first
+// entry of an index writes it.  Only elements that part [c0, c1) (+ loose) of the row owns.
+template <class T, int TH>
+__device__ __forceinline__ void fix_entries(const DistillArgs &a, T *g, const RowShape<T> &rs, int c0, int c1, bool loose, const Entries &sh,
+                                            MaxSum st, float w) {
+    for (int i = threadIdx.x; i < a.k; i += TH) {
+        const int j = sh.idx[i];
+        if (j < 0) continue;
+        const int b = j - rs.head;
+        const bool in_body = b >= 0 && j < rs.tail;
+        if (in_body ? (b / RowShape<T>::E < c0 || b / RowShape<T>::E >= c1) : !loose) continue;
+        float p = 0.f;
+        bool first = true;
+        for (int t = 0; t < a.k; ++t) {
+            if (sh.idx[t] != j) continue;
+            p += sh.p[t];
+            first &= t >= i;
+        }
+        if (first) g[j] = from_f32<T>(w * a.T * (exp2_fast((sh.z[i] - st.m) * a.c) / st.s - p));
+    }
+}
+
+// The loss alone: one workgroup streams a row.
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void distill_eval_kernel(const DistillArgs a) {
+    __shared__ Entries sh;
+    const int64_t row = blockIdx.x;
+    const T *z = (const T *)a.z + row * a.ldz;
+    const RowShape<T> rs(z, a.V);
+    load_entries(a, row, z, nullptr, sh);
+    const MaxSum st = block_join<TH>(scan_row<T, TH, 4>(z, rs, 0, rs.nb, true, a.c), a.c, sh.red);
+    __syncthreads();
+    entries_loss(a, row, sh, st);
+}
+
+// Value and gradient of a row that fits the registers of its workgroup: NC chunks of 16 bytes per thread.
+template <class T, int TH, int NC>
+__global__ __launch_bounds__(TH, NC <= 8 ? 8 : 4) void distill_row_kernel(const DistillArgs a) {
+    constexpr int E = RowShape<T>::E;
+    __shared__ Entries sh;
+    const int64_t row = blockIdx.x;
+    const T *z = (const T *)a.z + row * a.ldz;
+    T *g = (T *)a.grad + row * a.ldg;
+    const RowShape<T> rs(z, a.V);
+    const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + rs.head);
+    Vec<T, E> v[NC];
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+        const int i = u * TH + threadIdx.x;
+        if (i < rs.nb) v[u] = body[i];
+    }
+    const bool has_loose = (int)threadIdx.x < rs.extra;
+    const float loose = has_loose ? to_f32(z[rs.at(threadIdx.x)]) : -INFINITY;
+    load_entries(a, row, z, nullptr, sh);
+    MaxSum r{loose, 0.f};
+#pragma unroll
+    for (int u = 0; u < NC; ++u)
+        if (u * TH + (int)threadIdx.x < rs.nb)
+#pragma unroll
+            for (int e = 0; e < E; ++e) r.m = fmaxf(r.m, to_f32(v[u].v[e]));
+    const float mm = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll
+    for (int u = 0; u < NC; ++u)
+        if (u * TH + (int)threadIdx.x < rs.nb)
+#pragma unroll
+            for (int e = 0; e < E; ++e) r.s += exp2_fast((to_f32(v[u].v[e]) - mm) * a.c);
+    if (has_loose) r.s += exp2_fast((loose - mm) * a.c);
+    const MaxSum st = block_join<TH>(r, a.c, sh.red);
+    __syncthreads();
+    entries_loss(a, row, sh, st);
+    if (distill_empty(sh, st)) {
+        zero_row<T, TH>(g, rs, 0, rs.nb, true);
+        return;
+    }
+    const float w = a.row_w ? a.row_w[row] : 1.f;
+    const float s = w * a.T / st.s;
+    Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + rs.head);
+    const bool wide = on_16_dev(out);
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+        const int i = u * TH + threadIdx.x;
+        if (i >= rs.nb) break;
+        Vec<T, E> o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(s * exp2_fast((to_f32(v[u].v[e]) - st.m) * a.c));
+        if (wide) {
+            out[i] = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) g[rs.head + i * E + e] = o.v[e];
+        }
+    }
+    if (has_loose) g[rs.at(threadIdx.x)] = from_f32<T>(s * exp2_fast((loose - st.m) * a.c));
+    __syncthreads();
+    fix_entries<T, TH>(a, g, rs, 0, rs.nb, true, sh, st, w);
+}
+
+// Rows longer than that: the row is read twice, the second time out of the caches where they hold it.
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void distill_long_kernel(const DistillArgs a) {
+    __shared__ Entries sh;
+    const int64_t row = blockIdx.x;
+    const T *z = (const T *)a.z + row * a.ldz;
+    T *g = (T *)a.grad + row * a.ldg;
+    const RowShape<T> rs(z, a.V);
+    load_entries(a, row, z, nullptr, sh);
+    const MaxSum st = block_join<TH>(scan_row<T, TH, 4>(z, rs, 0, rs.nb, true, a.c), a.c, sh.red);
+    __syncthreads();
+    entries_loss(a, row, sh, st);
+    if (distill_empty(sh, st)) {
+        zero_row<T, TH>(g, rs, 0, rs.nb, true);
+        return;
+    }
+    const float w = a.row_w ? a.row_w[row] : 1.f;
+    write_row<T, TH, 4>(z, g, rs, 0, rs.nb, true, st.m, a.c, w * a.T / st.s, -1, 0.f);
+    __syncthreads();
+    fix_entries<T, TH>(a, g, rs, 0, rs.nb, true, sh, st, w);
+}
+
+// Few rows: S workgroups share one.  First launch: (m, s) of each part; part 0 keeps the entries' logits.
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void distill_part_kernel(const DistillArgs a) {
+    __shared__ MaxSum red[TH / kWave];
+    const int64_t row = blockIdx.y;
+    const T *z = (const T *)a.z + row * a.ldz;
+    const RowShape<T> rs(z, a.V);
+    int c0, c1;
+    part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
+    const MaxSum st = block_join<TH>(scan_row<T, TH, 4>(z, rs, c0, c1, blockIdx.x == 0, a.c), a.c, red);
+    if (threadIdx.x == 0) a.part[row * gridDim.x + blockIdx.x] = st;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.k; i += TH) {
+            const int64_t j = a.idx[row * a.k + i];
+            a.zt[row * a.k + i] = j >= 0 && j < a.V ? to_f32(z[j]) : 0.f;
+        }
+}
+
+// The parts of a row, joined in their order by every wave.
+__device__ __forceinline__ MaxSum join_parts(const MaxSum *part, int S, float c) {
+    const int lane = threadIdx.x & 63;
+    MaxSum v{-INFINITY, 0.f};
+    if (lane < S) v = part[lane];  // S <= 64
+    return wave_join(v, c);
+}
+
+// Second launch: a part's gradient.  Also the backward form, from (m, s) of an earlier call.
+template <class T, int TH, bool PARTS>
+__global__ __launch_bounds__(TH) void distill_grad_kernel(const DistillArgs a) {
+    __shared__ Entries sh;
+    const int64_t row = blockIdx.y;
+    const T *z = (const T *)a.z + row * a.ldz;
+    T *g = (T *)a.grad + row * a.ldg;
+    const RowShape<T> rs(z, a.V);
+    load_entries(a, row, z, PARTS ? a.zt : nullptr, sh);
+    MaxSum st;
+    if constexpr (PARTS) st = join_parts(a.part + row * gridDim.x, gridDim.x, a.c);
+    else st = MaxSum{a.stats[2 * row], a.stats[2 * row + 1]};
+    __syncthreads();
+    if constexpr (PARTS)
+        if (blockIdx.x == 0) entries_loss(a, row, sh, st);
+    if (!a.grad) return;
+    int c0, c1;
+    part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
+    const bool loose = blockIdx.x == 0;
+    if (distill_empty(sh, st)) {
+        zero_row<T, TH>(g, rs, c0, c1, loose);
+        return;
+    }
+    const float w = a.row_w ? a.row_w[row] : 1.f;
+    write_row<T, TH, 4>(z, g, rs, c0, c1, loose, st.m, a.c, w * a.T / st.s, -1, 0.f);
+    __syncthreads();
+    fix_entries<T, TH>(a, g, rs, c0, c1, loose, sh, st, w);
+}
+
+// ---- log-probabilities of targets and the preference loss ---------------------------------------------------------------
+
+struct LogpArgs {
+    const void *z;
+    int64_t ldz;
+    int V;
+    const int64_t *targets;
+    float *logp;         // either
+    double *logp64;      // or
+    float *coef;         // set to 0 when given
+    float *stats;        // [m][2]
+    MaxSum *part;        // [m][S] when a row is split
+};
+
+__device__ __forceinline__ void store_logp(const LogpArgs &a, int64_t row, bool there, float zt, MaxSum st) {
+    double l = 0.0;
+    if (there && !(st.m == -INFINITY && st.s == 0.f)) l = ((double)zt - (double)st.m) - log((double)st.s);
+    if (a.logp) a.logp[row] = (float)l;
+    if (a.logp64) a.logp64[row] = l;
+    if (a.coef) a.coef[row] = 0.f;
+    if (a.stats) a.stats[2 * row] = st.m, a.stats[2 * row + 1] = st.s;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// One workgroup per row and part; a row without a target is not read.
+template <class T, int TH, bool PARTS>
+__global__ __launch_bounds__(TH) void logp_kernel(const LogpArgs a) {
+    __shared__ MaxSum red[TH / kWave];
+    const int64_t row = PARTS ? blockIdx.y : blockIdx.x;
+    const int64_t t = a.targets[row];
+    const bool there = t >= 0 && t < a.V;
+    const T *z = (const T *)a.z + row * a.ldz;
+    MaxSum st{-INFINITY, 0.f};
+    if (there) {
+        const RowShape<T> rs(z, a.V);
+        int c0 = 0, c1 = rs.nb;
+        if constexpr (PARTS) part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
+        st = block_join<TH>(scan_row<T, TH, 4>(z, rs, c0, c1, !PARTS || blockIdx.x == 0, kLog2e), kLog2e, red);
+    }
+    if (threadIdx.x) return;
+    if constexpr (PARTS) a.part[row * gridDim.x + blockIdx.x] = st;
+    else store_logp(a, row, there, there ? to_f32(z[t]) : 0.f, st);
+}
+
+template <class T>
+__global__ __launch_bounds__(kWave) void logp_join_kernel(const LogpArgs a, int S) {
+    const int64_t row = blockIdx.x;
+    const int64_t t = a.targets[row];
+    const bool there = t >= 0 && t < a.V;
+    const MaxSum st = join_parts(a.part + row * S, S, kLog2e);
+    if (threadIdx.x == 0) store_logp(a, row, there, there ? to_f32(((const T *)a.z + row * a.ldz)[t]) : 0.f, st);
+}
+
+// grad = row_g (onehot - softmax), one workgroup per row and part; row = the last one first: what the pass before read last is
+// what the caches still hold.
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void logp_grad_kernel(const void *zv, int64_t ldz, int V, const int64_t *targets, const float *stats,
+                                                       const float *row_g, void *gv, int64_t ldg) {
+    const int64_t row = (int64_t)gridDim.y - 1 - blockIdx.y;
+    const int64_t t = targets[row];
+    const T *z = (const T *)zv + row * ldz;
+    T *g = (T *)gv + row * ldg;
+    const RowShape<T> rs(z, V);
+    int c0, c1;
+    part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
+    const bool loose = blockIdx.x == 0;
+    const float m = stats[2 * row], s = stats[2 * row + 1], w = row_g[row];
+    if (t < 0 || t >= V || (m == -INFINITY && s == 0.f) || w == 0.f) zero_row<T, TH>(g, rs, c0, c1, loose);
+    else write_row<T, TH, 4>(z, g, rs, c0, c1, loose, m, kLog2e, -w / s, (int)t, w);
+}
+
+__device__ __forceinline__ float sigmoid_d(float h, float smoothing) {  // d loss / d margin
+    return smoothing / (1.f + expf(-h)) - (1.f - smoothing) / (1.f + expf(h));
+}
+
+__device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_t m, int64_t &lo, int64_t &hi) {
+    lo = offsets[s], hi = offsets[s + 1];
+    lo = lo < 0 ? 0 : lo > m ? m : lo;
+    hi = hi < lo ? lo : hi > m ? m : hi;
+}
+
+// One workgroup per pair: both sums in 64 bits, the loss, and (COEF) the tokens' gradients of pair_w loss.
+template <class L, bool COEF>
+__global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, const int64_t *offsets, const float *ref, float beta,
+                                                   float smoothing, const float *pair_w, float *loss, float *margin, float *coef) {
+    __shared__ double red[2][4];
+    const int64_t i = blockIdx.x;
+    int64_t lo[2], hi[2];
+    double sum[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        seq_of(offsets, 2 * i + k, m, lo[k], hi[k]);
+        double v = 0.0;
+        for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) v += (double)logp[t];
+        v = wave_sum(v);
+        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) sum[k] = ((red[k][0] + red[k][1]) + (red[k][2] + red[k][3])) - (double)ref[2 * i + k];
+    const float h = (float)((double)beta * (sum[0] - sum[1]));
+    if (threadIdx.x == 0) {
+        // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)); a term of weight 0 is left out (its value may be infinite)
+        const float l = log1pf(expf(-fabsf(h)));
+        float v = 0.f;
+        if (smoothing < 1.f) v += (1.f - smoothing) * (fmaxf(-h, 0.f) + l);
+        if (smoothing > 0.f) v += smoothing * (fmaxf(h, 0.f) + l);
+        if (h != h) v = h;
+        loss[i] = v;
+        margin[i] = h;
+    }
+    if constexpr (COEF) {
+        const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) coef[t] = k ? -d : d;
+    }
+}
+
+// grad_logp of every token: its sequence is found by bisection (the last one that begins at or before it and is not empty).
+__global__ __launch_bounds__(256) void pair_grad_kernel(const float *margin, int64_t m, const int64_t *offsets, int64_t pairs, float beta,
+                                                        float smoothing, const float *g_loss, const float *g_margin, float *grad) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= m) return;
+    int64_t lo = 0, hi = 2 * pairs;  // offsets[lo] <= t < offsets[hi], if t is in a sequence
+    float v = 0.f;
+    if (offsets[0] <= t && t < offsets[hi]) {
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (offsets[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        const int64_t i = lo >> 1;
+        if (g_loss) v += g_loss[i] * sigmoid_d(margin[i], smoothing);
+        if (g_margin) v += g_margin[i];
+        v *= lo & 1 ? -beta : beta;
+    }
+    grad[t] = v;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+
+// How many workgroups share a row: one where the rows alone give every CU two; else enough for about four per CU, of at least 4 096
+// elements each.  (64 parts at most: one wave joins them.)
+static int row_parts(int64_t n, int64_t V) {
+    if (n >= 512) return 1;
+    const int64_t want = std::min<int64_t>((1024 + n - 1) / std::max<int64_t>(n, 1), V / 4096);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
+}
+
+static int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
+
+// Workgroups per row of a pass that needs nothing from the rest of the row: 256 threads x 4 chunks each.
+static int grad_parts(int64_t V, int elem) { return (int)std::max<int64_t>(1, std::min<int64_t>((V * elem + 16383) / 16384, 1024)); }
+
+static int check_rows(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V) {
+    if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
+    if (n < 0 || V <= 0 || ldz < V) return fail(RBG_ESHAPE, "n = %lld, V = %lld, ldz = %lld", (long long)n, (long long)V, (long long)ldz);
+    if (V > 0x7fffff00ll || n > 0x7fffffffll) return fail(RBG_EUNSUPPORTED, "rows or columns beyond 2^31");
+    if (n && !z) return fail(RBG_EINVAL, "NULL pointer");
+    if (reinterpret_cast<uintptr_t>(z) % elem_size(dtype)) return fail(RBG_EINVAL, "logits are not aligned to their type");
+    return RBG_OK;
+}
+
+// A gradient is written to rows of its own or, element for element, to the rows it is computed from.
+static int check_grad(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V, const void *g, int64_t ldg) {
+    if (ldg < V) return fail(RBG_ESHAPE, "V = %lld, ldg = %lld", (long long)V, (long long)ldg);
+    if (reinterpret_cast<uintptr_t>(g) % elem_size(dtype)) return fail(RBG_EINVAL, "the gradient is not aligned to its type");
+    if (g == z) return ldg == ldz ? RBG_OK : fail(RBG_EINVAL, "a gradient in place of the logits needs their row stride");
+    const uintptr_t z0 = (uintptr_t)z, g0 = (uintptr_t)g;
+    const uintptr_t z1 = z0 + (uintptr_t)((n - 1) * ldz + V) * elem_size(dtype), g1 = g0 + (uintptr_t)((n - 1) * ldg + V) * elem_size(dtype);
+    if (z0 < g1 && g0 < z1) return fail(RBG_EINVAL, "the gradient overlaps the logits");
+    return RBG_OK;
+}
+
+template <class T>
+static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, hipStream_t s) {
+    const int S = row_parts(n, V);
+    if (S > 1) {
+        hipLaunchKernelGGL((distill_part_kernel<T, 256>), dim3(S, (unsigned)n), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((distill_grad_kernel<T, 256, true>), dim3(S, (unsigned)n), dim3(256), 0, s, a);
+    } else if (!a.grad) {
+        if (V * (int64_t)sizeof(T) <= 4096) hipLaunchKernelGGL((distill_eval_kernel<T, 64>), dim3((unsigned)n), dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((distill_eval_kernel<T, 256>), dim3((unsigned)n), dim3(256), 0, s, a);
+    } else {
+        const int64_t chunks = V * (int64_t)sizeof(T) / 16;  // at most this many whole ones
+        const dim3 grid((unsigned)n);
+        if (chunks <= 64 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 64, 4>), grid, dim3(64), 0, s, a);
+        else if (chunks <= 256 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 256, 4>), grid, dim3(256), 0, s, a);
+        else if (chunks <= 1024 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 4>), grid, dim3(1024), 0, s, a);
+        else if (chunks <= 1024 * 6) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 6>), grid, dim3(1024), 0, s, a);
+        else if (chunks <= 1024 * 8) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 8>), grid, dim3(1024), 0, s, a);
+        else if (chunks <= 1024 * 12) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 12>), grid, dim3(1024), 0, s, a);
+        else if (chunks <= 1024 * 16) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 16>), grid, dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((distill_long_kernel<T, 1024>), grid, dim3(1024), 0, s, a);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+template <class T>
+static int launch_logp(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
+    const int S = row_parts(m, V);
+    if (S > 1) {
+        hipLaunchKernelGGL((logp_kernel<T, 256, true>), dim3(S, (unsigned)m), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((logp_join_kernel<T>), dim3((unsigned)m), dim3(64), 0, s, a, S);
+    } else if (V * (int64_t)sizeof(T) <= 4096) {
+        hipLaunchKernelGGL((logp_kernel<T, 64, false>), dim3((unsigned)m), dim3(64), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((logp_kernel<T, 256, false>), dim3((unsigned)m), dim3(256), 0, s, a);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+// A grid's y dimension ends at 65 535: the rows go in slices of that.
+constexpr int64_t kMaxGridY = 65535;
+
+template <class T>
+static int launch_logp_grad(const T *z, int64_t ldz, int64_t m, int64_t V, const int64_t *targets, const float *stats, const float *row_g,
+                            T *g, int64_t ldg, hipStream_t s) {
+    const int S = grad_parts(V, sizeof(T));
+    const int64_t slices = (m + kMaxGridY - 1) / kMaxGridY;
+    for (int64_t k = slices - 1; k >= 0; --k) {
+        const int64_t r0 = k * kMaxGridY, cnt = std::min(kMaxGridY, m - r0);
+        const dim3 grid(S, (unsigned)cnt);
+        if (V * (int64_t)sizeof(T) <= 4096)
+            hipLaunchKernelGGL((logp_grad_kernel<T, 64>), grid, dim3(64), 0, s, z + r0 * ldz, ldz, (int)V, targets + r0, stats + 2 * r0,
+                               row_g + r0, g + r0 * ldg, ldg);
+        else
+            hipLaunchKernelGGL((logp_grad_kernel<T, 256>), grid, dim3(256), 0, s, z + r0 * ldz, ldz, (int)V, targets + r0, stats + 2 * r0,
+                               row_g + r0, g + r0 * ldg, ldg);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+static int check_pairs(int64_t m, const int64_t *offsets, int64_t pairs, float beta, float smoothing) {
+    if (m < 0 || pairs < 0 || pairs > 0x3fffffff || m > 0x7fffffffll) return fail(RBG_ESHAPE, "m = %lld, pairs = %lld", (long long)m, (long long)pairs);
+    if (!std::isfinite(beta) || !(smoothing >= 0.f && smoothing <= 1.f)) return fail(RBG_EINVAL, "beta = %g, smoothing = %g", beta, smoothing);
+    if (!offsets) return fail(RBG_EINVAL, "NULL pointer");
+    return RBG_OK;
+}
+
+}  // namespace rbg
+
+using namespace rbg;
+
+extern "C" {
+
+int rbg_distill_topk_workspace(int64_t n, int64_t V, int64_t *bytes) {
+    clear_error();
+    if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
+    if (n < 0 || V <= 0) return fail(RBG_ESHAPE, "n = %lld, V = %lld", (long long)n, (long long)V);
+    const int S = row_parts(n, V);
+    *bytes = S > 1 ? round16(n * S * (int64_t)sizeof(MaxSum)) + round16(n * kMaxEntries * 4) : 16;
+    return RBG_OK;
+}
+
+int rbg_distill_topk(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V, const int64_t *idx, const float *val, int k, float T,
+                     const float *row_w, float *loss, float *stats, void *grad, int64_t ldg, void *workspace, void *stream) {
+    clear_error();
+    if (int rc = check_rows(z, ldz, dtype, n, V)) return rc;
+    if (k < 1 || k > kMaxEntries) return fail(RBG_EUNSUPPORTED, "k = %d: 1 to %d entries per row", k, kMaxEntries);
+    if (!(T >= 1e-15f && T <= 1e15f)) return fail(RBG_EINVAL, "T = %g", T);  // (1 / T and T^2 stay normal numbers)
+    if (n == 0) return RBG_OK;
+    if (!idx || !val || !loss || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
+    if (grad)
+        if (int rc = check_grad(z, ldz, dtype, n, V, grad, ldg)) return rc;
+    const int S = row_parts(n, V);
+    DistillArgs a{z, ldz, (int)V, k, idx, val, (float)(1.4426950408889634 / (double)T), T, row_w, loss, stats, grad, ldg, (MaxSum *)workspace,
+                  (float *)((char *)workspace + round16(n * S * (int64_t)sizeof(MaxSum)))};
+    return with_elem(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, V, (hipStream_t)stream); });
+}
+
+int rbg_distill_topk_backward(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V, const int64_t *idx, const float *val, int k,
+                              float T, const float *stats, const float *row_w, void *grad, int64_t ldg, void *stream) {
+    clear_error();
+    if (int rc = check_rows(z, ldz, dtype, n, V)) return rc;
+    if (k < 1 || k > kMaxEntries) return fail(RBG_EUNSUPPORTED, "k = %d: 1 to %d entries per row", k, kMaxEntries);
+    if (!(T >= 1e-15f && T <= 1e15f)) return fail(RBG_EINVAL, "T = %g", T);
+    if (n == 0) return RBG_OK;
+    if (!idx || !val || !stats || !grad) return fail(RBG_EINVAL, "NULL pointer");
+    if (int rc = check_grad(z, ldz, dtype, n, V, grad, ldg)) return rc;
+    const int S = grad_parts(V, elem_size(dtype));
+    return with_elem(dtype, [&](auto t) {
+        typedef decltype(t) E;
+        for (int64_t r0 = 0; r0 < n; r0 += kMaxGridY) {
+            const DistillArgs a{(const E *)z + r0 * ldz, ldz, (int)V, k, idx + r0 * k, val + r0 * k, (float)(1.4426950408889634 / (double)T), T,
+                                row_w ? row_w + r0 : nullptr, nullptr, const_cast<float *>(stats) + 2 * r0, (E *)grad + r0 * ldg, ldg, nullptr, nullptr};
+            const dim3 grid(S, (unsigned)std::min(kMaxGridY, n - r0));
+            hipLaunchKernelGGL((distill_grad_kernel<E, 256, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
+        }
+        RBG_HIP(hipGetLastError());
+        return (int)RBG_OK;
+    });
+}
+
+int rbg_token_logp_workspace(int64_t m, int64_t V, int64_t *bytes) {
+    clear_error();
+    if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
+    if (m < 0 || V <= 0) return fail(RBG_ESHAPE, "m = %lld, V = %lld", (long long)m, (long long)V);
+    const int S = row_parts(m, V);
+    *bytes = S > 1 ? round16(m * S * (int64_t)sizeof(MaxSum)) : 16;
+    return RBG_OK;
+}
+
+int rbg_token_logp(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, const int64_t *targets, float *logp, float *stats,
+                   void *workspace, void *stream) {
+    clear_error();
+    if (int rc = check_rows(z, ldz, dtype, m, V)) return rc;
+    if (m == 0) return RBG_OK;
+    if (!targets || !logp || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
+    const LogpArgs a{z, ldz, (int)V, targets, logp, nullptr, nullptr, stats, (MaxSum *)workspace};
+    return with_elem(dtype, [&](auto t) { return launch_logp<decltype(t)>(a, m, V, (hipStream_t)stream); });
+}
+
+int rbg_token_logp_backward(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, const int64_t *targets, const float *stats,
+                            const float *row_g, void *grad, int64_t ldg, void *stream) {
+    clear_error();
+    if (int rc = check_rows(z, ldz, dtype, m, V)) return rc;
+    if (m == 0) return RBG_OK;
+    if (!targets || !stats || !row_g || !grad) return fail(RBG_EINVAL, "NULL pointer");
+    if (int rc = check_grad(z, ldz, dtype, m, V, grad, ldg)) return rc;
+    return with_elem(dtype, [&](auto t) {
+        typedef decltype(t) E;
+        return launch_logp_grad<E>((const E *)z, ldz, m, V, targets, stats, row_g, (E *)grad, ldg, (hipStream_t)stream);
+    });
+}
+
+int rbg_preference_loss(const float *logp, int64_t m, const int64_t *offsets, int64_t pairs, const float *ref, float beta, float smoothing,
+                        float *loss, float *margin, void *stream) {
+    clear_error();
+    if (int rc = check_pairs(m, offsets, pairs, beta, smoothing)) return rc;
+    if (pairs == 0) return RBG_OK;
+    if ((m && !logp) || !ref || !loss || !margin) return fail(RBG_EINVAL, "NULL pointer");
+    hipLaunchKernelGGL((pair_kernel<float, false>), dim3((unsigned)pairs), dim3(256), 0, (hipStream_t)stream, logp, m, offsets, ref, beta,
+                       smoothing, (const float *)nullptr, loss, margin, (float *)nullptr);
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+int rbg_preference_loss_backward(const float *margin, int64_t m, const int64_t *offsets, int64_t pairs, float beta, float smoothing,
+                                 const float *g_loss, const float *g_margin, float *grad_logp, void *stream) {
+    clear_error();
+    if (int rc = check_pairs(m, offsets, pairs, beta, smoothing)) return rc;
+    if (m == 0) return RBG_OK;
+    if ((pairs && !margin) || !grad_logp) return fail(RBG_EINVAL, "NULL pointer");
+    hipLaunchKernelGGL(pair_grad_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, (hipStream_t)stream, margin, m, offsets, pairs, beta,
+                       smoothing, g_loss, g_margin, grad_logp);
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+int rbg_preference_grad_workspace(int64_t m, int64_t V, int64_t *bytes) {
+    if (int rc = rbg_token_logp_workspace(m, V, bytes)) return rc;
+    *bytes += round16(8 * m) + round16(8 * m) + round16(4 * m);  // logp in 64 bits, (m, S), the tokens' coefficients
+    return RBG_OK;
+}
+
+int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, const int64_t *targets, const int64_t *offsets,
+                        int64_t pairs, const float *ref, float beta, float smoothing, const float *pair_w, float *loss, float *margin,
+                        void *grad, int64_t ldg, void *workspace, void *stream) {
+    clear_error();
+    if (int rc = check_rows(z, ldz, dtype, m, V)) return rc;
+    if (int rc = check_pairs(m, offsets, pairs, beta, smoothing)) return rc;
+    if (m == 0 && pairs == 0) return RBG_OK;
+    if ((pairs && (!ref || !loss || !margin)) || (m && (!targets || !grad || !workspace))) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
+    if (m)
+        if (int rc = check_grad(z, ldz, dtype, m, V, grad, ldg)) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    char *w = (char *)workspace;
+    double *logp = (double *)w;
+    float *stats = (float *)(w + round16(8 * m));
+    float *coef = (float *)(w + 2 * round16(8 * m));
+    MaxSum *part = (MaxSum *)(w + 2 * round16(8 * m) + round16(4 * m));
+    return with_elem(dtype, [&](auto t) {
+        typedef decltype(t) E;
+        if (m) {
+            const LogpArgs a{z, ldz, (int)V, targets, nullptr, logp, coef, stats, part};
+            if (int rc = launch_logp<E>(a, m, V, s)) return rc;
+        }
+        if (pairs) {
+            hipLaunchKernelGGL((pair_kernel<double, true>), dim3((unsigned)pairs), dim3(256), 0, s, logp, m, offsets, ref, beta, smoothing,
+                               pair_w, loss, margin, coef);
+            RBG_HIP(hipGetLastError());
+        }
+        return m ? launch_logp_grad<E>((const E *)z, ldz, m, V, targets, stats, coef, (E *)grad, ldg, s) : (int)RBG_OK;
+    });
+}
+
+}  // extern "C"

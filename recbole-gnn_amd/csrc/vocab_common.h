@@ -1,0 +1,58 @@
+// vocab_common.h — pieces shared by the operators over large item vocabularies (embed.hip, logits.hip, score_i8.hip): the three
+// element types, 16-byte vectors of them, and reductions over a workgroup.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "internal.h"
+
+namespace rbg {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+inline bool elem_ok(int dtype) { return dtype == RBG_F32 || dtype == RBG_BF16 || dtype == RBG_F16; }
+inline int elem_size(int dtype) { return dtype == RBG_F32 ? 4 : 2; }
+__device__ __forceinline__ bool on_16_dev(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// N consecutive elements moved by one load or store; the loads and stores below state the alignment they rely on.
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+    T v[N];
+};
+
+// All arithmetic is in 32 bits; a store rounds once, to nearest even (what the casts compile to on gfx950).
+template <class T>
+__device__ __forceinline__ float to_f32(T x) { return (float)x; }
+template <class T>
+__device__ __forceinline__ T from_f32(float x) { return (T)x; }
+
+constexpr int kWave = 64;
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Runs f(type tag) for the element type named by an RBG_* code that elem_ok() has accepted.
+template <class F>
+inline int with_elem(int dtype, F f) {
+    if (dtype == RBG_F32) return f(float{});
+    if (dtype == RBG_BF16) return f(bf16_t{});
+    return f(f16_t{});
+}
+
+}  // namespace rbg

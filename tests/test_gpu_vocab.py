@@ -1,0 +1,681 @@
+"""The operators over large item vocabularies against plain restatements in 64 bits.
+
+Tolerances are bounds by arithmetic, element by element.  u = 2^-24 is half a step of 32 bits; a store to type t adds at most
+finfo(t).eps / 2 of the value (or half the smallest subnormal).  The sum of a row's V exponentials is formed by at least 64 threads
+one element after the other and then over at most 64 + 16 partial sums, and each online rescaling repeats an exponential: with A the
+largest |z - m| log2(e) / T in the row, an exponential is off by (4 + 3 A) u (the difference, the product, the constant, 2 u of the
+hardware exp2), and S and every q by E = (4 + 3 A + 2 (V / 64 + 96)) u of their value."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+ALL = [F32, BF16, F16]
+
+
+def stored(ref, dtype):
+    """The most that one store of ``ref`` to ``dtype`` can be off (with the rounding to 32 bits in front of it)."""
+    f = torch.finfo(dtype)
+    return ref.abs() * (f.eps / 2 * (1 + U) + (0 if dtype == F32 else U)) + f.smallest_normal * f.eps / 2
+
+
+def within(got, ref, tol):
+    got, ref = got.double(), ref.double()
+    assert got.shape == ref.shape
+    odd = ~torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    assert torch.equal(got[odd & ~torch.isnan(ref)], ref[odd & ~torch.isnan(ref)])
+    off = torch.where(odd, 0.0, (got - ref).abs() - tol)
+    assert off.numel() == 0 or off.max() <= 0, f"off by {off.max().item():.3g} more than the bound, at {off.argmax().item()}"
+
+
+def gen(seed, dev):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+# ---- table rows --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,rows,d", [(1, 1, 1), (5, 3, 7), (32, 1000, 64), (257, 33, 65), (1000, 4097, 128), (63, 100, 1000), (4099, 50, 8)])
+def test_embedding(rbg, cuda, dtype, n, rows, d):
+    g = gen(n + d, cuda)
+    table = torch.randn(rows, d, generator=g, device=cuda).to(dtype)
+    ids = torch.randint(-2, rows + 2, (n,), generator=g, device=cuda)
+    ids[0] = rows - 1
+    there = (ids >= 0) & (ids < rows)
+    for scale in (1.0, math.sqrt(d) * 1.1):
+        out = rbg.embedding(table, ids, scale=scale, padding_idx=0)
+        ref = table[torch.where(there, ids, 0)].double() * scale * there[:, None]
+        within(out, ref, stored(ref, dtype) + 2 * U * ref.abs())  # (the scale itself is rounded to 32 bits)
+        assert torch.all(out[~there] == 0)
+    assert torch.equal(rbg.embedding(table, ids)[there], table[ids[there]])  # scale 1 copies
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_embedding_layouts(rbg, cuda, dtype):
+    g = gen(3, cuda)
+    wide = torch.randn(50, 200, generator=g, device=cuda).to(dtype)
+    ids = torch.randint(50, (3, 5, 7), generator=g, device=cuda)
+    for table in (wide[:, 3:67], wide[:, 8:72], wide[5:, :64], wide.t()[:64].t(), wide[:, :64].t().contiguous().t(), wide[::2, 1:65], wide[:1].expand(50, 200)):
+        own = ids % table.shape[0]
+        assert torch.equal(rbg.embedding(table, own), table[own])
+        assert torch.equal(rbg.embedding(table, own.int()), table[own])
+        assert torch.equal(rbg.embedding(table, own.permute(2, 0, 1)), table[own.permute(2, 0, 1)])
+    assert rbg.embedding(wide, ids[:0]).shape == (0, 5, 7, 200)
+    assert torch.all(rbg.embedding(wide[:0], ids) == 0)
+
+
+def runs_reference(grad, ids, rows, scale, padding):
+    """(sum, sum of magnitudes, count) per row in 64 bits."""
+    ok = (ids >= 0) & (ids < rows) & (ids != padding)
+    g = grad.double()[ok] * scale
+    zero = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device=grad.device)
+    return (zero.index_add(0, ids[ok], g), zero.index_add(0, ids[ok], g.abs()),
+            torch.bincount(ids[ok], minlength=rows)[:, None].double())
+
+
+GRAD_SHAPES = [(1, 1, 1), (2, 5, 64), (7, 3, 65), (300, 50, 64), (5000, 40, 128), (6144, 40982, 64), (4096, 1, 32), (16384, 1000, 32), (16385, 511, 24),
+               (16385, 512, 8), (20000, 70000, 64), (40000, 3, 100), (50000, 300000, 16), (70001, 100, 1), (33000, 1, 4), (1000, 20, 1024), (3000, 7, 2051)]
+
+
+@pytest.mark.parametrize("n,rows,d", GRAD_SHAPES)
+@pytest.mark.parametrize("dtype", ALL)
+def test_embedding_grad(rbg, cuda, dtype, n, rows, d):
+    g = gen(n + rows, cuda)
+    grad = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    u = torch.rand(n, generator=g, device=cuda)
+    ids = (rows * u * u * u).long().clamp_(max=rows - 1)
+    ids[torch.rand(n, generator=g, device=cuda) < 0.05] = -1
+    ids[n // 2:n // 2 + 1] = rows  # out of range
+    for padding, out_dtype in ((None, None), (0, F32)):
+        got = rbg.embedding_grad(grad, ids, rows, scale=1.7, padding_idx=padding, out_dtype=out_dtype)
+        assert got.dtype == (out_dtype or dtype)
+        ref, mag, cnt = runs_reference(grad, ids, rows, 1.7, -1 if padding is None else padding)
+        within(got, ref, stored(ref, got.dtype) + mag * U * (cnt + 4))  # cnt additions in some order, the scale, its rounding
+        assert torch.all(got[cnt[:, 0] == 0] == 0)
+        assert torch.equal(got, rbg.embedding_grad(grad, ids, rows, scale=1.7, padding_idx=padding, out_dtype=out_dtype))
+
+
+@pytest.mark.parametrize("n", [0, 1, 9, 3000, 20000])
+def test_embedding_grad_of_nothing_and_of_one_row(rbg, cuda, n):
+    grad = torch.ones(n, 64, device=cuda)
+    none = torch.full((n,), -1, device=cuda)
+    assert torch.all(rbg.embedding_grad(grad, none, 300) == 0)
+    assert torch.all(rbg.embedding_grad(grad, torch.full_like(none, 299), 300)[299] == n)  # whole numbers below 2^24: exact in any order
+    assert torch.all(rbg.embedding_grad(grad, torch.full_like(none, 7), 300, padding_idx=7) == 0)
+    last = rbg.embedding_grad(grad, torch.arange(n, device=cuda) % 300, 300)
+    assert torch.equal(last[:, 0], torch.bincount(torch.arange(n, device=cuda) % 300, minlength=300).float())
+
+
+def test_embedding_grad_sums_in_ascending_order(rbg, cuda):
+    """Within a chunk places are added one after the other in their order: 2^24 + 1 + 1 - 2^24 shows it (1 + 1 first would give 2)."""
+    grad = torch.tensor([2.0 ** 24, 1.0, 1.0, -2.0 ** 24], device=cuda)[:, None].repeat(1, 4)
+    ids = torch.zeros(4, dtype=torch.int64, device=cuda)
+    assert torch.all(rbg.embedding_grad(grad, ids, 1) == 0.0)
+    order = torch.tensor([1, 2, 0, 3], device=cuda)
+    assert torch.all(rbg.embedding_grad(grad[order], ids, 1) == 2.0)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_embedding_grad_layouts(rbg, cuda, dtype):
+    g = gen(5, cuda)
+    wide = torch.randn(400, 200, generator=g, device=cuda).to(dtype)
+    ids = torch.randint(30, (400,), generator=g, device=cuda)
+    for grad in (wide[:, 3:67], wide[:, 8:72], wide[:, ::2], wide[:1].expand(400, 200)):
+        assert torch.equal(rbg.embedding_grad(grad, ids, 30), rbg.embedding_grad(grad.contiguous(), ids, 30))
+    three = rbg.embedding_grad(wide.view(8, 50, 200), ids.view(8, 50), 30)
+    assert torch.equal(three, rbg.embedding_grad(wide, ids, 30))
+
+
+def test_embedding_autograd(rbg, cuda):
+    g = gen(6, cuda)
+    table = torch.randn(20, 12, generator=g, device=cuda, requires_grad=True)
+    ids = torch.randint(20, (4, 9), generator=g, device=cuda)
+    w = torch.randn(4, 9, 12, generator=g, device=cuda)
+    (rbg.embedding(table, ids, scale=0.5, padding_idx=3) * w).sum().backward()
+    ref, mag, cnt = runs_reference(w.view(-1, 12), ids.view(-1), 20, 0.5, 3)
+    within(table.grad, ref, stored(ref, F32) + mag * U * (cnt + 4))
+    # differences: the sum is linear in the table, so a step of 1 is exact up to the roundings of two sums of 432 terms
+    t = table.detach().clone()
+    i = int(ids[0, 0]) if int(ids[0, 0]) != 3 else int(ids[0, 1])
+    lo = (rbg.embedding(t, ids, scale=0.5).double() * w.double()).sum()
+    t[i, 5] += 1.0
+    hi = (rbg.embedding(t, ids, scale=0.5).double() * w.double()).sum()
+    assert abs((hi - lo) - table.grad[i, 5].double()) <= 36 * 4 * U * float(w.abs().max()) * 8
+
+
+def test_embedding_beyond_32_bits(rbg, cuda):
+    rows, d = (1 << 25) + 11, 64  # 2^31 + 704 elements
+    table = torch.zeros(rows, d, dtype=BF16, device=cuda)
+    table[-1] = 3.0
+    table[(1 << 25) - 1] = 2.0
+    ids = torch.tensor([rows - 1, (1 << 25) - 1, rows, 5], device=cuda)
+    out = rbg.embedding(table, ids)
+    assert [float(v) for v in out[:, 63]] == [3.0, 2.0, 0.0, 0.0]
+    del table
+    grad = rbg.embedding_grad(torch.ones(4, d, dtype=BF16, device=cuda), ids, rows)
+    assert torch.all(grad[-1] == 1) and torch.all(grad[(1 << 25) - 1] == 1) and torch.all(grad[5] == 1)
+    assert float(grad.sum(dtype=F32)) == 3 * d
+
+
+# ---- distillation ------------------------------------------------------------------------------------------------------
+
+def distill_reference(z, idx, val, temp, w):
+    """(loss, its bound, gradient, its bound) in 64 bits."""
+    n, v = z.shape
+    z = z.double()
+    there = (idx >= 0) & (idx < v)
+    at = torch.where(there, idx, 0)
+    val = torch.where(there, val.double(), -math.inf)
+    some = there & ~torch.isneginf(val)
+    m = z.amax(1, keepdim=True)
+    empty = ~some.any(1) | torch.isneginf(m[:, 0])
+    p = torch.softmax(val / temp, 1)
+    logq = torch.log_softmax(z / temp, 1)
+    terms = torch.where(there & (p > 0), torch.xlogy(p, p) - p * logq.gather(1, at), torch.where(torch.isnan(p), p, 0.0))
+    loss = torch.where(empty, 0.0, temp * temp * terms.sum(1))
+    grad = logq.exp().scatter_add(1, at, torch.where(there, -p, 0.0))
+    grad = torch.where(empty[:, None], 0.0, grad * (w[:, None] * temp))
+    k = idx.shape[1]
+    fin = torch.where(torch.isfinite(z), z, m)
+    far = ((m - fin) * (1.4427 / temp)).amax(1, keepdim=True).clamp(max=160.0)  # below 2^-150 an exponential is 0 either way
+    e = (4 + 3 * far + 2 * (v / 64 + 96)) * U
+    tfar = torch.where(some, (val.amax(1, keepdim=True) - val) * (1.4427 / temp), 0.0).clamp(max=160.0)
+    ep = (6 + 3 * tfar + k + 8) * U
+    lq = torch.where(some, logq.gather(1, at), 0.0)
+    lp = torch.where(some & (p > 0), torch.log(p), 0.0)
+    tl = (p * (e + ep + 6 * U * (lq.abs() + lp.abs()) + (lq - lp).abs() * (ep + (k + 4) * U))).sum(1) * temp * temp + 1e-37
+    q = logq.exp()
+    tg = (w[:, None].abs() * temp) * (q * (e + 4 * U) + q.new_zeros(n, v).scatter_add(1, at, torch.where(some, p * (ep + 4 * U), 0.0)))
+    tg = tg + (w[:, None].abs() * temp + 1) * 2.0 ** -125 + stored(grad, F32)
+    return loss, torch.nan_to_num(tl, nan=0.0, posinf=0.0), grad, torch.nan_to_num(tg, nan=0.0)
+
+
+def distill_inputs(seed, n, v, k, dtype, dev, pad=0):
+    g = gen(seed, dev)
+    z = (2 * torch.randn(n, v + pad, generator=g, device=dev)).to(dtype)[:, :v]
+    idx = torch.randint(v, (n, k), generator=g, device=dev)
+    val = 2 * torch.randn(n, k, generator=g, device=dev) + 3
+    left = torch.randint(0, 2 * k + 1, (n, 1), generator=g, device=dev)
+    none = torch.arange(k, device=dev)[None] >= left
+    idx[none] = -1
+    val[none] = math.nan  # whatever stands beside a missing entry
+    return z, idx, val, torch.rand(n, generator=g, device=dev) + 0.5
+
+
+def distill_check(rbg, z, idx, val, temp, w):
+    loss, tl, grad, tg = distill_reference(z, idx, val, temp, w)
+    got, gg = rbg.distill_topk_grad(z, idx, val, temperature=temp, row_weight=w)
+    within(got, loss, tl)
+    within(gg, grad, tg + stored(grad, z.dtype))
+    assert torch.equal(rbg.distill_topk(z, idx, val, temperature=temp).isnan(), loss.isnan())
+    within(rbg.distill_topk(z, idx, val, temperature=temp), loss, tl)
+    leaf = z.detach().clone().requires_grad_()
+    out = rbg.distill_topk(leaf, idx, val, temperature=temp)
+    out.backward(w)
+    within(out.detach(), loss, tl)
+    within(leaf.grad, grad, tg + stored(grad, z.dtype))
+    again, g2 = rbg.distill_topk_grad(z, idx, val, temperature=temp, row_weight=w)
+    assert torch.equal(torch.nan_to_num(again), torch.nan_to_num(got)) and torch.equal(torch.nan_to_num(g2), torch.nan_to_num(gg))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,v,k", [(1, 1, 1), (3, 2, 2), (5, 7, 3), (64, 1683, 10), (17, 1024, 256), (600, 63, 4), (2, 50001, 33), (100, 16390, 5), (513, 4099, 12),
+                                   (1, 300007, 64)])
+def test_distill(rbg, cuda, dtype, n, v, k):
+    z, idx, val, w = distill_inputs(n + v, n, v, k, dtype, cuda)
+    distill_check(rbg, z, idx, val, 2.0, w)
+
+
+@pytest.mark.parametrize("dtype,v", [(F32, 12289), (F32, 20001), (F32, 30000), (F32, 40982), (F32, 60001), (F32, 65539), (F32, 70001), (BF16, 33000), (BF16, 40982),
+                                     (F16, 65530), (BF16, 90001), (F16, 131077)])
+def test_distill_every_row_length(rbg, cuda, dtype, v):
+    """Enough rows that each has a workgroup of its own: every size of register-resident row, and the longer ones."""
+    z, idx, val, w = distill_inputs(v, 512, v, 20, dtype, cuda)
+    distill_check(rbg, z, idx, val, 1.0, w)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n", [6, 520])
+@pytest.mark.parametrize("v", [40, 9001, 40000])
+def test_distill_masks(rbg, cuda, dtype, n, v):
+    z, idx, val, w = distill_inputs(7, n, v, 6, dtype, cuda, pad=5)
+    idx[:6], val[:6] = torch.arange(6, device=cuda) * 5, 1.0
+    low = torch.finfo(dtype).min
+    idx[0] = -1                                   # no entry
+    val[1] = -math.inf                            # entries without weight
+    z[2] = -math.inf                              # no logits
+    z[3] = low                                    # all masked by the lowest value: a uniform row
+    z[4, ::2] = -math.inf                         # masked items, entries 0, 10, 20 among them: an infinite loss
+    z[5, 1::2], idx[5, 3:] = low, 10              # masked items, and one index four times (10 and 10, 10, 10)
+    z[5, 10], val[5] = 1.0, torch.tensor([0.5, 1.0, 1.5, -math.inf, 2.0, 2.5], device=cuda)
+    distill_check(rbg, z, idx, val, 1.5, w)
+    loss, grad = rbg.distill_topk_grad(z, idx, val, temperature=1.5)
+    assert torch.all(loss[:3] == 0) and torch.all(grad[:3] == 0) and float(loss[4]) == math.inf
+    bad = z.clone()
+    bad[0, 3], bad[3, 0], bad[1, 0], bad[5, 7] = math.nan, math.nan, math.inf, math.inf
+    loss, grad = rbg.distill_topk_grad(bad, idx, val, temperature=1.5)
+    assert torch.all(loss[:2] == 0) and torch.all(grad[:2] == 0) and torch.all(loss[3:6:2].isnan()) and torch.all(grad[3].isnan())
+    # a row spoils itself alone (the same bits, from rows of the same layout: where a row starts decides which thread adds what)
+    assert torch.equal(grad[6:], rbg.distill_topk_grad(z.clone(), idx, val, temperature=1.5)[1][6:])
+
+
+def test_distill_differences(rbg, cuda):
+    """Central differences with h = 2^-5: off by h^2 / 6 times the third derivative (at most T = 1 here) and by the losses' own bound / h."""
+    z, idx, val, _ = distill_inputs(11, 4, 9, 3, F32, cuda)
+    idx[:, 0], val[:, 0] = 4, 1.0
+    w = torch.ones(4, device=cuda)
+    _, tl, _, _ = distill_reference(z, idx, val, 1.0, w)
+    _, grad = rbg.distill_topk_grad(z, idx, val)
+    h = 2.0 ** -5
+    for j in range(9):
+        zp, zm = z.clone(), z.clone()
+        zp[:, j] += h
+        zm[:, j] -= h
+        diff = (rbg.distill_topk(zp, idx, val).double() - rbg.distill_topk(zm, idx, val).double()) / ((zp - zm)[:, j].double())
+        assert torch.all((diff - grad[:, j].double()).abs() <= h * h / 6 + 4 * tl / h + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("n,v", [(3, 50000), (520, 777), (520, 70001)])
+def test_distill_in_place(rbg, cuda, n, v):
+    z, idx, val, w = distill_inputs(2, n, v, 9, F32, cuda)
+    loss, grad = rbg.distill_topk_grad(z, idx, val, row_weight=w)
+    lib, b = rbg._lib.lib, ctypes.c_int64()
+    rbg._lib.check(lib.rbg_distill_topk_workspace(n, v, ctypes.byref(b)))
+    work = torch.empty(b.value, dtype=torch.uint8, device=cuda)
+    out = torch.empty_like(loss)
+    rbg._lib.check(lib.rbg_distill_topk(z.data_ptr(), v, 0, n, v, idx.data_ptr(), val.data_ptr(), 9, 1.0, w.data_ptr(), out.data_ptr(), None,
+                                        z.data_ptr(), v, work.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(z, grad) and torch.equal(out, loss)
+
+
+def test_distill_rows_beyond_32_bits(rbg, cuda):
+    n, v = 2051, (1 << 20) + 1  # 2^31 + 3 M elements
+    z = torch.zeros(n, v, dtype=BF16, device=cuda)
+    z[-1, -1] = 8.0
+    idx = torch.full((n, 1), v - 1, device=cuda)
+    val = torch.zeros(n, 1, device=cuda)
+    loss, grad = rbg.distill_topk_grad(z, idx, val)
+    ref = math.log((v - 1) * math.exp(-8.0) + 1.0)
+    assert abs(float(loss[-1]) - ref) < ref * 1e-3 and abs(float(loss[0]) - math.log(v)) < 1e-3
+    q = math.exp(-ref)
+    assert abs(float(grad[-1, -1]) - (q - 1)) < 2.0 ** -8 and abs(float(grad[-1, 0]) - math.exp(-8.0 - ref)) < 2.0 ** -8 * math.exp(-8.0 - ref)
+    assert abs(float(grad[-2, -1]) - (1.0 / v - 1)) < 2.0 ** -8
+
+
+# ---- log-probabilities and the preference loss -----------------------------------------------------------------------------
+
+def logp_reference(z, y):
+    """(logp, its bound, softmax, E) in 64 bits; 0 for rows without a target or without logits."""
+    v = z.shape[1]
+    z = z.double()
+    m = z.amax(1, keepdim=True)
+    there = (y >= 0) & (y < v) & ~torch.isneginf(m[:, 0])
+    lq = torch.log_softmax(z, 1)
+    lp = torch.where(there, lq.gather(1, torch.where(there, y, 0)[:, None])[:, 0], 0.0)
+    fin = torch.where(torch.isfinite(z), z, m)
+    far = ((m - fin) * 1.4427).amax(1).clamp(max=160.0)
+    e = torch.nan_to_num((4 + 3 * far + 2 * (v / 64 + 96)) * U, nan=0.0)
+    return lp, e + 2 * U * torch.nan_to_num(lp.abs(), posinf=0.0), lq.exp(), e, there
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("m,v", [(1, 1), (3, 2), (40, 1683), (7, 60001), (600, 1025), (530, 9000), (2, 262147)])
+def test_token_logp(rbg, cuda, dtype, m, v):
+    g = gen(m + v, cuda)
+    z = (3 * torch.randn(m, v + 3, generator=g, device=cuda)).to(dtype)[:, 1:v + 1]
+    y = torch.randint(-1, v + 1, (m,), generator=g, device=cuda)
+    y[0] = v - 1
+    if m > 6:
+        z[1], z[2], z[3, :v // 2], z[4] = -math.inf, torch.finfo(dtype).min, -math.inf, math.nan
+        y[:6] = torch.tensor([v - 1, 0, 1, v - 1, -1, 0], device=cuda)
+        z[5, 0] = -math.inf
+    lp, tol, q, e, there = logp_reference(z, y)
+    leaf = z.detach().clone().requires_grad_()
+    out = rbg.token_logp(leaf, y)
+    within(out.detach(), lp, tol)
+    w = torch.randn(m, generator=g, device=cuda)
+    out.backward(w)
+    ref = -q * (w.double() * there)[:, None]
+    ref[torch.arange(m, device=cuda), torch.where(there, y, 0)] += w.double() * there
+    ref = torch.where(there[:, None], ref, 0.0)
+    bound = w.double().abs()[:, None] * (q * (e + 4 * U)[:, None] + 2.0 ** -125) + stored(ref, F32) + 2 * U * w.double().abs()[:, None]
+    within(leaf.grad, ref, torch.nan_to_num(bound) + stored(ref, dtype))
+
+
+def packed(seed, m, pairs, dev, lead=0, behind=0):
+    g = torch.Generator().manual_seed(seed)
+    cuts = torch.sort(torch.randint(lead, m - behind + 1, (2 * pairs - 1,), generator=g)).values
+    return torch.cat([torch.tensor([lead]), cuts, torch.tensor([m - behind])]).to(dev)
+
+
+def preference_reference(lp, tol, offsets, ref, beta, smoothing):
+    """(margin, its bound, loss, its bound, d loss / d margin, its bound) in 64 bits."""
+    o = offsets.tolist()
+    s = torch.stack([lp[a:b].sum() for a, b in zip(o[:-1], o[1:])]) - ref.double()
+    t = torch.stack([tol[a:b].sum() for a, b in zip(o[:-1], o[1:])])
+    h = beta * (s[0::2] - s[1::2])
+    th = abs(beta) * (t[0::2] + t[1::2]) * (1 + U) + 2 * U * h.abs()
+    ls = torch.nn.functional.logsigmoid
+    loss = -(1 - smoothing) * ls(h) - (smoothing * ls(-h) if smoothing else 0.0)
+    dh = smoothing * torch.sigmoid(h) - (1 - smoothing) * torch.sigmoid(-h)
+    return h, th, loss, th + 8 * U * (loss.abs() + 1), dh, th / 4 + 8 * U  # |d loss / d h| <= 1, |d2 loss / d h2| <= 1/4
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("m,v,pairs,lead,behind", [(1, 1, 1, 0, 0), (2, 3, 1, 0, 0), (40, 1683, 4, 3, 5), (9, 50001, 2, 0, 1), (700, 513, 300, 0, 0), (600, 9001, 5, 7, 11)])
+@pytest.mark.parametrize("smoothing,beta", [(0.0, 0.1), (0.3, 1.0), (1.0, -0.5)])
+def test_preference(rbg, cuda, dtype, m, v, pairs, lead, behind, smoothing, beta):
+    g = gen(m + pairs, cuda)
+    z = (2 * torch.randn(m, v, generator=g, device=cuda)).to(dtype)
+    y = torch.randint(v, (m,), generator=g, device=cuda)
+    y[torch.rand(m, generator=g, device=cuda) < 0.2] = -1
+    offsets = packed(pairs, m, pairs, cuda, lead, behind)
+    ref = -5 * torch.rand(2 * pairs, generator=g, device=cuda)
+    weight = torch.rand(pairs, generator=g, device=cuda) + 0.5
+    lp, tol, q, e, there = logp_reference(z, y)
+    h, th, loss, tl, dh, td = preference_reference(lp, tol, offsets, ref, beta, smoothing)
+    got, margin, grad = rbg.preference_grad(z, y, offsets, ref, beta=beta, label_smoothing=smoothing, pair_weight=weight)
+    within(margin, h, th)
+    within(got, loss, tl)
+    c, tc = torch.zeros(m, dtype=torch.float64, device=cuda), torch.zeros(m, dtype=torch.float64, device=cuda)
+    o = offsets.tolist()
+    for s in range(2 * pairs):
+        c[o[s]:o[s + 1]] = (1 if s % 2 == 0 else -1) * beta * dh[s // 2] * weight[s // 2].double()
+        tc[o[s]:o[s + 1]] = abs(beta) * (td[s // 2] + 4 * U) * weight[s // 2].double()
+    c, tc = c * there, tc * there
+    want = -q * c[:, None]
+    want[torch.arange(m, device=cuda), torch.where(there, y, 0)] += c
+    one = torch.zeros_like(q)
+    one[torch.arange(m, device=cuda), torch.where(there, y, 0)] = 1.0
+    bound = tc[:, None] * (q + one) + c.abs()[:, None] * (q * (e[:, None] + 4 * U) + 2 * U) + 2.0 ** -125 + stored(want, F32)
+    within(grad, want, bound + stored(want, dtype))
+    assert torch.all(grad[~there] == 0) and torch.all(grad[:lead] == 0) and torch.all(grad[m - behind:] == 0)
+    # the same through autograd, with a gradient for the margin too
+    leaf = z.detach().clone().requires_grad_()
+    l2, h2 = rbg.preference_loss(rbg.token_logp(leaf, y), offsets, ref, beta=beta, label_smoothing=smoothing)
+    within(l2.detach(), loss, tl + th)
+    torch.autograd.backward([l2, h2], [weight, torch.zeros_like(weight)])
+    within(leaf.grad, want, 2 * bound + stored(want, dtype))
+    leaf.grad = None
+    rbg.preference_loss(rbg.token_logp(leaf, y), offsets, ref, beta=beta, label_smoothing=smoothing)[1].sum().backward()
+    plain = torch.autograd.grad(sum((1 if s % 2 == 0 else -1) * beta * x for s, x in enumerate(_sums(leaf, y, there, o))), leaf)[0]
+    within(leaf.grad, plain.double(), abs(beta) * ((e + 12 * U)[:, None] * (q + one)) + 2 * stored(plain.double(), dtype) + 2.0 ** -125)
+
+
+def _sums(z, y, there, o):
+    lq = torch.log_softmax(z.double(), 1)
+    lp = torch.where(there, lq.gather(1, torch.where(there, y, 0)[:, None])[:, 0], 0.0)
+    return [lp[a:b].sum() for a, b in zip(o[:-1], o[1:])]
+
+
+def test_preference_long_sums(rbg, cuda):
+    """A margin of order 1 from sums of order 1e6: 32-bit sums would lose it."""
+    m = 200_000
+    g = gen(1, cuda)
+    logp = -5 * torch.rand(m, generator=g, device=cuda)
+    offsets = torch.tensor([0, m // 2, m], device=cuda)
+    sums = torch.stack([logp[:m // 2].double().sum(), logp[m // 2:].double().sum()])
+    ref = sums.float() + torch.tensor([0.5, -0.25], device=cuda)
+    loss, margin = rbg.preference_loss(logp, offsets, ref, beta=1.0)
+    want = (sums[0] - ref[0].double()) - (sums[1] - ref[1].double())
+    assert abs(float(margin[0]) - float(want)) <= 2 * U * abs(float(want)) + 1e-9
+    assert abs(float(loss[0]) - math.log1p(math.exp(-float(want)))) <= 1e-6
+
+
+def test_preference_extreme_margins(rbg, cuda):
+    logp = torch.tensor([0.0, -2e4, -math.inf, 0.0, math.nan, 0.0, 0.0, 0.0], device=cuda)
+    offsets = torch.arange(9, device=cuda)
+    loss, margin = rbg.preference_loss(logp, offsets, torch.zeros(8, device=cuda), beta=1.0)
+    assert float(loss[0]) == 0.0 and float(loss[1]) == math.inf and math.isnan(float(loss[2])) and abs(float(loss[3]) - math.log(2)) < 1e-6
+    assert float(margin[0]) == 2e4 and float(margin[1]) == -math.inf
+
+
+def test_preference_offsets_outside_are_clamped(rbg, cuda):
+    logp = torch.ones(5, device=cuda)
+    offsets = torch.tensor([-3, 2, 1 << 40], device=cuda)
+    _, margin = rbg.preference_loss(logp, offsets, torch.zeros(2, device=cuda), beta=1.0)
+    assert float(margin[0]) == 2 - 3
+    z, y = torch.zeros(5, 4, device=cuda), torch.zeros(5, dtype=torch.int64, device=cuda)
+    _, _, grad = rbg.preference_grad(z, y, torch.tensor([3, 1, 2], device=cuda), torch.zeros(2, device=cuda))
+    assert grad.shape == (5, 4) and bool(torch.isfinite(grad).all())
+
+
+def test_preference_is_bpr_for_single_tokens(rbg, cuda):
+    """One token each on a shared row and no reference model: the normalizers cancel and the loss is BPR's -log sigmoid(pos - neg)."""
+    g = gen(9, cuda)
+    u, items = torch.randn(50, 16, generator=g, device=cuda), torch.randn(200, 16, generator=g, device=cuda)
+    pos, neg = torch.randint(200, (50,), generator=g, device=cuda), torch.randint(200, (50,), generator=g, device=cuda)
+    scores = rbg.score(u, items)
+    y = torch.stack([pos, neg], 1).view(-1)
+    loss, margin, _ = rbg.preference_grad(scores.repeat_interleave(2, 0), y, torch.arange(101, device=cuda), torch.zeros(100, device=cuda), beta=1.0)
+    s = scores.double()
+    want = s.gather(1, pos[:, None])[:, 0] - s.gather(1, neg[:, None])[:, 0]
+    # the same row twice: the same S, and its logarithm in 64 bits cancels to the rounding of 64 bits
+    within(margin, want, 2 * U * want.abs() + 1e-12)
+    within(loss, -torch.nn.functional.logsigmoid(want), 8 * U * (want.abs() + 1))
+
+
+# ---- 8 bits ------------------------------------------------------------------------------------------------------------
+
+def codes_reference(x):
+    """The definition: fl32(max / 127), the nearest whole number to fl32(x / scale).  (A quotient of two 32-bit numbers rounded to 64
+    and then to 32 bits is the one rounded to 32 bits.)"""
+    x = x.double().cpu()
+    s = (x.abs().amax(1) / 127.0).float().double()
+    s = torch.where(s < 2.0 ** -126, 0.0, s)
+    q = torch.where(s[:, None] > 0, (x / s[:, None]).float().double().round().clamp(-127, 127), 0.0)
+    return q, s
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,k", [(1, 1), (3, 5), (33, 64), (7, 127), (5, 513), (40, 1000), (2, 8193), (1, 131071)])
+def test_quantize_rows(rbg, cuda, dtype, n, k):
+    g = gen(n + k, cuda)
+    x = (torch.randn(n, k + 3, generator=g, device=cuda) * 10.0 ** torch.randint(-3, 4, (n, 1), generator=g, device=cuda)).to(dtype)[:, 2:k + 2]
+    if n > 2:
+        x[0] = 0.0
+        x[1] = torch.finfo(dtype).smallest_normal / 4
+        x[2] = torch.arange(k, device=cuda).to(dtype) - k // 2  # ties
+    codes, scale = rbg.quantize_rows(x)
+    q, s = codes_reference(x)
+    assert torch.equal(codes.cpu().double(), q) and torch.equal(scale.cpu().double(), s)
+    full = codes.as_strided((n, codes.stride(0)), (codes.stride(0), 1))
+    assert torch.all(full[:, k:] == 0)
+
+
+def test_quantize_rows_that_are_not_finite(rbg, cuda):
+    x = torch.randn(4, 700, device=cuda)
+    x[1, 699], x[2, 0] = math.nan, -math.inf
+    codes, scale = rbg.quantize_rows(x)
+    assert scale.isnan().tolist() == [False, True, True, False] and torch.all(codes[1:3] == 0)
+    s = rbg.score_int8(x, *rbg.quantize_rows(torch.randn(5, 700, device=cuda)))
+    assert torch.all(s[1:3].isnan()) and bool(torch.isfinite(s[::3]).all())
+
+
+def scores_check(rbg, u, codes, scales, out_dtype):
+    got = rbg.score_int8(u, codes, scales, out_dtype=out_dtype)
+    q, s = codes_reference(u)
+    ref = (q @ codes.cpu().double().t().contiguous()) * s[:, None] * scales.cpu().double()[None]  # whole-number sums below 2^53: exact
+    # the sum to 32 bits, and two products
+    within(got.cpu(), ref, 3.1 * U * ref.abs() + stored(ref, out_dtype) + 2.0 ** -148)
+    return got
+
+
+@pytest.mark.parametrize("b,n,k", [(1, 1, 1), (1, 1000, 128), (2, 333, 64), (3, 5, 7), (4, 4097, 100), (8, 130, 1000), (16, 257, 8192), (17, 129, 65), (33, 64, 4096),
+                                   (130, 257, 64), (129, 130, 1000), (300, 1025, 48), (64, 300, 8208), (513, 511, 2049), (1, 3, 131071), (700, 40, 16)])
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, F32), (BF16, BF16), (F16, F32), (F32, F16)])
+def test_score_int8(rbg, cuda, b, n, k, dtype, out_dtype):
+    g = gen(b + n + k, cuda)
+    u = torch.randn(b, k, generator=g, device=cuda).to(dtype)
+    codes, scales = rbg.quantize_rows(torch.randn(n, k, generator=g, device=cuda) * 0.1)
+    scores_check(rbg, u, codes, scales, out_dtype)
+
+
+def test_score_int8_exact_sums(rbg, cuda):
+    """All codes at their ends: sums of 131 071 products of 127 x 127 and 127 x -128 stay whole."""
+    k = 131071
+    u = torch.ones(3, k, device=cuda)
+    u[1] = -1.0
+    codes = torch.full((130, k), 127, dtype=torch.int8, device=cuda)
+    codes[5] = -128
+    codes[6, 1:] = 0
+    s = rbg.score_int8(u, codes, torch.ones(130, device=cuda))
+    su = float(torch.tensor(1.0) / torch.tensor(127.0))
+    f = lambda acc: float(torch.tensor(float(acc), dtype=F32) * torch.tensor(su, dtype=F32))  # noqa: E731
+    assert float(s[0, 0]) == f(127 * 127 * k) and float(s[1, 0]) == -f(127 * 127 * k) and float(s[0, 5]) == f(-128 * 127 * k) and float(s[2, 6]) == f(127 * 127)
+
+
+@pytest.mark.parametrize("b", [1, 5, 200])
+@pytest.mark.parametrize("k", [7, 64, 130, 1024])
+def test_score_int8_layouts(rbg, cuda, b, k):
+    g = gen(k, cuda)
+    u = torch.randn(b, k, generator=g, device=cuda)
+    codes, scales = rbg.quantize_rows(torch.randn(150, k, generator=g, device=cuda))
+    want = scores_check(rbg, u, codes, scales, F32)
+    junk = torch.randint(-128, 128, (150, k + 77), generator=g, device=cuda, dtype=torch.int8)
+    junk[:, 5:k + 5] = codes
+    wide = torch.randint(-128, 128, (300, (k + 127) // 64 * 64), generator=g, device=cuda, dtype=torch.int8)
+    wide[::2, 16:k + 16] = codes if k + 16 <= wide.shape[1] else 0
+    forms = [codes.contiguous(), junk[:, 5:k + 5], codes.t().contiguous().t()] + ([wide[::2, 16:k + 16]] if k + 16 <= wide.shape[1] else [])
+    for c in forms:  # (the columns behind K hold anything; rows may start anywhere)
+        assert torch.equal(rbg.score_int8(u, c, scales), want)
+    big = torch.randn(b, k + 5, generator=g, device=cuda)
+    big[:, 2:k + 2] = u
+    assert torch.equal(rbg.score_int8(big[:, 2:k + 2], codes, scales), want)
+    assert rbg.score_int8(u[:0], codes, scales).shape == (0, 150) and rbg.score_int8(u, codes[:0], scales[:0]).shape == (b, 0)
+
+
+def test_score_int8_beyond_32_bits(rbg, cuda):
+    n = (1 << 25) + 77  # the codes' bytes pass 2^31
+    codes = torch.zeros(n, 64, dtype=torch.int8, device=cuda)
+    codes[-1], codes[-2, 0] = 1, 2
+    s = rbg.score_int8(torch.full((1, 64), 127.0, device=cuda), codes, torch.ones(n, device=cuda))
+    assert float(s[0, -1]) == 64 * 127 and float(s[0, -2]) == 2 * 127 and float(s[0, 0]) == 0
+    s = rbg.score_int8(torch.full((130, 64), 127.0, device=cuda), codes[-(1 << 24):], torch.ones(1 << 24, device=cuda), out_dtype=BF16)  # 2^31 + .. scores
+    assert float(s[129, -1]) == 64 * 127 and float(s[128, -2]) == 254 and float(s[129, 0]) == 0 and float(s[0, -1]) == 64 * 127
+
+
+# ---- together ----------------------------------------------------------------------------------------------------------
+
+def test_a_student_from_ids_to_table_gradient(rbg, cuda):
+    """Ids -> rows -> logits -> a teacher's lists (full_sort_topk) -> loss -> gradients of the logits and of the table, all through the
+    public entry points, against the same in 64 bits; then the table answers in 8 bits."""
+    g = gen(21, cuda)
+    n, v, d, k = 300, 1200, 32, 10
+    teacher_u, teacher_i = torch.randn(n, 64, generator=g, device=cuda), torch.randn(v, 64, generator=g, device=cuda)
+    val, idx = rbg.full_sort_topk(None, teacher_u, teacher_i, torch.arange(n, device=cuda), k)
+    table = torch.randn(v, d, generator=g, device=cuda, requires_grad=True)
+    ids = torch.randint(v, (n,), generator=g, device=cuda)
+    rows = rbg.embedding(table, ids, scale=0.5, padding_idx=0)
+    logits = rows @ table.t()
+    loss = rbg.distill_topk(logits, idx, val, temperature=2.0)
+    loss.mean().backward()
+    t64 = table.detach().double().requires_grad_()
+    r64 = t64[ids] * 0.5
+    r64 = torch.where((ids == 0)[:, None], r64.detach(), r64)
+    z64 = (r64 @ t64.t()) / 2.0
+    p = torch.softmax(val.double() / 2.0, 1)
+    l64 = 4.0 * (torch.xlogy(p, p) - p * torch.log_softmax(z64, 1).gather(1, idx)).sum(1)
+    l64.mean().backward()
+    # 32-bit products of d terms of order |row| |item| <= ~ 30: each logit is off by at most d u sum|..| < 1e-4, and d loss / d z < T
+    assert float((loss.detach().double() - l64.detach()).abs().max()) < 4e-4
+    assert float((table.grad.double() - t64.grad).abs().max()) < 1e-3 * float(t64.grad.abs().max())
+    codes, scales = rbg.quantize_rows(table.detach())
+    s8, s32 = rbg.score_int8(rows.detach(), codes, scales), rbg.score(rows.detach(), table.detach())
+    # a code is off by half a step: |s8 - s| <= sum (|u| step_i / 2 + |i| step_u / 2 + ..) <= d max|u| max|i| / 127
+    bound = d * rows.detach().abs().amax(1)[:, None] * table.detach().abs().amax(1)[None] / 127.0 * 1.01
+    assert bool(torch.all((s8 - s32).abs() <= bound))
+
+
+def all_ops(rbg, cuda, seed):
+    g = gen(seed, cuda)
+    table = torch.randn(500, 40, generator=g, device=cuda)
+    ids = torch.randint(-1, 500, (20000,), generator=g, device=cuda)
+    grad = torch.randn(20000, 40, generator=g, device=cuda)
+    z, idx, val, w = distill_inputs(seed, 40, 9001, 7, BF16, cuda)
+    y = torch.randint(-1, 9001, (40,), generator=g, device=cuda)
+    offsets = packed(3, 40, 3, cuda)
+    ref = torch.randn(6, generator=g, device=cuda)
+    codes, scales = rbg.quantize_rows(torch.randn(700, 96, generator=g, device=cuda))
+    u1, u2 = torch.randn(1, 96, generator=g, device=cuda), torch.randn(150, 96, generator=g, device=cuda)
+
+    def run():
+        out = [rbg.embedding(table, ids, scale=2.0), rbg.embedding_grad(grad, ids, 500), rbg.embedding_grad(grad[:3000], ids[:3000], 500)]
+        out += rbg.distill_topk_grad(z, idx, val, row_weight=w)
+        out += rbg.preference_grad(z, y, offsets, ref)
+        out += [rbg.score_int8(u1, codes, scales), rbg.score_int8(u2, codes, scales), rbg.token_logp(z, y)]
+        return out
+
+    return run, [table, grad, z, u1, u2]
+
+
+def test_captured_and_replayed(rbg, cuda):
+    """Two captured graphs of every operator, replayed in turn with new inputs and eager work between the replays."""
+    graphs = []
+    for seed in (1, 2):
+        run, inputs = all_ops(rbg, cuda, seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((run, inputs, graph, out))
+    for turn in range(3):
+        for run, inputs, graph, out in graphs:
+            for t in inputs:
+                t.mul_(-0.75)
+            graph.replay()
+            eager = run()
+            torch.cuda.synchronize()
+            for a, b in zip(out, eager):
+                assert torch.equal(a, b)
+
+
+def test_on_another_stream(rbg, cuda):
+    run, _ = all_ops(rbg, cuda, 4)
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(run())
+    torch.cuda.synchronize()
+    for out in got:
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_wrappers_refuse(rbg, cuda):
+    f, i = torch.zeros(2, 4, device=cuda), torch.zeros(2, dtype=torch.int64, device=cuda)
+    o3 = torch.tensor([0, 1, 2], device=cuda)
+    refused = [
+        (TypeError, lambda: rbg.embedding(f.double(), i)), (TypeError, lambda: rbg.embedding(f, i.float())), (ValueError, lambda: rbg.embedding(f[0], i)),
+        (RuntimeError, lambda: rbg.embedding(f, i.cpu())), (ValueError, lambda: rbg.embedding_grad(f, i[:1], 3)), (TypeError, lambda: rbg.embedding_grad(f, i, 3, out_dtype=F16)),
+        (ValueError, lambda: rbg.distill_topk(f, i, f[:, 0])), (ValueError, lambda: rbg.distill_topk(f, i[:, None], f)), (rbg.RbgError, lambda: rbg.distill_topk(f, i[:, None], f[:, :1], temperature=0.0)),
+        (rbg.RbgError, lambda: rbg.distill_topk(f, i[:, None].expand(2, 257), f[:, :1].expand(2, 257))), (rbg.RbgError, lambda: rbg.distill_topk(f, i[:, None][:, :0], f[:, :0])),
+        (ValueError, lambda: rbg.distill_topk_grad(f, i[:, None], f[:, :1], row_weight=f[0])), (rbg.RbgError, lambda: rbg.distill_topk(f[:, :0], i[:, None], f[:, :1])),
+        (ValueError, lambda: rbg.token_logp(f, i[:1])), (ValueError, lambda: rbg.preference_loss(f[0], o3[:2], f[0, :1])), (ValueError, lambda: rbg.preference_loss(f[0], o3, f[0])),
+        (TypeError, lambda: rbg.preference_loss(f, o3, f[0, :2])), (rbg.RbgError, lambda: rbg.preference_loss(f[0], o3, f[0, :2], label_smoothing=2.0)),
+        (ValueError, lambda: rbg.preference_grad(f, i, o3, f[0, :2], pair_weight=f[0])), (ValueError, lambda: rbg.quantize_rows(f[:, :0])),
+        (TypeError, lambda: rbg.score_int8(f, f, f[0])), (ValueError, lambda: rbg.score_int8(f, torch.zeros(3, 5, dtype=torch.int8, device=cuda), f[0, :3])),
+        (ValueError, lambda: rbg.score_int8(f, torch.zeros(3, 4, dtype=torch.int8, device=cuda), f[0])), (TypeError, lambda: rbg.score_int8(f, torch.zeros(4, 4, dtype=torch.int8, device=cuda), f[0], out_dtype=torch.int8)),
+        (rbg.RbgError, lambda: rbg.score_int8(torch.zeros(1, 131072, device=cuda), torch.zeros(1, 131072, dtype=torch.int8, device=cuda), f[0, :1])),
+    ]
+    for k, (error, call) in enumerate(refused):
+        with pytest.raises(error):
+            call()
+            pytest.fail(f"call {k} was not refused")
+    for leaf in (torch.zeros(3, 4, device=cuda, requires_grad=True),):  # gradients of gradients are refused, not wrong
+        (g,) = torch.autograd.grad(rbg.token_logp(leaf, torch.zeros(3, dtype=torch.int64, device=cuda)).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
