@@ -131,6 +131,8 @@ SIGNATURES = {
                                     c_vp, c_vp]),
     "rbg_quantize_rows_i8": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
     "rbg_score_i8": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_int, c_vp]),
+    "rbg_score_rows_i8_workspace": (c_int, [c_i64, c_i64, P(c_i64)]),
+    "rbg_score_rows_i8": (c_int, [c_vp, c_i64, c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp]),
 }
 
 

@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vocab_common.h"
 
@@ -19,46 +20,112 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // ---- rows to 8 bits ------------------------------------------------------------------------------------------------------
 
-// One workgroup per row.  The quotient is the IEEE one (no reciprocal): a code is the nearest whole number to x / s, so whoever
-// restates the operator gets the same codes.
-template <class T, int TH>
-__global__ __launch_bounds__(TH) void quantize_kernel(const T *__restrict__ x, int64_t ldx, int64_t K, int8_t *__restrict__ codes, int64_t ldc,
-                                                      float *__restrict__ scale) {
-    __shared__ float red[TH / kWave];
+// The quotient is the IEEE one (no reciprocal): a code is the nearest whole number to x / s, so whoever restates the operator gets the
+// same codes.
+struct RowScale {
+    float s;    // what the row is divided by; 0: its codes are 0
+    float out;  // what is stored
+};
+__device__ __forceinline__ RowScale row_scale(float m) {  // m: the largest magnitude, infinite for a row that is not finite
+    const float s = m / 127.f;
+    if (m == INFINITY) return {0.f, NAN};
+    return s >= 1.17549435e-38f ? RowScale{s, s} : RowScale{0.f, 0.f};
+}
+__device__ __forceinline__ uint32_t code_of(float x, float s) { return (uint32_t)(int)fminf(fmaxf(rintf(x / s), -127.f), 127.f) & 255u; }
+__device__ __forceinline__ float magnitude(float x) {  // NaN counts as infinite
+    const float v = fabsf(x);
+    return v < INFINITY ? v : INFINITY;
+}
+
+// Rows that start on 16 bytes: G lanes per row hold NC vectors each, read once.
+template <class T, int G, int NC>
+__global__ __launch_bounds__(256) void quantize_kernel(const T *__restrict__ x, int64_t ldx, int64_t n, int K, int8_t *__restrict__ codes,
+                                                       int ldc, float *__restrict__ scale) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int sub = threadIdx.x % G;
+    const bool on = row < n;
+    const T *p = x + (on ? row : 0) * ldx;
+    Vec<T, E> v[NC];
+    float m = 0.f;
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+        const int c = (u * G + sub) * E;
+        if (c + E <= K) {
+            v[u] = *reinterpret_cast<const Vec<T, E> *>(p + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u].v[e] = c + e < K ? p[c + e] : from_f32<T>(0.f);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < NC; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, magnitude(to_f32(v[u].v[e])));
+#pragma unroll
+    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if constexpr (G > 64) {
+        __shared__ float red[4];
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
+    if (!on) return;
+    const RowScale s = row_scale(m);
+    if (sub == 0) scale[row] = s.out;
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+        const int c = (u * G + sub) * E;
+        if (c >= ldc) break;
+        Vec<uint32_t, E / 4> w;
+#pragma unroll
+        for (int k = 0; k < E / 4; ++k) {
+            w.v[k] = 0;
+            if (s.s != 0.f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.v[k] |= code_of(to_f32(v[u].v[4 * k + e]), s.s) << (8 * e);
+        }
+        *reinterpret_cast<Vec<uint32_t, E / 4> *>(codes + row * ldc + c) = w;
+    }
+}
+
+// Rows that start anywhere, or are too long for that: one workgroup per row, which it reads twice.
+template <class T>
+__global__ __launch_bounds__(256) void quantize_any_kernel(const T *__restrict__ x, int64_t ldx, int64_t K, int8_t *__restrict__ codes, int64_t ldc,
+                                                           float *__restrict__ scale) {
+    __shared__ float red[4];
     const int64_t row = blockIdx.x;
     const T *p = x + row * ldx;
     float m = 0.f;
-    bool odd = false;  // an infinity or NaN
-    for (int64_t j = threadIdx.x; j < K; j += TH) {
-        const float v = fabsf(to_f32(p[j]));
-        odd |= !(v < INFINITY);
-        m = fmaxf(m, v);
-    }
-    m = wave_max(odd ? INFINITY : m);
-    if constexpr (TH > kWave) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-        __syncthreads();
-        m = red[0];
-#pragma unroll
-        for (int i = 1; i < TH / kWave; ++i) m = fmaxf(m, red[i]);
-    }
-    float s = m / 127.f;
-    const bool zero = !(s >= 1.17549435e-38f) || m == INFINITY;
-    if (threadIdx.x == 0) scale[row] = m == INFINITY ? NAN : zero ? 0.f : s;
+    for (int64_t j = threadIdx.x; j < K; j += 256) m = fmaxf(m, magnitude(to_f32(p[j])));
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const RowScale s = row_scale(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    if (threadIdx.x == 0) scale[row] = s.out;
     uint32_t *out = reinterpret_cast<uint32_t *>(codes + row * ldc);
-    for (int64_t c = threadIdx.x; c < ldc / 4; c += TH) {
+    for (int64_t c = threadIdx.x; c < ldc / 4; c += 256) {
         uint32_t w = 0;
-        if (!zero)
+        if (s.s != 0.f)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t j = 4 * c + e;
-                if (j < K) {
-                    const float q = fminf(fmaxf(rintf(to_f32(p[j]) / s), -127.f), 127.f);
-                    w |= ((uint32_t)(int)q & 255u) << (8 * e);
-                }
-            }
+            for (int e = 0; e < 4; ++e)
+                if (4 * c + e < K) w |= code_of(to_f32(p[4 * c + e]), s.s) << (8 * e);
         out[c] = w;
     }
+}
+
+template <class T>
+static int launch_quantize(const T *x, int64_t ldx, int64_t n, int64_t K, int8_t *codes, int64_t ldc, float *scale, hipStream_t s) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const bool wide = on_16(x) && ldx * (int64_t)sizeof(T) % 16 == 0;
+    auto blocks = [&](int per) { return dim3((unsigned)((n + per - 1) / per)); };
+    if (wide && ldc <= 32 * E) hipLaunchKernelGGL((quantize_kernel<T, 32, 1>), blocks(8), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else if (wide && ldc <= 128 * E) hipLaunchKernelGGL((quantize_kernel<T, 64, 2>), blocks(4), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else if (wide && ldc <= 1024 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 4>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else if (wide && ldc <= 4096 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 16>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else hipLaunchKernelGGL((quantize_any_kernel<T>), blocks(1), dim3(256), 0, s, x, ldx, K, codes, ldc, scale);
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
 }
 
 // ---- the product ---------------------------------------------------------------------------------------------------------
@@ -71,10 +138,12 @@ struct ScoreArgs {
     int kc;        // chunks of 16 bytes in a row of codes
     void *S;
     int64_t lds;
+    const void *u;  // rows that a kernel makes the codes of for itself (then ldu counts their elements)
+    int K;
 };
 
 // A 128 x 128 tile of S per workgroup of four waves (64 x 64 each: 2 x 2 tiles of 32 x 32); K in steps of 128 bytes, both
-// operands' steps staged in LDS (rows of 128 bytes; 16-byte chunk c of row r at slot c ^ (r & 7), so that the 32 rows a
+// operands' steps staged in LDS (rows of 128 bytes; 16-byte chunk c of row r at slot c ^ (r / 2 % 8), so that any 16 rows a
 // fragment read touches spread over the banks), the next step in flight in registers.
 template <class TO>
 __global__ __launch_bounds__(256) void score_i8_kernel(const ScoreArgs a) {
@@ -105,8 +174,8 @@ __global__ __launch_bounds__(256) void score_i8_kernel(const ScoreArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int r = sr + 32 * q;
-            lu[r * 8 + (sc ^ (r & 7))] = ru[q];
-            li[r * 8 + (sc ^ (r & 7))] = ri[q];
+            lu[r * 8 + (sc ^ ((r >> 1) & 7))] = ru[q];
+            li[r * 8 + (sc ^ ((r >> 1) & 7))] = ri[q];
         }
         __syncthreads();
         if (t + 1 < steps) fetch(t + 1);
@@ -115,7 +184,7 @@ __global__ __launch_bounds__(256) void score_i8_kernel(const ScoreArgs a) {
             i32x4 fu[2], fi[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int r = 32 * q + m, c = (2 * k + h) ^ (r & 7);
+                const int r = 32 * q + m, c = (2 * k + h) ^ ((r >> 1) & 7);
                 fu[q] = lu[(wu + r) * 8 + c];
                 fi[q] = li[(wi + r) * 8 + c];
             }
@@ -141,8 +210,381 @@ __global__ __launch_bounds__(256) void score_i8_kernel(const ScoreArgs a) {
     }
 }
 
+// Short rows (K <= 32 KS): the scores are written at the rate of the stores and everything else has to hide behind them.  A workgroup
+// keeps 32 users' codes in registers and walks item tiles of TB bytes of scores per row: each wave multiplies 32 items' codes at a time,
+// taken straight from the table, and puts its scores into LDS, every row shifted by its distance from a 128-byte line.  Whole lines then
+// leave as 16-byte stores of consecutive lanes (1 KB of a row per wave and store at TB = 2048), whatever the row stride; what a tile leaves
+// over of a row's last line (less than LINE scores) moves to the front of the row for the next tile.
+template <class TO, int KS, int TB>
+__global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel(const ScoreArgs a, int tiles_per_walk) {
+    constexpr int E = 16 / (int)sizeof(TO), TILE = TB / (int)sizeof(TO), LINE = 128 / (int)sizeof(TO), PITCH = TILE + LINE;
+    __shared__ alignas(16) TO buf[32 * PITCH];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 31, h = lane >> 5;
+    const int64_t b0 = (int64_t)blockIdx.y * 32;
+    const int64_t t0 = (int64_t)blockIdx.x * tiles_per_walk, t1 = min(t0 + tiles_per_walk, (a.n + TILE - 1) / TILE);
+    const int64_t js = t0 * TILE, je = min(t1 * TILE, a.n);
+    TO *S = (TO *)a.S + b0 * a.lds;
+    const int rows = (int)min<int64_t>(32, a.B - b0);
+    // row r starts (off0 + r step) mod LINE scores behind a line, and so does every tile of it (TILE is whole lines)
+    const unsigned off0 = (unsigned)((reinterpret_cast<uintptr_t>(S) / sizeof(TO)) % LINE), step = (unsigned)(a.lds % LINE);
+    i32x4 fu[KS];
+    const i32x4 *pu = reinterpret_cast<const i32x4 *>(a.qu + min(b0 + m, a.B - 1) * a.ldu) + h;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) fu[k] = pu[2 * k];
+    float su[16];
+    unsigned at[16];  // where this lane's item of sub-tile 0 goes, for each of its 16 rows
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const unsigned row = (r & 3) + 8 * (r >> 2) + 4 * h;
+        su[r] = a.su[min<int64_t>(b0 + row, a.B - 1)];
+        at[r] = row * PITCH + ((off0 + row * step) & (LINE - 1)) + w * 32 + m;
+    }
+    i32x4 fi[KS];
+    float si;
+    auto fetch = [&](int64_t sub) {  // sub-tiles of 128 items, 32 for each wave
+        const int64_t j = min(sub * 128 + w * 32 + m, a.n - 1);
+        const i32x4 *p = reinterpret_cast<const i32x4 *>(a.qi + j * a.ldi);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) fi[k] = p[min(2 * k + h, a.kc - 1)];  // behind the row's end the users' codes are zero
+        si = a.si[j];
+    };
+    // the scores of a row's last piece of a line: LINE of them from (threadIdx.x / (LINE / KEEP)), KEEP for each thread
+    constexpr int KEEP = 32 * LINE / 256;
+    const unsigned krow = threadIdx.x / (LINE / KEEP), kcol = threadIdx.x % (LINE / KEEP) * KEEP;
+    fetch(t0 * (TILE / 128));
+    for (int64_t t = t0; t < t1; ++t) {
+#pragma unroll
+        for (int u = 0; u < TILE / 128; ++u) {
+            i32x16 acc = {};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fu[k], fi[k], acc, 0, 0, 0);
+            const float sj = si;
+            if (u + 1 < TILE / 128 || t + 1 < t1) fetch(t * (TILE / 128) + u + 1);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) buf[at[r] + u * 128] = from_f32<TO>((float)acc[r] * su[r] * sj);
+        }
+        __syncthreads();
+        const bool first = t == t0, last = t + 1 == t1;
+        constexpr int L = TILE / E;  // lanes that store a row's lines of one tile
+#pragma unroll
+        for (int q = 0; q < 32 / (256 / L); ++q) {
+            const unsigned row = q * (256 / L) + threadIdx.x / L;
+            const int64_t line = t * TILE - (int)((off0 + row * step) & (LINE - 1));  // the column at the row's front in LDS
+            if ((int)row >= rows) continue;
+            TO *to = S + row * a.lds + line;
+            const TO *from = &buf[row * PITCH];
+            const int lo = first ? (int)(js - line) : 0, hi = last ? (int)(je - line) : TILE;
+            for (int c = threadIdx.x % L * E; c < hi; c += TILE) {
+                if (c >= lo && c + E <= hi) {
+                    __builtin_nontemporal_store(*reinterpret_cast<const i32x4 *>(from + c), reinterpret_cast<i32x4 *>(to + c));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (c + e >= lo && c + e < hi) to[c + e] = from[c + e];
+                }
+            }
+        }
+        const Vec<TO, KEEP> keep = *reinterpret_cast<const Vec<TO, KEEP> *>(&buf[krow * PITCH + TILE + kcol]);
+        __syncthreads();
+        const unsigned ph = (off0 + krow * step) & (LINE - 1);
+#pragma unroll
+        for (int e = 0; e < KEEP; ++e)
+            if (kcol + e < ph) buf[krow * PITCH + kcol + e] = keep.v[e];
+    }
+}
+
+template <class TO, int KS, int TB>
+static int launch_short(const ScoreArgs &a, int64_t resident, hipStream_t s) {
+    constexpr int TILE = TB / (int)sizeof(TO);
+    const int64_t tiles = (a.n + TILE - 1) / TILE, panels = (a.B + 31) / 32;
+    // once round the workgroups that fit the chip, and walks of at least two tiles (their ends store pieces of lines)
+    int64_t walks = std::max<int64_t>(1, std::min<int64_t>((tiles + 1) / 2, resident / panels));
+    const int per = (int)((tiles + walks - 1) / walks);
+    walks = (tiles + per - 1) / per;
+    for (int64_t y0 = 0; y0 < panels; y0 += 65535) {  // (a grid's y dimension ends at 65 535)
+        ScoreArgs p = a;
+        p.qu += y0 * 32 * a.ldu, p.su += y0 * 32, p.B -= y0 * 32;
+        p.S = (TO *)a.S + y0 * 32 * a.lds;
+        hipLaunchKernelGGL((score_i8_short_kernel<TO, KS, TB>), dim3((unsigned)walks, (unsigned)std::min<int64_t>(65535, panels - y0)), dim3(256), 0, s, p, per);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+// 2 KB of a row per tile where that leaves every CU work; else 512 bytes: four times the workgroups.
+template <class TO, int KS>
+static int launch_short(const ScoreArgs &a, hipStream_t s) {
+    const int64_t panels = (a.B + 31) / 32, lines = (a.n * (int64_t)sizeof(TO) + 2047) / 2048;
+    return panels * lines >= 1024 ? launch_short<TO, KS, 2048>(a, 512, s) : launch_short<TO, KS, 512>(a, 1024, s);
+}
+
+// Few users (B <= 16 UT): the table is read once and everything else is small.  16 x 16 tiles straight from the rows, no staging: a
+// wave's load touches 64 bytes of each of 16 items' rows.  KW waves of a workgroup share 16 IT items and split K (their sums meet in LDS);
+// the other 4 / KW have items of their own.
+// TU other than void: the users' rows are a.u, of that type and at most kOwnCodes values in all; every workgroup makes their codes for
+// itself in LDS, and the call is one launch.
+constexpr int kOwnCodes = 8192;
+
+template <class TO, class TU, int UT, int IT, int KW>
+__global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
+    constexpr int U = 4;  // steps of 64 bytes in flight
+    constexpr bool OWN = !std::is_void_v<TU>;
+    // a row of codes: K rounded up to 64, and 16 more bytes so that the 16 rows of a fragment spread over the banks
+    __shared__ alignas(16) int8_t own[OWN ? kOwnCodes + 16 * 80 : 16];
+    __shared__ float own_su[16];
+    const int pitch = (a.kc + 3) / 4 * 64 + 16;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int64_t j0 = ((int64_t)blockIdx.x * (4 / KW) + w / KW) * (16 * IT);
+    const i32x4 *pu[UT], *pi[IT];
+#pragma unroll
+    for (int x = 0; x < UT; ++x) {
+        if constexpr (OWN) pu[x] = reinterpret_cast<const i32x4 *>(own + min<int>(m, (int)a.B - 1) * pitch);
+        else pu[x] = reinterpret_cast<const i32x4 *>(a.qu + min<int64_t>(16 * x + m, a.B - 1) * a.ldu);
+    }
+#pragma unroll
+    for (int y = 0; y < IT; ++y) pi[y] = reinterpret_cast<const i32x4 *>(a.qi + min<int64_t>(j0 + 16 * y + m, a.n - 1) * a.ldi);
+    if constexpr (OWN) {
+        static_assert(UT == 1);
+        for (int r = w; r < (int)a.B; r += 4) {  // a wave per row
+            const TU *p = (const TU *)a.u + r * a.ldu;
+            float mag = 0.f;
+            for (int c = lane; c < a.K; c += 64) mag = fmaxf(mag, magnitude(to_f32(p[c])));
+            const RowScale s = row_scale(wave_max(mag));
+            for (int c = lane; c < pitch - 16; c += 64)
+                own[r * pitch + c] = c < a.K && s.s != 0.f ? (int8_t)code_of(to_f32(p[c]), s.s) : (int8_t)0;
+            if (lane == 0) own_su[r] = s.out;
+        }
+        __syncthreads();
+    }
+    const float *su = OWN ? own_su : a.su;
+    const int steps = (a.kc + 3) / 4, per = (steps + KW - 1) / KW;
+    const int s0 = w % KW * per, s1 = min(s0 + per, steps);
+    i32x4 acc[UT][IT] = {};
+    for (int t = s0; t < s1; t += U) {
+        i32x4 fu[U][UT], fi[U][IT];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (t + u < s1) {
+                const int c = 4 * (t + u) + g;  // behind the row's end the users' codes are zero, up to a multiple of 128 bytes
+#pragma unroll
+                for (int x = 0; x < UT; ++x) fu[u][x] = pu[x][c];
+#pragma unroll
+                for (int y = 0; y < IT; ++y) fi[u][y] = pi[y][min(c, a.kc - 1)];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (t + u < s1)
+#pragma unroll
+                for (int x = 0; x < UT; ++x)
+#pragma unroll
+                    for (int y = 0; y < IT; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fu[u][x], fi[u][y], acc[x][y], 0, 0, 0);
+    }
+    if constexpr (KW > 1) {
+        __shared__ i32x4 part[4][UT * IT][64];
+#pragma unroll
+        for (int x = 0; x < UT; ++x)
+#pragma unroll
+            for (int y = 0; y < IT; ++y) part[w][x * IT + y][lane] = acc[x][y];
+        __syncthreads();
+        if (w % KW) return;
+#pragma unroll
+        for (int q = 1; q < KW; ++q)
+#pragma unroll
+            for (int x = 0; x < UT; ++x)
+#pragma unroll
+                for (int y = 0; y < IT; ++y) acc[x][y] += part[w + q][x * IT + y][lane];
+    }
+    TO *S = (TO *)a.S;
+#pragma unroll
+    for (int y = 0; y < IT; ++y) {
+        const int64_t j = j0 + 16 * y + m;
+        if (j >= a.n) continue;
+        const float si = a.si[j];
+#pragma unroll
+        for (int x = 0; x < UT; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t b = 16 * x + 4 * g + r;
+                if (b < a.B) S[b * a.lds + j] = from_f32<TO>((float)acc[x][y][r] * su[b] * si);
+            }
+    }
+}
+
+template <class TO, class TU, int UT>
+static int launch_few(const ScoreArgs &a, hipStream_t s) {
+    if (a.kc >= 64) {  // 1 KB and more of a row: four waves share it
+        if (a.n <= 16 * 2048) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), dim3((unsigned)((a.n + 31) / 32)), dim3(256), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 1>), dim3((unsigned)((a.n + 127) / 128)), dim3(256), 0, s, a);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+// 16 bytes per lane from base + off to the LDS bytes dst + 16 lane.  (m0 is this kernel's to use: nothing the compiler emits in it needs it.)
+__device__ __forceinline__ void dma16(const void *base, uint32_t off, unsigned dst) {
+    asm volatile(
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %1"
+        :
+        : "v"(off), "s"(base), "s"(dst)
+        : "memory");
+}
+
+// Large products: a 256 x 256 tile of S per workgroup, one wave per SIMD with 128 x 128 of it (4 x 4 accumulators of 32 x 32), K in
+// steps of 128 bytes through two LDS stages of 64 KB that LDS-DMA fills.  A step is four slices of 32 bytes: while a slice's
+// sixteen products run, the next slice's eight fragments are read; the barrier that hands over a stage stands in front of the last
+// slice's products, so that the next stage's first fragments arrive under them.  Chunk c of row r lies at slot c ^ (r / 2 % 8): any 16 rows' fragments cover the 64 banks.
+template <class TO>
+__global__ __launch_bounds__(256, 1) void score_i8_wide_kernel(const ScoreArgs a, int gx, int gy) {
+    constexpr int STAGE = 2 * 256 * 128;
+    __shared__ alignas(16) int8_t lds[2 * STAGE];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, h = lane >> 5;
+    // workgroup i runs on XCD i % 8: give each XCD a run of tiles, four user tiles deep, so that its L2 sees few rows at a time
+    const int total = gx * gy, q8 = total / 8, r8 = total % 8, xcd = blockIdx.x % 8;
+    const int t = xcd * q8 + min(xcd, r8) + blockIdx.x / 8;
+    const int group = t / (4 * gx), y0 = group * 4, deep = min(4, gy - y0), in = t - group * 4 * gx;
+    const int64_t b0 = (int64_t)(y0 + in % deep) * 256, j0 = (int64_t)(in / deep) * 256;
+    const int steps = (a.kc + 7) / 8;
+    // this wave fills rows 64 w .. 64 w + 63 of both operands, eight rows per request
+    const int sc = (lane & 7) ^ (lane >> 4);  // its chunk in rows of an even q; ^ 4 in those of an odd one
+    const int8_t *bu = a.qu + b0 * a.ldu, *bi = a.qi + j0 * a.ldi;
+    uint32_t ou[8], oi[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const int r = 64 * w + 8 * q + (lane >> 3);
+        ou[q] = (uint32_t)(min<int64_t>(r, a.B - 1 - b0) * a.ldu) + 16 * (sc ^ (q & 1) * 4);
+        oi[q] = (uint32_t)(min<int64_t>(r, a.n - 1 - j0) * a.ldi) + 16 * (sc ^ (q & 1) * 4);
+    }
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t *)lds;
+    // behind a row's end: the users' codes are zero there, the items' row ends at its last whole chunk
+    const int last = a.kc - 1 - 8 * (steps - 1);
+    const uint32_t back[2] = {16u * (uint32_t)max(0, sc - last), 16u * (uint32_t)max(0, (sc ^ 4) - last)};
+    auto fill = [&](int step, auto part) {  // a quarter of a stage: two requests for either operand
+        const unsigned to = lds0 + (step & 1) * STAGE + w * 8192;
+        const int8_t *pu = bu + (int64_t)step * 128, *pi = bi + (int64_t)step * 128;
+        const bool end = step + 1 == steps;
+        constexpr int q = 2 * decltype(part)::value;
+        dma16(pu, ou[q], to + q * 1024);
+        dma16(pu, ou[q + 1], to + q * 1024 + 1024);
+        dma16(pi, oi[q] - (end ? back[0] : 0u), to + STAGE / 2 + q * 1024);
+        dma16(pi, oi[q + 1] - (end ? back[1] : 0u), to + STAGE / 2 + q * 1024 + 1024);
+    };
+    constexpr std::integral_constant<int, 0> p0;
+    constexpr std::integral_constant<int, 1> p1;
+    constexpr std::integral_constant<int, 2> p2;
+    constexpr std::integral_constant<int, 3> p3;
+    auto fill_all = [&](int step) { fill(step, p0), fill(step, p1), fill(step, p2), fill(step, p3); };
+    i32x16 acc[4][4] = {};
+    i32x4 f0[8], f1[8];
+    const int wu = (w >> 1) * 128, wi = (w & 1) * 128;
+    auto read = [&](i32x4(&to)[8], int step, int k) {
+        const int8_t *from = lds + (step & 1) * STAGE + (((2 * k + h) ^ ((m >> 1) & 7)) * 16);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) to[x] = *reinterpret_cast<const i32x4 *>(from + (wu + 32 * x + m) * 128);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) to[4 + y] = *reinterpret_cast<const i32x4 *>(from + STAGE / 2 + (wi + 32 * y + m) * 128);
+    };
+    auto multiply = [&](const i32x4(&g)[8], auto part) {
+        constexpr int x = decltype(part)::value;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(g[x], g[4 + y], acc[x][y], 0, 0, 0);
+    };
+    auto slice = [&](const i32x4(&g)[8], i32x4(&next)[8], int step, int k) {  // read (step, k) under the products of g
+        read(next, step, k);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(g, p0), multiply(g, p1), multiply(g, p2), multiply(g, p3);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    fill_all(0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (steps > 1) fill_all(1);
+    read(f0, 0, 0);
+    for (int st = 0; st < steps; ++st) {
+        slice(f0, f1, st, 1);
+        slice(f1, f0, st, 2);
+        slice(f0, f1, st, 3);
+        // The next stage is filled, and nobody reads this one any more: its refill goes out between the products.  (After the last
+        // step the fragments read here are of no use, but they are read all the same: no wait then depends on a branch.)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        read(f0, st + 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool more = st + 2 < steps;
+        multiply(f1, p0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) fill(st + 2, p0);
+        multiply(f1, p1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) fill(st + 2, p1);
+        multiply(f1, p2);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) fill(st + 2, p2);
+        multiply(f1, p3);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) fill(st + 2, p3);
+    }
+    __syncthreads();
+    // the wave's tile through its quarter of the LDS, a strip of 32 users at a time, and out in rows
+    constexpr int E = 16 / (int)sizeof(TO), L = 128 / E;
+    TO *strip = reinterpret_cast<TO *>(lds + w * (STAGE / 2));
+    TO *S = (TO *)a.S;
+    const bool wide = (reinterpret_cast<uintptr_t>(S) | (uintptr_t)(a.lds * (int64_t)sizeof(TO))) % 16 == 0;
+    float si[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) si[y] = a.si[min<int64_t>(j0 + wi + 32 * y + m, a.n - 1)];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const int64_t bx = b0 + wu + 32 * x;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = (r & 3) + 8 * (r >> 2) + 4 * h;
+            const float su = a.su[min<int64_t>(bx + row, a.B - 1)];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) strip[row * 128 + 32 * y + m] = from_f32<TO>((float)acc[x][y][r] * su * si[y]);
+        }
+        if (wide) {
+#pragma unroll
+            for (int q = 0; q < 32 * L / 64; ++q) {
+                const int row = q * (64 / L) + lane / L, c = lane % L * E;
+                const int64_t j = j0 + wi + c;
+                if (bx + row < a.B) {
+                    TO *to = S + (bx + row) * a.lds + j;
+                    const TO *from = strip + row * 128 + c;
+                    if (j + E <= a.n) {
+                        *reinterpret_cast<i32x4 *>(to) = *reinterpret_cast<const i32x4 *>(from);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (j + e < a.n) to[e] = from[e];
+                    }
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int q = 0; q < 64; ++q) {
+                const int row = q >> 1, c = (q & 1) * 64 + lane;
+                const int64_t j = j0 + wi + c;
+                if (bx + row < a.B && j < a.n) S[(bx + row) * a.lds + j] = strip[row * 128 + c];
+            }
+        }
+    }
+}
+
 template <class TO>
 static int launch_score(const ScoreArgs &a, hipStream_t s) {
+    if (a.B <= 16) return launch_few<TO, void, 1>(a, s);
+    if (a.kc <= 4) return launch_short<TO, 2>(a, s);
+    if (a.kc <= 8) return launch_short<TO, 4>(a, s);
+    if (a.B <= 32) return launch_few<TO, void, 2>(a, s);
+    if (a.B <= 64) return launch_few<TO, void, 4>(a, s);
+    const int64_t gx = (a.n + 255) / 256, gw = (a.B + 255) / 256;
+    if (gx * gw >= 192 && gx * gw < (1 << 30) && a.ldu <= 1 << 23 && a.ldi <= 1 << 23) {  // (32-bit offsets inside a tile)
+        hipLaunchKernelGGL((score_i8_wide_kernel<TO>), dim3((unsigned)(gx * gw)), dim3(256), 0, s, a, (int)gx, (int)gw);
+        RBG_HIP(hipGetLastError());
+        return RBG_OK;
+    }
     const int64_t gy = (a.B + 127) / 128;
     for (int64_t y0 = 0; y0 < gy; y0 += 65535) {  // (a grid's y dimension ends at 65 535)
         ScoreArgs p = a;
@@ -156,6 +598,19 @@ static int launch_score(const ScoreArgs &a, hipStream_t s) {
 }
 
 constexpr int64_t kMaxK = 131071;  // 128 x 128 x K < 2^31
+
+// What both product entries ask of the items and the scores.
+static int check_score(int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n, int64_t K, const void *S, int64_t lds, int out_dtype) {
+    if (!elem_ok(out_dtype)) return fail(RBG_EINVAL, "out_dtype = %d", out_dtype);
+    if (B < 0 || n < 0 || K <= 0 || ldi < K || lds < n)
+        return fail(RBG_ESHAPE, "B = %lld, n = %lld, K = %lld, ldi = %lld, lds = %lld", (long long)B, (long long)n, (long long)K, (long long)ldi, (long long)lds);
+    if (ldi % 16) return fail(RBG_EINVAL, "ldi = %lld is not a multiple of 16", (long long)ldi);
+    if (K > kMaxK) return fail(RBG_EUNSUPPORTED, "K = %lld: sums of more than 131071 products may pass 32 bits", (long long)K);
+    if (n > 0x7fffffffll || B > 0x7fffffffll) return fail(RBG_EUNSUPPORTED, "rows beyond 2^31");
+    if (B && n && (!qi || !si || !S)) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(qi) || reinterpret_cast<uintptr_t>(S) % elem_size(out_dtype)) return fail(RBG_EINVAL, "codes need 16-byte alignment, scores that of their type");
+    return RBG_OK;
+}
 
 }  // namespace rbg
 
@@ -174,28 +629,52 @@ int rbg_quantize_rows_i8(const void *x, int64_t ldx, int dtype, int64_t n, int64
     if (!on_16(codes) || reinterpret_cast<uintptr_t>(x) % elem_size(dtype)) return fail(RBG_EINVAL, "codes need 16-byte alignment, rows that of their type");
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
-        if (K <= 512) hipLaunchKernelGGL((quantize_kernel<E, 64>), dim3((unsigned)n), dim3(64), 0, (hipStream_t)stream, (const E *)x, ldx, K, codes, ldc, scale);
-        else hipLaunchKernelGGL((quantize_kernel<E, 256>), dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, (const E *)x, ldx, K, codes, ldc, scale);
-        RBG_HIP(hipGetLastError());
-        return (int)RBG_OK;
+        return launch_quantize<E>((const E *)x, ldx, n, K, codes, ldc, scale, (hipStream_t)stream);
     });
 }
 
 int rbg_score_i8(const int8_t *qu, int64_t ldu, const float *su, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n,
                  int64_t K, void *S, int64_t lds, int out_dtype, void *stream) {
     clear_error();
-    if (!elem_ok(out_dtype)) return fail(RBG_EINVAL, "out_dtype = %d", out_dtype);
-    if (B < 0 || n < 0 || K <= 0 || ldu < K || ldi < K || lds < n)
-        return fail(RBG_ESHAPE, "B = %lld, n = %lld, K = %lld, ldu = %lld, ldi = %lld, lds = %lld", (long long)B, (long long)n, (long long)K, (long long)ldu, (long long)ldi, (long long)lds);
-    if (ldu % 128 || ldi % 16) return fail(RBG_EINVAL, "ldu = %lld is not a multiple of 128, or ldi = %lld of 16", (long long)ldu, (long long)ldi);
-    if (K > kMaxK) return fail(RBG_EUNSUPPORTED, "K = %lld: sums of more than 131071 products may pass 32 bits", (long long)K);
-    if (n > 0x7fffffffll || B > 0x7fffffffll) return fail(RBG_EUNSUPPORTED, "rows beyond 2^31");
+    if (int rc = check_score(B, qi, ldi, si, n, K, S, lds, out_dtype)) return rc;
+    if (ldu < K) return fail(RBG_ESHAPE, "K = %lld, ldu = %lld", (long long)K, (long long)ldu);
+    if (ldu % 128) return fail(RBG_EINVAL, "ldu = %lld is not a multiple of 128", (long long)ldu);
     if (B == 0 || n == 0) return RBG_OK;
-    if (!qu || !su || !qi || !si || !S) return fail(RBG_EINVAL, "NULL pointer");
-    if (!on_16(qu) || !on_16(qi) || reinterpret_cast<uintptr_t>(S) % elem_size(out_dtype))
-        return fail(RBG_EINVAL, "codes need 16-byte alignment, scores that of their type");
-    const ScoreArgs a{qu, qi, ldu, ldi, su, si, B, n, (int)((K + 15) / 16), S, lds};
+    if (!qu || !su) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(qu)) return fail(RBG_EINVAL, "codes need 16-byte alignment");
+    const ScoreArgs a{qu, qi, ldu, ldi, su, si, B, n, (int)((K + 15) / 16), S, lds, nullptr, (int)K};
     return with_elem(out_dtype, [&](auto t) { return launch_score<decltype(t)>(a, (hipStream_t)stream); });
+}
+
+int rbg_score_rows_i8_workspace(int64_t B, int64_t K, int64_t *bytes) {
+    clear_error();
+    if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
+    if (B < 0 || K <= 0) return fail(RBG_ESHAPE, "B = %lld, K = %lld", (long long)B, (long long)K);
+    const int64_t ldc = (K + 127) / 128 * 128;
+    *bytes = B * ldc + (4 * B + 15) / 16 * 16;
+    return RBG_OK;
+}
+
+int rbg_score_rows_i8(const void *u, int64_t ldu, int dtype, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n, int64_t K,
+                      void *S, int64_t lds, int out_dtype, void *workspace, void *stream) {
+    clear_error();
+    if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
+    if (int rc = check_score(B, qi, ldi, si, n, K, S, lds, out_dtype)) return rc;
+    if (ldu < K) return fail(RBG_ESHAPE, "K = %lld, ldu = %lld", (long long)K, (long long)ldu);
+    if (B == 0 || n == 0) return RBG_OK;
+    if (!u || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if (!on_16(workspace) || reinterpret_cast<uintptr_t>(u) % elem_size(dtype)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned, or rows not to their type");
+    const int64_t ldc = (K + 127) / 128 * 128;
+    int8_t *qu = (int8_t *)workspace;
+    float *su = (float *)(qu + B * ldc);
+    if (B <= 16 && B * K <= kOwnCodes) {
+        const ScoreArgs a{nullptr, qi, ldu, ldi, nullptr, si, B, n, (int)((K + 15) / 16), S, lds, u, (int)K};
+        return with_elem(out_dtype, [&](auto o) {
+            return with_elem(dtype, [&](auto t) { return launch_few<decltype(o), decltype(t), 1>(a, (hipStream_t)stream); });
+        });
+    }
+    if (int rc = rbg_quantize_rows_i8(u, ldu, dtype, B, K, qu, ldc, su, stream)) return rc;
+    return rbg_score_i8(qu, ldc, su, B, qi, ldi, si, n, K, S, lds, out_dtype, stream);
 }
 
 }  // extern "C"

@@ -8,6 +8,7 @@ for values that live on the device.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -18,25 +19,19 @@ from ._lib import check, lib
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-class _On:
-    """The device of ``t`` as the current one, where it is not already."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _call(fn, t, *args):
+    """``fn(*args, stream)`` on the current stream of ``t``'s device, which is made the current device where it is not."""
+    index = t.get_device()
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc)
 
 
 def _rows(t, name):
@@ -47,6 +42,8 @@ def _rows(t, name):
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t
     n, d = t.shape
     if d > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < d:
         t = t.contiguous()
@@ -59,10 +56,10 @@ def _ld(t):
 
 def _like(t, of, name, shape, dtype):
     """``t`` as a contiguous ``dtype`` tensor of that shape on ``of``'s device; other devices are refused, never copied from."""
-    if t.device != of.device:
+    if t.get_device() != of.get_device():
         raise RuntimeError(f"{name} is on {t.device}, expected {of.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
             raise TypeError(f"{name} must hold whole numbers, got {t.dtype}")
@@ -74,10 +71,16 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _workspace(fn, *args, device):
+@functools.lru_cache(maxsize=1024)
+def _bytes(fn, *sizes):
     nbytes = _lib.c_i64()
-    check(fn(*args, ctypes.byref(nbytes)))
-    return torch.empty(max(nbytes.value, 16), dtype=torch.uint8, device=device)
+    check(getattr(lib, fn)(*sizes, ctypes.byref(nbytes)))
+    return max(nbytes.value, 16)
+
+
+def _workspace(of, fn, *sizes):
+    """A workspace of the call's own, on the current stream (the caching allocator hands it out in stream order)."""
+    return of.new_empty(_bytes(fn, *sizes), dtype=torch.uint8)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -85,11 +88,10 @@ def _workspace(fn, *args, device):
 # ---------------------------------------------------------------------------------------------------------------------
 def _embedding(table, ids, scale):
     n, d = ids.numel(), table.shape[1]
-    out = torch.empty((*ids.shape, d), dtype=table.dtype, device=table.device)
+    out = table.new_empty((*ids.shape, d), dtype=table.dtype)
     if n and d:
-        with _On(table):
-            check(lib.rbg_embedding(table.data_ptr(), _ld(table), table.shape[0], d, _DTYPES[table.dtype], ids.data_ptr(), n, scale,
-                                    out.data_ptr(), d, _stream(table)))
+        _call(lib.rbg_embedding, table, table.data_ptr(), _ld(table), table.shape[0], d, _DTYPES[table.dtype], ids.data_ptr(), n, scale,
+              out.data_ptr(), d)
     return out
 
 
@@ -107,14 +109,12 @@ def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=Non
     out_dtype = out_dtype or grad.dtype
     if out_dtype not in (grad.dtype, torch.float32):
         raise TypeError(f"out_dtype must be {grad.dtype} or float32, got {out_dtype}")
-    out = torch.empty((n_rows, d), dtype=out_dtype, device=grad.device)
+    out = grad.new_empty((n_rows, d), dtype=out_dtype)
     if n_rows and d:
         n = ids.numel()
-        work = _workspace(lib.rbg_embedding_grad_workspace, n, n_rows, d, device=grad.device)
-        with _On(grad):
-            check(lib.rbg_embedding_grad(grad.data_ptr(), _ld(grad), _DTYPES[grad.dtype], ids.data_ptr(), n, n_rows, d, float(scale),
-                                         -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _DTYPES[out_dtype],
-                                         work.data_ptr(), _stream(grad)))
+        work = _workspace(grad, "rbg_embedding_grad_workspace", n, n_rows, d)
+        _call(lib.rbg_embedding_grad, grad, grad.data_ptr(), _ld(grad), _DTYPES[grad.dtype], ids.data_ptr(), n, n_rows, d, float(scale),
+              -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _DTYPES[out_dtype], work.data_ptr())
     return out
 
 
@@ -156,15 +156,12 @@ def _teacher(logits, idx, val):
 
 def _distill(logits, idx, val, temperature, row_weight, want_stats, want_grad):
     n, v = logits.shape
-    dev = logits.device
-    loss = torch.empty(n, dtype=torch.float32, device=dev)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if want_stats else None
-    grad = torch.empty((n, v), dtype=logits.dtype, device=dev) if want_grad else None
-    work = _workspace(lib.rbg_distill_topk_workspace, n, v, device=dev)
-    with _On(logits):
-        check(lib.rbg_distill_topk(logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], n, v, idx.data_ptr(), val.data_ptr(), idx.shape[1],
-                                   temperature, _ptr(row_weight), loss.data_ptr(), _ptr(stats), _ptr(grad), v, work.data_ptr(),
-                                   _stream(logits)))
+    loss = logits.new_empty(n, dtype=torch.float32)
+    stats = logits.new_empty((n, 2), dtype=torch.float32) if want_stats else None
+    grad = logits.new_empty((n, v), dtype=logits.dtype) if want_grad else None
+    work = _workspace(logits, "rbg_distill_topk_workspace", n, v)
+    _call(lib.rbg_distill_topk, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], n, v, idx.data_ptr(), val.data_ptr(),
+          idx.shape[1], temperature, _ptr(row_weight), loss.data_ptr(), _ptr(stats), _ptr(grad), v, work.data_ptr())
     return loss, stats, grad
 
 
@@ -182,11 +179,9 @@ class _DistillTopk(torch.autograd.Function):
         logits, idx, val, stats = ctx.saved_tensors
         n, v = logits.shape
         g = g.to(torch.float32).contiguous()
-        grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
-        with _On(logits):
-            check(lib.rbg_distill_topk_backward(logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], n, v, idx.data_ptr(), val.data_ptr(),
-                                                idx.shape[1], ctx.temperature, stats.data_ptr(), g.data_ptr(), grad.data_ptr(), v,
-                                                _stream(logits)))
+        grad = logits.new_empty((n, v), dtype=logits.dtype)
+        _call(lib.rbg_distill_topk_backward, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], n, v, idx.data_ptr(),
+              val.data_ptr(), idx.shape[1], ctx.temperature, stats.data_ptr(), g.data_ptr(), grad.data_ptr(), v)
         return grad, None, None, None
 
 
@@ -221,12 +216,11 @@ class _TokenLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets):
         m, v = logits.shape
-        logp = torch.empty(m, dtype=torch.float32, device=logits.device)
-        stats = torch.empty((m, 2), dtype=torch.float32, device=logits.device)
-        work = _workspace(lib.rbg_token_logp_workspace, m, v, device=logits.device)
-        with _On(logits):
-            check(lib.rbg_token_logp(logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(), logp.data_ptr(),
-                                     stats.data_ptr(), work.data_ptr(), _stream(logits)))
+        logp = logits.new_empty(m, dtype=torch.float32)
+        stats = logits.new_empty((m, 2), dtype=torch.float32)
+        work = _workspace(logits, "rbg_token_logp_workspace", m, v)
+        _call(lib.rbg_token_logp, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(), logp.data_ptr(),
+              stats.data_ptr(), work.data_ptr())
         ctx.save_for_backward(logits, targets, stats)
         return logp
 
@@ -236,10 +230,9 @@ class _TokenLogp(torch.autograd.Function):
         logits, targets, stats = ctx.saved_tensors
         m, v = logits.shape
         g = g.to(torch.float32).contiguous()
-        grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
-        with _On(logits):
-            check(lib.rbg_token_logp_backward(logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(),
-                                              stats.data_ptr(), g.data_ptr(), grad.data_ptr(), v, _stream(logits)))
+        grad = logits.new_empty((m, v), dtype=logits.dtype)
+        _call(lib.rbg_token_logp_backward, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(),
+              stats.data_ptr(), g.data_ptr(), grad.data_ptr(), v)
         return grad, None
 
 
@@ -261,11 +254,10 @@ def _pairs(of, offsets, ref):
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, offsets, ref, pairs, beta, smoothing):
-        loss = torch.empty(pairs, dtype=torch.float32, device=logp.device)
-        margin = torch.empty_like(loss)
-        with _On(logp):
-            check(lib.rbg_preference_loss(logp.data_ptr(), logp.shape[0], offsets.data_ptr(), pairs, ref.data_ptr(), beta, smoothing,
-                                          loss.data_ptr(), margin.data_ptr(), _stream(logp)))
+        loss = logp.new_empty(pairs, dtype=torch.float32)
+        margin = logp.new_empty(pairs, dtype=torch.float32)
+        _call(lib.rbg_preference_loss, logp, logp.data_ptr(), logp.shape[0], offsets.data_ptr(), pairs, ref.data_ptr(), beta, smoothing,
+              loss.data_ptr(), margin.data_ptr())
         ctx.save_for_backward(margin, offsets)
         ctx.rest = logp.shape[0], pairs, beta, smoothing
         return loss, margin
@@ -276,10 +268,9 @@ class _PreferenceLoss(torch.autograd.Function):
         margin, offsets = ctx.saved_tensors
         m, pairs, beta, smoothing = ctx.rest
         g_loss, g_margin = (g.to(torch.float32).contiguous() if g is not None else None for g in (g_loss, g_margin))
-        grad = torch.empty(m, dtype=torch.float32, device=margin.device)
-        with _On(margin):
-            check(lib.rbg_preference_loss_backward(margin.data_ptr(), m, offsets.data_ptr(), pairs, beta, smoothing, _ptr(g_loss),
-                                                   _ptr(g_margin), grad.data_ptr(), _stream(margin)))
+        grad = margin.new_empty(m, dtype=torch.float32)
+        _call(lib.rbg_preference_loss_backward, margin, margin.data_ptr(), m, offsets.data_ptr(), pairs, beta, smoothing, _ptr(g_loss),
+              _ptr(g_margin), grad.data_ptr())
         return grad, None, None, None, None, None
 
 
@@ -306,13 +297,12 @@ def preference_grad(logits, targets, offsets, ref_logp, beta=0.1, label_smoothin
     offsets, ref, pairs = _pairs(logits, offsets, ref_logp)
     if pair_weight is not None:
         pair_weight = _like(pair_weight, logits, "pair_weight", (pairs,), torch.float32)
-    loss = torch.empty((2, pairs), dtype=torch.float32, device=logits.device)
-    grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
-    work = _workspace(lib.rbg_preference_grad_workspace, m, v, device=logits.device)
-    with _On(logits):
-        check(lib.rbg_preference_grad(logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(), offsets.data_ptr(), pairs,
-                                      ref.data_ptr(), float(beta), float(label_smoothing), _ptr(pair_weight), loss[0].data_ptr(),
-                                      loss[1].data_ptr(), grad.data_ptr(), v, work.data_ptr(), _stream(logits)))
+    loss = logits.new_empty((2, pairs), dtype=torch.float32)
+    grad = logits.new_empty((m, v), dtype=logits.dtype)
+    work = _workspace(logits, "rbg_preference_grad_workspace", m, v)
+    _call(lib.rbg_preference_grad, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(),
+          offsets.data_ptr(), pairs, ref.data_ptr(), float(beta), float(label_smoothing), _ptr(pair_weight), loss[0].data_ptr(),
+          loss[1].data_ptr(), grad.data_ptr(), v, work.data_ptr())
     return loss[0], loss[1], grad
 
 
@@ -322,11 +312,10 @@ def preference_grad(logits, targets, offsets, ref_logp, beta=0.1, label_smoothin
 def _quantize(x, pad):
     n, k = x.shape
     ldc = (k + pad - 1) // pad * pad
-    codes = torch.empty((n, ldc), dtype=torch.int8, device=x.device)
-    scale = torch.empty(n, dtype=torch.float32, device=x.device)
+    codes = x.new_empty((n, ldc), dtype=torch.int8)
+    scale = x.new_empty(n, dtype=torch.float32)
     if n:
-        with _On(x):
-            check(lib.rbg_quantize_rows_i8(x.data_ptr(), _ld(x), _DTYPES[x.dtype], n, k, codes.data_ptr(), ldc, scale.data_ptr(), _stream(x)))
+        _call(lib.rbg_quantize_rows_i8, x, x.data_ptr(), _ld(x), _DTYPES[x.dtype], n, k, codes.data_ptr(), ldc, scale.data_ptr())
     return codes, scale
 
 
@@ -350,7 +339,7 @@ def _codes(codes, k):
         room = codes.untyped_storage().nbytes() - codes.storage_offset()
         if ld % 16 == 0 and ld >= need and (n - 1) * ld + need <= room:
             return codes, ld
-    padded = torch.zeros((n, need), dtype=torch.int8, device=codes.device)
+    padded = codes.new_zeros((n, need))
     padded[:, :k] = codes
     return padded, need
 
@@ -371,11 +360,10 @@ def score_int8(u, codes, scales, out_dtype=torch.float32):
     if out_dtype not in _DTYPES:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     scales = _like(scales, u, "scales", (n,), torch.float32)
-    out = torch.empty((b, n), dtype=out_dtype, device=u.device)
+    out = u.new_empty((b, n), dtype=out_dtype)
     if b and n:
         codes, ldi = _codes(codes, k)
-        qu, su = _quantize(u, 128)
-        with _On(u):
-            check(lib.rbg_score_i8(qu.data_ptr(), qu.shape[1], su.data_ptr(), b, codes.data_ptr(), ldi, scales.data_ptr(), n, k, out.data_ptr(), n,
-                                   _DTYPES[out_dtype], _stream(u)))
+        work = _workspace(u, "rbg_score_rows_i8_workspace", b, k)
+        _call(lib.rbg_score_rows_i8, u, u.data_ptr(), _ld(u), _DTYPES[u.dtype], b, codes.data_ptr(), ldi, scales.data_ptr(), n, k,
+              out.data_ptr(), n, _DTYPES[out_dtype], work.data_ptr())
     return out

@@ -517,6 +517,50 @@ def test_score_int8(rbg, cuda, b, n, k, dtype, out_dtype):
     scores_check(rbg, u, codes, scales, out_dtype)
 
 
+@pytest.mark.parametrize("b,n,k,out_dtype", [(3500, 3600, 129, F32), (4096, 4096, 1024, BF16), (2050, 8003, 300, F32), (1025, 10241, 257, F16), (256, 49153, 2048, BF16),
+                                             (70, 49000, 64, F32), (2048, 40982, 64, F32), (333, 9001, 100, BF16), (40, 70003, 33, F16)])
+def test_score_int8_many(rbg, cuda, b, n, k, out_dtype):
+    """Sizes that fill the chip with large tiles or with long walks; every score against the same in 64 bits (here on the GPU), and nothing
+    written outside the scores."""
+    g = gen(b + k, cuda)
+    u = torch.randn(b, k, generator=g, device=cuda)
+    codes, scales = rbg.quantize_rows(torch.randn(n, k, generator=g, device=cuda))
+    got = rbg.score_int8(u, codes, scales, out_dtype=out_dtype)
+    q, s = codes_reference(u)
+    ref = torch.matmul(q.to(cuda), codes.double().t().contiguous()) * s.to(cuda)[:, None] * scales.double()[None]
+    within(got, ref, 3.1 * U * ref.abs() + stored(ref, out_dtype) + 2.0 ** -148)
+    # rows of a wider tensor at every offset of a line: the columns beside them keep what they hold
+    qu, su = torch.zeros(b, (k + 127) // 128 * 128, dtype=torch.int8, device=cuda), torch.empty(b, device=cuda)
+    lib = rbg._lib.lib
+    rbg._lib.check(lib.rbg_quantize_rows_i8(u.data_ptr(), k, 0, b, k, qu.data_ptr(), qu.shape[1], su.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    wide = torch.full((b + 1, n + 13), 77.0, dtype=out_dtype, device=cuda)
+    rbg._lib.check(lib.rbg_score_i8(qu.data_ptr(), qu.shape[1], su.data_ptr(), b, codes.data_ptr(), codes.stride(0), scales.data_ptr(), n, k,
+                                    wide.data_ptr() + 5 * wide.element_size(), n + 13, rbg.vocab._DTYPES[out_dtype], torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(wide[:b, 5:n + 5], got)
+    wide[:b, 5:n + 5] = 77.0
+    assert bool(torch.all(wide == 77.0))
+
+
+@pytest.mark.parametrize("b,n,k", [(1, 40982, 128), (1, 77, 1), (5, 1000, 1638), (16, 300, 512), (16, 301, 513), (3, 40000, 2000)])
+@pytest.mark.parametrize("dtype", ALL)
+def test_score_int8_in_one_launch_or_two(rbg, cuda, b, n, k, dtype):
+    """Few users' codes made where they are used, against the same codes made first: the same bits."""
+    g = gen(n, cuda)
+    u = torch.randn(b, k + 1, generator=g, device=cuda).to(dtype)[:, 1:]
+    if b > 2:
+        u[1], u[2, k // 2] = 0.0, math.inf
+    codes, scales = rbg.quantize_rows(torch.randn(n, k, generator=g, device=cuda))
+    qu, su = torch.zeros(b, (k + 127) // 128 * 128, dtype=torch.int8, device=cuda), torch.empty(b, device=cuda)
+    st, lib = torch.cuda.current_stream().cuda_stream, rbg._lib.lib
+    rbg._lib.check(lib.rbg_quantize_rows_i8(u.data_ptr(), k + 1, rbg.vocab._DTYPES[dtype], b, k, qu.data_ptr(), qu.shape[1], su.data_ptr(), st))
+    want = torch.empty(b, n, device=cuda)
+    rbg._lib.check(lib.rbg_score_i8(qu.data_ptr(), qu.shape[1], su.data_ptr(), b, codes.data_ptr(), codes.stride(0), scales.data_ptr(), n, k, want.data_ptr(), n, 0, st))
+    got = rbg.score_int8(u, codes, scales)
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want)) and torch.equal(got.isnan(), want.isnan())
+    if b > 2:
+        assert bool(got[2].isnan().all()) and bool((got[1] == 0).all())
+
+
 def test_score_int8_exact_sums(rbg, cuda):
     """All codes at their ends: sums of 131 071 products of 127 x 127 and 127 x -128 stay whole."""
     k = 131071

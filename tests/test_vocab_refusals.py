@@ -39,6 +39,10 @@ def score(lib, qu=A, ldu=128, su=B, b=2, qi=C, ldi=16, si=B, n=3, k=8, s=D, lds=
     return lib.rbg_score_i8(qu, ldu, su, b, qi, ldi, si, n, k, s, lds, out, None)
 
 
+def score_rows(lib, u=A, ldu=8, dtype=0, b=2, qi=C, ldi=16, si=B, n=3, k=8, s=D, lds=3, out=0, work=W):
+    return lib.rbg_score_rows_i8(u, ldu, dtype, b, qi, ldi, si, n, k, s, lds, out, work, None)
+
+
 REFUSED = [
     (embedding, dict(dtype=3), EINVAL), (embedding, dict(d=0), ESHAPE), (embedding, dict(ldt=7), ESHAPE), (embedding, dict(ldo=7), ESHAPE),
     (embedding, dict(n=-1), ESHAPE), (embedding, dict(ids=None), EINVAL), (embedding, dict(table=None), EINVAL), (embedding, dict(out=P(2)), EINVAL),
@@ -57,6 +61,9 @@ REFUSED = [
     (quantize, dict(x=P(2)), EINVAL), (quantize, dict(scale=None), EINVAL),
     (score, dict(ldu=64), EINVAL), (score, dict(ldi=24), EINVAL), (score, dict(k=131072, ldu=131072, ldi=131072), EUNSUPPORTED), (score, dict(lds=2), ESHAPE),
     (score, dict(qi=P(8)), EINVAL), (score, dict(out=3), EINVAL), (score, dict(k=0), ESHAPE), (score, dict(su=None), EINVAL),
+    (score_rows, dict(dtype=3), EINVAL), (score_rows, dict(out=-1), EINVAL), (score_rows, dict(ldu=7), ESHAPE), (score_rows, dict(work=None), EINVAL),
+    (score_rows, dict(work=P(8)), EINVAL), (score_rows, dict(u=P(2)), EINVAL), (score_rows, dict(k=131072, ldu=131072, ldi=131072), EUNSUPPORTED),
+    (score_rows, dict(lds=2), ESHAPE), (score_rows, dict(n=1 << 31, lds=1 << 31), EUNSUPPORTED), (score_rows, dict(k=0), ESHAPE),
 ]
 
 
@@ -73,14 +80,14 @@ def test_nothing_to_do_is_no_error(rbg):
     assert distill(lib, n=0, z=None) == OK
     assert logp(lib, m=0, z=None) == OK
     assert preference(lib, m=0, pairs=0, z=None) == OK
-    assert quantize(lib, n=0) == OK and score(lib, b=0) == OK and score(lib, n=0, lds=0) == OK
+    assert quantize(lib, n=0) == OK and score(lib, b=0) == OK and score(lib, n=0, lds=0) == OK and score_rows(lib, b=0) == OK
     assert lib.rbg_preference_loss(None, 0, A, 0, None, 0.1, 0.0, None, None, None) == OK
 
 
 def test_workspaces(rbg):
     lib, n = rbg._lib.lib, ctypes.c_int64()
     for fn, args in ((lib.rbg_embedding_grad_workspace, (5, 7, 8)), (lib.rbg_embedding_grad_workspace, (100000, 7, 8)), (lib.rbg_distill_topk_workspace, (3, 50000)),
-                     (lib.rbg_token_logp_workspace, (3, 50000)), (lib.rbg_preference_grad_workspace, (3, 50000))):
+                     (lib.rbg_token_logp_workspace, (3, 50000)), (lib.rbg_score_rows_i8_workspace, (3, 500)), (lib.rbg_preference_grad_workspace, (3, 50000))):
         assert fn(*args, ctypes.byref(n)) == OK and n.value > 0 and n.value % 16 == 0
         assert fn(*args, None) == EINVAL
         assert fn(-1, *args[1:], ctypes.byref(n)) == ESHAPE
