@@ -37,6 +37,17 @@ struct RowShape {
     __device__ __forceinline__ int at(int x) const { return x < head ? x : tail + (x - head); }
 };
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of a gradient.  One that the L2s cannot hold anyway (`nt`) goes past them: written back line by line it would compete with the
+// logits still to be read (2048 x 40 982 bf16, value and gradient: 91.6 us with plain stores, 73.8 us).
+__device__ __forceinline__ void put16(void *p, const void *v, bool nt) {
+    u32x4 x;
+    __builtin_memcpy(&x, v, 16);
+    if (nt) __builtin_nontemporal_store(x, reinterpret_cast<u32x4 *>(p));
+    else *reinterpret_cast<u32x4 *>(p) = x;
+}
+
 struct MaxSum {
     float m, s;
 };
@@ -121,7 +132,7 @@ __device__ __forceinline__ MaxSum scan_row(const T *__restrict__ z, const RowSha
 // z and g may be the same row: an element is read and written by the same thread.
 template <class T, int TH, int U>
 __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &sh, int c0, int c1, bool loose, float m, float c, float a,
-                                          int hot, float more) {
+                                          int hot, float more, bool nt) {
     constexpr int E = RowShape<T>::E;
     const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + sh.head);
     Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
@@ -149,7 +160,7 @@ __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &s
 #pragma unroll
             for (int e = 0; e < E; ++e) v[u].v[e] = from_f32<T>(x[e]);
             if (wide) {
-                out[i] = v[u];
+                put16(out + i, &v[u], nt);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v[u].v[e];
@@ -165,7 +176,7 @@ __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &s
 }
 
 template <class T, int TH>
-__device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, int c1, bool loose) {
+__device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, int c1, bool loose, bool nt) {
     constexpr int E = RowShape<T>::E;
     Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
     const bool wide = on_16_dev(out);
@@ -174,7 +185,7 @@ __device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, in
     for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(0.f);
     for (int i = c0 + threadIdx.x; i < c1; i += TH) {
         if (wide) {
-            out[i] = v;
+            put16(out + i, &v, nt);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v.v[e];
@@ -204,6 +215,7 @@ struct DistillArgs {
     int64_t ldg;
     MaxSum *part;  // [n][S] when a row is split
     float *zt;     // [n][k] when a row is split: the entries' logits (the gradient may overwrite them)
+    bool nt;       // the gradient goes past the caches
 };
 
 struct Entries {
@@ -302,17 +314,32 @@ __global__ __launch_bounds__(TH) void distill_eval_kernel(const DistillArgs a) {
     entries_loss(a, row, sh, st);
 }
 
-// Value and gradient of a row that fits the registers of its workgroup: NC chunks of 16 bytes per thread.
+// The passes over a row in registers each convert its elements anew: kept, the converted ones would take twice the registers of a 16-bit row.
+template <int N>
+__device__ __forceinline__ void forget(u32x4 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+}
+template <class T, int E>
+__device__ __forceinline__ Vec<T, E> as_elems(const u32x4 &v) {
+    Vec<T, E> r;
+    __builtin_memcpy(&r, &v, 16);
+    return r;
+}
+
+// Value and gradient of a row that fits the registers of its workgroup: NC chunks of 16 bytes per thread.  The teacher's entries are set
+// right behind the row's stores and a barrier.  (Finding each thread's entries on a list in LDS before its stores instead: 82 us
+// against 74 at 2048 x 40 982 bf16 — the lists' making delays every store of the row, the second look only its last ones.)
 template <class T, int TH, int NC>
-__global__ __launch_bounds__(TH, NC <= 8 ? 8 : 4) void distill_row_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(TH, NC <= 12 ? 5 : 4) void distill_row_kernel(const DistillArgs a) {
     constexpr int E = RowShape<T>::E;
     __shared__ Entries sh;
     const int64_t row = blockIdx.x;
     const T *z = (const T *)a.z + row * a.ldz;
     T *g = (T *)a.grad + row * a.ldg;
     const RowShape<T> rs(z, a.V);
-    const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + rs.head);
-    Vec<T, E> v[NC];
+    const u32x4 *body = reinterpret_cast<const u32x4 *>(z + rs.head);
+    u32x4 v[NC];
 #pragma unroll
     for (int u = 0; u < NC; ++u) {
         const int i = u * TH + threadIdx.x;
@@ -326,42 +353,45 @@ __global__ __launch_bounds__(TH, NC <= 8 ? 8 : 4) void distill_row_kernel(const 
     for (int u = 0; u < NC; ++u)
         if (u * TH + (int)threadIdx.x < rs.nb)
 #pragma unroll
-            for (int e = 0; e < E; ++e) r.m = fmaxf(r.m, to_f32(v[u].v[e]));
+            for (int e = 0; e < E; ++e) r.m = fmaxf(r.m, to_f32(as_elems<T, E>(v[u]).v[e]));
+    forget(v);
     const float mm = r.m == -INFINITY ? 0.f : r.m;
 #pragma unroll
     for (int u = 0; u < NC; ++u)
         if (u * TH + (int)threadIdx.x < rs.nb)
 #pragma unroll
-            for (int e = 0; e < E; ++e) r.s += exp2_fast((to_f32(v[u].v[e]) - mm) * a.c);
+            for (int e = 0; e < E; ++e) r.s += exp2_fast((to_f32(as_elems<T, E>(v[u]).v[e]) - mm) * a.c);
+    forget(v);
     if (has_loose) r.s += exp2_fast((loose - mm) * a.c);
     const MaxSum st = block_join<TH>(r, a.c, sh.red);
-    __syncthreads();
-    entries_loss(a, row, sh, st);
+    if constexpr (TH == kWave) __syncthreads();  // (block_join's own barrier hands over the entries elsewhere)
+    entries_loss(a, row, sh, st);                // (the other waves are storing meanwhile: at the end it would prolong the workgroup)
+    const bool nt = TH >= 512 || a.nt;           // (512 threads: rows of over 16 KB, and at least 512 of them)
     if (distill_empty(sh, st)) {
-        zero_row<T, TH>(g, rs, 0, rs.nb, true);
-        return;
-    }
-    const float w = a.row_w ? a.row_w[row] : 1.f;
-    const float s = w * a.T / st.s;
-    Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + rs.head);
-    const bool wide = on_16_dev(out);
+        zero_row<T, TH>(g, rs, 0, rs.nb, true, nt);
+    } else {
+        const float w = a.row_w ? a.row_w[row] : 1.f;
+        const float s = w * a.T / st.s;
+        Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + rs.head);
+        const bool wide = on_16_dev(out);
 #pragma unroll
-    for (int u = 0; u < NC; ++u) {
-        const int i = u * TH + threadIdx.x;
-        if (i >= rs.nb) break;
-        Vec<T, E> o;
+        for (int u = 0; u < NC; ++u) {
+            const int i = u * TH + threadIdx.x;
+            if (i >= rs.nb) break;
+            Vec<T, E> o;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(s * exp2_fast((to_f32(v[u].v[e]) - st.m) * a.c));
-        if (wide) {
-            out[i] = o;
-        } else {
+            for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(s * exp2_fast((to_f32(as_elems<T, E>(v[u]).v[e]) - st.m) * a.c));
+            if (wide) {
+                put16(out + i, &o, nt);
+            } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) g[rs.head + i * E + e] = o.v[e];
+                for (int e = 0; e < E; ++e) g[rs.head + i * E + e] = o.v[e];
+            }
         }
+        if (has_loose) g[rs.at(threadIdx.x)] = from_f32<T>(s * exp2_fast((loose - st.m) * a.c));
+        __syncthreads();
+        fix_entries<T, TH>(a, g, rs, 0, rs.nb, true, sh, st, w);
     }
-    if (has_loose) g[rs.at(threadIdx.x)] = from_f32<T>(s * exp2_fast((loose - st.m) * a.c));
-    __syncthreads();
-    fix_entries<T, TH>(a, g, rs, 0, rs.nb, true, sh, st, w);
 }
 
 // Rows longer than that: the row is read twice, the second time out of the caches where they hold it.
@@ -377,11 +407,11 @@ __global__ __launch_bounds__(TH) void distill_long_kernel(const DistillArgs a) {
     __syncthreads();
     entries_loss(a, row, sh, st);
     if (distill_empty(sh, st)) {
-        zero_row<T, TH>(g, rs, 0, rs.nb, true);
+        zero_row<T, TH>(g, rs, 0, rs.nb, true, a.nt);
         return;
     }
     const float w = a.row_w ? a.row_w[row] : 1.f;
-    write_row<T, TH, 4>(z, g, rs, 0, rs.nb, true, st.m, a.c, w * a.T / st.s, -1, 0.f);
+    write_row<T, TH, 4>(z, g, rs, 0, rs.nb, true, st.m, a.c, w * a.T / st.s, -1, 0.f, a.nt);
     __syncthreads();
     fix_entries<T, TH>(a, g, rs, 0, rs.nb, true, sh, st, w);
 }
@@ -432,11 +462,11 @@ __global__ __launch_bounds__(TH) void distill_grad_kernel(const DistillArgs a) {
     part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
     const bool loose = blockIdx.x == 0;
     if (distill_empty(sh, st)) {
-        zero_row<T, TH>(g, rs, c0, c1, loose);
+        zero_row<T, TH>(g, rs, c0, c1, loose, a.nt);
         return;
     }
     const float w = a.row_w ? a.row_w[row] : 1.f;
-    write_row<T, TH, 4>(z, g, rs, c0, c1, loose, st.m, a.c, w * a.T / st.s, -1, 0.f);
+    write_row<T, TH, 4>(z, g, rs, c0, c1, loose, st.m, a.c, w * a.T / st.s, -1, 0.f, a.nt);
     __syncthreads();
     fix_entries<T, TH>(a, g, rs, c0, c1, loose, sh, st, w);
 }
@@ -499,7 +529,7 @@ __global__ __launch_bounds__(kWave) void logp_join_kernel(const LogpArgs a, int 
 // what the caches still hold.
 template <class T, int TH>
 __global__ __launch_bounds__(TH) void logp_grad_kernel(const void *zv, int64_t ldz, int V, const int64_t *targets, const float *stats,
-                                                       const float *row_g, void *gv, int64_t ldg) {
+                                                       const float *row_g, void *gv, int64_t ldg, bool nt) {
     const int64_t row = (int64_t)gridDim.y - 1 - blockIdx.y;
     const int64_t t = targets[row];
     const T *z = (const T *)zv + row * ldz;
@@ -509,8 +539,8 @@ __global__ __launch_bounds__(TH) void logp_grad_kernel(const void *zv, int64_t l
     part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
     const bool loose = blockIdx.x == 0;
     const float m = stats[2 * row], s = stats[2 * row + 1], w = row_g[row];
-    if (t < 0 || t >= V || (m == -INFINITY && s == 0.f) || w == 0.f) zero_row<T, TH>(g, rs, c0, c1, loose);
-    else write_row<T, TH, 4>(z, g, rs, c0, c1, loose, m, kLog2e, -w / s, (int)t, w);
+    if (t < 0 || t >= V || (m == -INFINITY && s == 0.f) || w == 0.f) zero_row<T, TH>(g, rs, c0, c1, loose, nt);
+    else write_row<T, TH, 4>(z, g, rs, c0, c1, loose, m, kLog2e, -w / s, (int)t, w, nt);
 }
 
 __device__ __forceinline__ float sigmoid_d(float h, float smoothing) {  // d loss / d margin
@@ -597,6 +627,9 @@ static int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
 // Workgroups per row of a pass that needs nothing from the rest of the row: 256 threads x 4 chunks each.
 static int grad_parts(int64_t V, int elem) { return (int)std::max<int64_t>(1, std::min<int64_t>((V * elem + 16383) / 16384, 1024)); }
 
+// A gradient of more than the eight L2s' 32 MB.
+static bool past_caches(int64_t n, int64_t V, int elem) { return n * V * elem > 32 << 20; }
+
 static int check_rows(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V) {
     if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
     if (n < 0 || V <= 0 || ldz < V) return fail(RBG_ESHAPE, "n = %lld, V = %lld, ldz = %lld", (long long)n, (long long)V, (long long)ldz);
@@ -631,11 +664,12 @@ static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, hipStream_
         const dim3 grid((unsigned)n);
         if (chunks <= 64 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 64, 4>), grid, dim3(64), 0, s, a);
         else if (chunks <= 256 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 256, 4>), grid, dim3(256), 0, s, a);
-        else if (chunks <= 1024 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 4>), grid, dim3(1024), 0, s, a);
-        else if (chunks <= 1024 * 6) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 6>), grid, dim3(1024), 0, s, a);
-        else if (chunks <= 1024 * 8) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 8>), grid, dim3(1024), 0, s, a);
-        else if (chunks <= 1024 * 12) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 12>), grid, dim3(1024), 0, s, a);
-        else if (chunks <= 1024 * 16) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 16>), grid, dim3(1024), 0, s, a);
+        else if (chunks <= 512 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 512, 4>), grid, dim3(512), 0, s, a);
+        else if (chunks <= 512 * 7) hipLaunchKernelGGL((distill_row_kernel<T, 512, 7>), grid, dim3(512), 0, s, a);
+        else if (chunks <= 512 * 11) hipLaunchKernelGGL((distill_row_kernel<T, 512, 11>), grid, dim3(512), 0, s, a);
+        else if (chunks <= 512 * 16) hipLaunchKernelGGL((distill_row_kernel<T, 512, 16>), grid, dim3(512), 0, s, a);
+        else if (chunks <= 512 * 24) hipLaunchKernelGGL((distill_row_kernel<T, 512, 24>), grid, dim3(512), 0, s, a);
+        else if (chunks <= 1024 * 24) hipLaunchKernelGGL((distill_row_kernel<T, 1024, 24>), grid, dim3(1024), 0, s, a);
         else hipLaunchKernelGGL((distill_long_kernel<T, 1024>), grid, dim3(1024), 0, s, a);
     }
     RBG_HIP(hipGetLastError());
@@ -665,15 +699,16 @@ static int launch_logp_grad(const T *z, int64_t ldz, int64_t m, int64_t V, const
                             T *g, int64_t ldg, hipStream_t s) {
     const int S = grad_parts(V, sizeof(T));
     const int64_t slices = (m + kMaxGridY - 1) / kMaxGridY;
+    const bool nt = past_caches(m, V, sizeof(T));
     for (int64_t k = slices - 1; k >= 0; --k) {
         const int64_t r0 = k * kMaxGridY, cnt = std::min(kMaxGridY, m - r0);
         const dim3 grid(S, (unsigned)cnt);
         if (V * (int64_t)sizeof(T) <= 4096)
             hipLaunchKernelGGL((logp_grad_kernel<T, 64>), grid, dim3(64), 0, s, z + r0 * ldz, ldz, (int)V, targets + r0, stats + 2 * r0,
-                               row_g + r0, g + r0 * ldg, ldg);
+                               row_g + r0, g + r0 * ldg, ldg, nt);
         else
             hipLaunchKernelGGL((logp_grad_kernel<T, 256>), grid, dim3(256), 0, s, z + r0 * ldz, ldz, (int)V, targets + r0, stats + 2 * r0,
-                               row_g + r0, g + r0 * ldg, ldg);
+                               row_g + r0, g + r0 * ldg, ldg, nt);
     }
     RBG_HIP(hipGetLastError());
     return RBG_OK;
@@ -714,7 +749,7 @@ int rbg_distill_topk(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V
         if (int rc = check_grad(z, ldz, dtype, n, V, grad, ldg)) return rc;
     const int S = row_parts(n, V);
     DistillArgs a{z, ldz, (int)V, k, idx, val, (float)(1.4426950408889634 / (double)T), T, row_w, loss, stats, grad, ldg, (MaxSum *)workspace,
-                  (float *)((char *)workspace + round16(n * S * (int64_t)sizeof(MaxSum)))};
+                  (float *)((char *)workspace + round16(n * S * (int64_t)sizeof(MaxSum))), past_caches(n, V, elem_size(dtype))};
     return with_elem(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, V, (hipStream_t)stream); });
 }
 
@@ -732,7 +767,7 @@ int rbg_distill_topk_backward(const void *z, int64_t ldz, int dtype, int64_t n, 
         typedef decltype(t) E;
         for (int64_t r0 = 0; r0 < n; r0 += kMaxGridY) {
             const DistillArgs a{(const E *)z + r0 * ldz, ldz, (int)V, k, idx + r0 * k, val + r0 * k, (float)(1.4426950408889634 / (double)T), T,
-                                row_w ? row_w + r0 : nullptr, nullptr, const_cast<float *>(stats) + 2 * r0, (E *)grad + r0 * ldg, ldg, nullptr, nullptr};
+                                row_w ? row_w + r0 : nullptr, nullptr, const_cast<float *>(stats) + 2 * r0, (E *)grad + r0 * ldg, ldg, nullptr, nullptr, past_caches(n, V, elem_size(dtype))};
             const dim3 grid(S, (unsigned)std::min(kMaxGridY, n - r0));
             hipLaunchKernelGGL((distill_grad_kernel<E, 256, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
         }
