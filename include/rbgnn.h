@@ -692,7 +692,7 @@ int rbg_mean_f32(const float *const *srcs, int n_srcs, int64_t n_floats, float s
  * 8-bit table.  `dtype` is RBG_F32, RBG_BF16 or RBG_F16; arithmetic is in 32 bits, an output is rounded once, to nearest even.
  * Leading dimensions count elements (bytes for codes).  Ids and targets are DEVICE int64; one outside its range reads nothing and
  * adds to nothing (-1 is the usual "none").  Sums run in an order that sizes and alignments alone decide: results are bit-stable.
- * A workspace belongs to the call until its work on `stream` has ended: calls that may overlap (two streams, two captured graphs
+ * A workspace (which may be NULL where its size is 0) belongs to the call until its work on `stream` has ended: calls that may overlap (two streams, two captured graphs
  * replayed side by side) need one each.  No call allocates or synchronizes; every call can be captured.
  * ------------------------------------------------------------------------------------------- */
 

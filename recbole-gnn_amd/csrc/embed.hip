@@ -22,34 +22,60 @@
 
 namespace rbg {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // ---- lookup --------------------------------------------------------------------------------------------------------------
 
-// One thread per vector of VEC elements; `per_row` vectors in a row.
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table, int64_t ldt, int64_t n_rows, const int64_t *__restrict__ ids,
-                                                     int64_t n, int per_row, float scale, T *__restrict__ out, int64_t ldo) {
-    const int64_t total = n * per_row, step = (int64_t)gridDim.x * 256;
-    for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < total; w += step) {
-        const int64_t i = w / per_row;
-        const int c = (int)(w - i * per_row) * VEC;
-        const int64_t id = ids[i];
-        Vec<T, VEC> v;
-        if (id >= 0 && id < n_rows) {
-            v = *reinterpret_cast<const Vec<T, VEC> *>(table + id * ldt + c);
+// 16 bytes of an output.  One that the L2s cannot hold anyway (`nt`) goes past them.
+template <class V>
+__device__ __forceinline__ void put(void *p, const V &v, bool nt) {
+    if constexpr (sizeof(V) % 16 == 0) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(scale * to_f32(v.v[e]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(0.f);
+        for (unsigned k = 0; k < sizeof(V) / 16; ++k) {
+            u32x4 x;
+            __builtin_memcpy(&x, (const char *)&v + 16 * k, 16);
+            u32x4 *to = reinterpret_cast<u32x4 *>(p) + k;
+            if (nt) __builtin_nontemporal_store(x, to);
+            else *to = x;
         }
-        *reinterpret_cast<Vec<T, VEC> *>(out + i * ldo + c) = v;
+    } else {
+        *reinterpret_cast<V *>(p) = v;
+    }
+}
+
+// G lanes per row, R rows of a lane-group in flight (ids, then rows, then stores).
+template <class T, int VEC, int G>
+__global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table, int64_t ldt, int64_t n_rows, const int64_t *__restrict__ ids,
+                                                     int64_t n, int d, float scale, T *__restrict__ out, int64_t ldo, bool nt) {
+    constexpr int R = 4;
+    const int sub = threadIdx.x % G;
+    const int64_t i0 = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * R;
+    if (i0 >= n) return;
+    int64_t id[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) id[r] = i0 + r < n ? ids[i0 + r] : -1;
+    for (int c = sub * VEC; c < d; c += G * VEC) {
+        Vec<T, VEC> v[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (id[r] >= 0 && id[r] < n_rows) v[r] = *reinterpret_cast<const Vec<T, VEC> *>(table + id[r] * ldt + c);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[r].v[e] = from_f32<T>(0.f);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (i0 + r >= n) break;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[r].v[e] = from_f32<T>(scale * to_f32(v[r].v[e]));
+            put(out + (i0 + r) * ldo + c, v[r], nt);
+        }
     }
 }
 
 // ---- sort ----------------------------------------------------------------------------------------------------------------
 
 constexpr int kRankMax = 16384;  // places ranked by counting
-constexpr int kTile = 2048;      // places of a radix tile (256 threads x 8)
 constexpr int kMaxBits = 9;
 
 // A place's sort key: its row, or n_rows for one that adds to nothing (such places end behind every row).
@@ -58,40 +84,53 @@ __device__ __forceinline__ uint32_t key_of(const int64_t *ids, int64_t i, int64_
     return id >= 0 && id < n_rows && id != padding ? (uint32_t)id : (uint32_t)n_rows;
 }
 
-// Rank by counting: a workgroup ranks 64 places; its 16 waves count over a sixteenth of the places each, out of LDS.
+// Rank by counting: a workgroup ranks P places.  Its 64-lane waves hold them 64 / P times over; wave and copy say which part of the
+// places a lane counts over, out of LDS: two instructions for 64 pairs, since all but the workgroup's own places lie wholly in front of or
+// wholly behind the ranked ones.
+template <int P>
 __global__ __launch_bounds__(1024) void rank_kernel(const int64_t *__restrict__ ids, int n, int64_t n_rows, int64_t padding,
                                                     uint32_t *__restrict__ keys, uint32_t *__restrict__ places, uint32_t *count) {
+    constexpr int PARTS = 16 * (64 / P);
     __shared__ __align__(16) uint32_t all[kRankMax];
-    __shared__ uint32_t before[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ uint32_t before[PARTS][P];
     const int n4 = (n + 3) & ~3;
+#pragma unroll 8
     for (int j = threadIdx.x; j < n4; j += 1024) all[j] = j < n ? key_of(ids, j, n_rows, padding) : 0xffffffffu;
     if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
-    const int i = blockIdx.x * 64 + lane;
+    const int own = threadIdx.x % P, part = threadIdx.x / P;
+    const int i0 = blockIdx.x * P, i = i0 + own;
     const uint32_t mine = i < n ? all[i] : 0u;
-    // places in front of i: of equal ids those before it, i.e. key <= mine for j < i and key < mine from i on
-    const int per = ((n4 / 4 + 15) / 16) * 4, j0 = min(w * per, n4), j1 = min(j0 + per, n4);
+    // of equal ids those in front come first: key <= mine for j < i, key < mine behind (parts an odd number of 16-byte pieces long: a wave's
+    // copies then read different banks)
+    const int per = ((n4 / 4 + PARTS - 1) / PARTS | 1) * 4, j0 = min(part * per, n4), j1 = min(j0 + per, n4);
     uint32_t r = 0;
-    for (int j = j0; j < j1; j += 4) {
+    int j = j0;
+    const int ja = min(j1, i0), jb = min(j1, i0 + P);
+#pragma unroll 8
+    for (; j < ja; j += 4) {
         const uint4 k = *reinterpret_cast<const uint4 *>(all + j);
-        r += k.x < mine || (k.x == mine && j < i);
-        r += k.y < mine || (k.y == mine && j + 1 < i);
-        r += k.z < mine || (k.z == mine && j + 2 < i);
-        r += k.w < mine || (k.w == mine && j + 3 < i);
+        r += k.x <= mine, r += k.y <= mine, r += k.z <= mine, r += k.w <= mine;
     }
-    before[w][lane] = r;
+    for (; j < jb; ++j) r += all[j] < mine || (all[j] == mine && j < i);
+#pragma unroll 8
+    for (; j < j1; j += 4) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(all + j);
+        r += k.x < mine, r += k.y < mine, r += k.z < mine, r += k.w < mine;
+    }
+    before[part][own] = r;
     __syncthreads();
-    if (w == 0 && i < n) {
+    if (threadIdx.x < P && i < n) {
         uint32_t rank = 0;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) rank += before[q][lane];
+#pragma unroll 16
+        for (int q = 0; q < PARTS; ++q) rank += before[q][own];
         keys[rank] = mine;
         places[rank] = (uint32_t)i;
     }
 }
 
 // Radix pass, first launch: how often each digit occurs in each tile -> hist[digit][tile].  (ids: the first pass.)
+template <int R>  // a tile is 256 R places
 __global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, const uint32_t *keys, int64_t n, int64_t n_rows, int64_t padding,
                                                           int shift, int bits, uint32_t *hist, uint32_t *count) {
     __shared__ uint32_t h[1 << kMaxBits];
@@ -99,8 +138,9 @@ __global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, co
     for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
-    const int64_t i0 = (int64_t)blockIdx.x * kTile;
-    for (int u = 0; u < kTile / 256; ++u) {
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * R);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
         const int64_t i = i0 + u * 256 + threadIdx.x;
         if (i < n) {
             const uint32_t k = ids ? key_of(ids, i, n_rows, padding) : keys[i];
@@ -138,6 +178,7 @@ __global__ __launch_bounds__(256) void digit_prefix_kernel(uint32_t *hist, int t
 }
 
 // Third launch: every place moves to (places of smaller digits) + (of its digit in earlier tiles) + (of its digit before it here).
+template <int R>
 __global__ __launch_bounds__(256) void digit_scatter_kernel(const int64_t *ids, const uint32_t *keys, const uint32_t *places, int64_t n,
                                                             int64_t n_rows, int64_t padding, int shift, int bits, const uint32_t *hist,
                                                             const uint32_t *total, uint32_t *keys_out, uint32_t *places_out) {
@@ -146,8 +187,7 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(const int64_t *ids, 
     const int bins = 1 << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     for (int d = threadIdx.x; d < 4 * (1 << kMaxBits); d += 256) (&at[0][0])[d] = 0;
     __syncthreads();
-    constexpr int R = kTile / 256;
-    const int64_t i0 = (int64_t)blockIdx.x * kTile + w * (kTile / 4);
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * R) + w * (64 * R);
     uint32_t key[R], rank[R];
 #pragma unroll
     for (int u = 0; u < R; ++u) {
@@ -219,23 +259,28 @@ struct RunArgs {
     float *part;               // [chunks][2][d]: sums of the chunk's first run and of its last, where they cross a border
     uint32_t *list, *count;    // chunks whose last run starts there and goes on
     int64_t run_blocks;        // the launch's workgroups that sum; the rest zero rows
+    bool nt;                   // the output goes past the caches
 };
 
 template <class T, int VEC>
-__device__ __forceinline__ void store_row(T *p, const float (&acc)[VEC], float scale) {
+__device__ __forceinline__ void store_row(T *p, const float (&acc)[VEC], float scale, bool nt) {
     Vec<T, VEC> v;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(scale * acc[e]);
-    *reinterpret_cast<Vec<T, VEC> *>(p) = v;
+    put(p, v, nt);
 }
 
-// First place of the sorted list whose key is not below v.
+// First place of the sorted list whose key is not below v, by a whole wave: 64 probes a round.
 __device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t n, uint32_t v) {
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < v) lo = mid + 1;
-        else hi = mid;
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, cnt = n;  // the answer is in [lo, lo + cnt]
+    while (cnt > 0) {
+        const int64_t step = (cnt + 63) / 64;
+        const int64_t at = lo + (lane + 1) * step - 1;
+        const int below = __popcll(__ballot(at < lo + cnt && keys[at] < v));  // probes 0 .. below - 1 are below v
+        const int64_t end = lo + cnt;
+        lo += below * step;
+        cnt = min(step - 1, end - lo);
     }
     return lo;
 }
@@ -243,27 +288,29 @@ __device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t
 // G lanes x VEC elements cover a piece of a row (blockIdx.y: which piece); 256 / G chunks per workgroup.
 template <class TI, class TO, int VEC, int G>
 __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
-    constexpr int U = 8;  // rows in flight per lane-group
+    constexpr int U = G < 8 ? G : 8;  // rows in flight per lane-group
     const int sub = threadIdx.x % G, grp = threadIdx.x / G;
     const int col = (blockIdx.y * G + sub) * VEC;
     const bool on = col < a.d;
     TO *out = (TO *)a.out;
-    if (blockIdx.x >= a.run_blocks) {  // zero rows: a lane-group takes the rows of its stripe that no place refers to
-        const int64_t b = blockIdx.x - a.run_blocks;
-        const int64_t r0 = b * 256;
-        const int64_t r = r0 + threadIdx.x;
-        __shared__ uint32_t empty[256];
-        bool none = false;
-        if (r < a.n_rows) {
-            const int64_t at = first_not_below(a.keys, a.n, (uint32_t)r);
-            none = at >= a.n || a.keys[at] != (uint32_t)r;
+    const float zero[VEC] = {};
+    if (blockIdx.x >= a.run_blocks) {  // zero the rows of a stripe of 256 that no place refers to
+        __shared__ uint32_t used[256];
+        __shared__ int64_t bounds[2];
+        const int64_t r0 = (int64_t)(blockIdx.x - a.run_blocks) * 256;
+        const int rows = (int)min<int64_t>(256, a.n_rows - r0);
+        used[threadIdx.x] = 0;
+        if (threadIdx.x < 128) {
+            const int w = threadIdx.x >> 6;
+            const int64_t at = first_not_below(a.keys, a.n, (uint32_t)(r0 + w * rows));
+            if ((threadIdx.x & 63) == 0) bounds[w] = at;
         }
-        empty[threadIdx.x] = none;
         __syncthreads();
-        const float zero[VEC] = {};
+        for (int64_t p = bounds[0] + threadIdx.x; p < bounds[1]; p += 256) used[a.keys[p] - (uint32_t)r0] = 1;
+        __syncthreads();
         if (on)
-            for (int q = grp; q < 256; q += 256 / G)
-                if (empty[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f);
+            for (int q = grp; q < rows; q += 256 / G)
+                if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f, a.nt);
         return;
     }
     const int64_t c = (int64_t)blockIdx.x * (256 / G) + grp;
@@ -276,25 +323,32 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     float acc[VEC] = {};
     uint32_t run = a.keys[p0];
     bool first = run == ahead;  // the current run began in an earlier chunk
+    // U places at a time, a lane each, one turn ahead of their rows
+    auto key_at = [&](int64_t p) { return sub < U && p + sub < p1 ? a.keys[p + sub] : none; };
+    auto place_at = [&](int64_t p) { return sub < U && p + sub < p1 ? a.places[p + sub] : 0u; };
+    uint32_t next_key = key_at(p0), next_place = place_at(p0);
     for (int64_t p = p0; p < p1; p += U) {
+        const uint32_t my_key = next_key, my_place = next_place;
+        next_key = key_at(p + U), next_place = place_at(p + U);
         uint32_t key[U];
         Vec<TI, VEC> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            key[u] = p + u < p1 ? a.keys[p + u] : none;
-            if (key[u] != none && on) v[u] = *reinterpret_cast<const Vec<TI, VEC> *>(grad + (int64_t)a.places[p + u] * a.ldg + col);
+            key[u] = __shfl(my_key, u, G);
+            const uint32_t place = __shfl(my_place, u, G);
+            if (key[u] != none && on) v[u] = *reinterpret_cast<const Vec<TI, VEC> *>(grad + (int64_t)place * a.ldg + col);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (p + u >= p1) break;
-            if (key[u] != run) {  // the run ends here
+            if (key[u] != run) {  // the run ends here (a place behind the chunk's last has no row: `none`)
+                if (p + u >= p1) break;
                 if (run != none && on) {
                     if (first) {
                         float *to = a.part + (2 * c) * a.d + col;
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) to[e] = acc[e];
                     } else {
-                        store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale);
+                        store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale, a.nt);
                     }
                 }
                 run = key[u];
@@ -311,7 +365,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     if (run == none) return;
     const bool goes_on = run == behind;
     if (!first && !goes_on) {
-        if (on) store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale);
+        if (on) store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale, a.nt);
         return;
     }
     if (on) {
@@ -320,6 +374,74 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
         for (int e = 0; e < VEC; ++e) to[e] = acc[e];
     }
     if (!first && sub == 0 && blockIdx.y == 0) a.list[atomicAdd(a.count, 1u)] = (uint32_t)c;  // (the list's order changes no sum)
+}
+
+// Few places (n <= kFewPlaces): one launch, no sorted list.  A workgroup owns 256 rows (and a piece of their columns), finds the places that
+// refer to them, ranks those by (row, place) by counting, and sums a run per lane-group; its other rows are zeroed.
+constexpr int kFewPlaces = 256;
+
+template <class TI, class TO, int VEC, int G>
+__global__ __launch_bounds__(256) void few_places_kernel(const RunArgs a, const int64_t *__restrict__ ids, int64_t padding) {
+    constexpr int U = 8;  // rows in flight per lane-group
+    __shared__ __align__(16) uint32_t row_of[kFewPlaces];  // of a place, from the workgroup's first row; 256: another's
+    __shared__ uint32_t run_of[kFewPlaces + 1], place_of[kFewPlaces];
+    __shared__ uint32_t used[256];
+    __shared__ uint32_t found;
+    const int n = (int)a.n, i = threadIdx.x;
+    const int64_t r0 = (int64_t)blockIdx.x * 256;
+    const int rows = (int)min<int64_t>(256, a.n_rows - r0);
+    uint32_t mine = 256;
+    if (i < n) {
+        const int64_t id = ids[i];
+        if (id >= r0 && id < r0 + rows && id != padding) mine = (uint32_t)(id - r0);
+    }
+    row_of[i] = mine;
+    used[i] = 0;
+    if (i == 0) found = 0;
+    __syncthreads();
+    if (mine < 256) {
+        uint32_t rank = 0;
+        const int n4 = (n + 3) & ~3;
+        for (int j = 0; j < n4; j += 4) {
+            const uint4 k = *reinterpret_cast<const uint4 *>(row_of + j);
+            rank += k.x < mine || (k.x == mine && j < i);
+            rank += k.y < mine || (k.y == mine && j + 1 < i);
+            rank += k.z < mine || (k.z == mine && j + 2 < i);
+            rank += k.w < mine || (k.w == mine && j + 3 < i);
+        }
+        run_of[rank] = mine;
+        place_of[rank] = (uint32_t)i;
+        used[mine] = 1;
+        atomicAdd(&found, 1u);
+    }
+    __syncthreads();
+    const int sub = i % G, grp = i / G, m = (int)found;
+    const int col = (blockIdx.y * G + sub) * VEC;
+    if (col >= a.d) return;
+    const TI *grad = (const TI *)a.grad;
+    TO *out = (TO *)a.out;
+    const float zero[VEC] = {};
+    for (int e0 = grp; e0 < m; e0 += 256 / G) {
+        const uint32_t run = run_of[e0];
+        if (e0 && run_of[e0 - 1] == run) continue;  // another lane-group has it
+        int end = e0 + 1;
+        while (end < m && run_of[end] == run) ++end;
+        float acc[VEC] = {};
+        for (int p = e0; p < end; p += U) {
+            Vec<TI, VEC> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p + u < end) v[u] = *reinterpret_cast<const Vec<TI, VEC> *>(grad + (int64_t)place_of[p + u] * a.ldg + col);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p + u < end)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] += to_f32(v[u].v[e]);
+        }
+        store_row<TO, VEC>(out + (r0 + run) * a.d + col, acc, a.scale, a.nt);
+    }
+    for (int q = grp; q < rows; q += 256 / G)
+        if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f, a.nt);
 }
 
 // Runs over several chunks: the last sum of the chunk they start in, then the first sums of the chunks they reach into.
@@ -334,8 +456,14 @@ __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
     for (uint32_t t = blockIdx.x; t < todo; t += gridDim.x) {
         const int64_t c = a.list[t];
         const uint32_t key = a.keys[(c + 1) * a.chunk];
-        const int64_t end = first_not_below(a.keys, a.n, key + 1u);
-        const int64_t last = (end - 1) / a.chunk;  // the chunk it ends in
+        int64_t last = c + 1;  // the last chunk that starts with the run's key
+        for (;;) {
+            const int64_t q = last + 1 + (threadIdx.x & 63);
+            const unsigned long long same = __ballot(q < a.chunks && a.keys[q * a.chunk] == key);
+            const int more = ~same ? __builtin_ctzll(~same) : 64;
+            last += more;
+            if (more < 64) break;
+        }
         // parts c, c + 1, .., last: an equal piece for each lane-group, the pieces joined in order
         const int64_t cnt = last - c + 1, per = (cnt + N - 1) / N;
         const int64_t q0 = c + grp * per, q1 = min(q0 + per, last + 1);
@@ -357,7 +485,7 @@ __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
             for (int q = 0; q < N; ++q)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] += sums[(q * G + sub) * VEC + e];
-            store_row<TO, VEC>((TO *)a.out + (int64_t)key * a.d + col, acc, a.scale);
+            store_row<TO, VEC>((TO *)a.out + (int64_t)key * a.d + col, acc, a.scale, a.nt);
         }
         __syncthreads();
     }
@@ -375,7 +503,7 @@ static int chunk_of(int64_t n, int d) {
 
 struct Layout {
     int64_t keys, places, keys2, places2, hist, total, part, list, count, bytes;
-    int chunk, tiles;
+    int chunk, tiles, tile_rounds;
     int64_t chunks;
 };
 
@@ -383,13 +511,15 @@ static Layout layout_of(int64_t n, int d) {
     Layout l{};
     l.chunk = chunk_of(n, d);
     l.chunks = (n + l.chunk - 1) / l.chunk;
-    l.tiles = (int)((n + kTile - 1) / kTile);
+    l.tile_rounds = n <= 1 << 19 ? 2 : 8;  // (at 65 536 places 32 tiles of 2 048 leave most CUs idle: 12 us a scatter)
+    l.tiles = (int)((n + 256 * l.tile_rounds - 1) / (256 * l.tile_rounds));
     int64_t at = 0;
     auto take = [&](int64_t b) {
         const int64_t r = at;
         at += round16e(b);
         return r;
     };
+    if (n <= kFewPlaces) return l;
     l.count = take(16);
     l.keys = take(4 * n), l.places = take(4 * n);
     if (n > kRankMax) {
@@ -404,8 +534,13 @@ static Layout layout_of(int64_t n, int d) {
 }
 
 template <class TI, class TO, int VEC, int G>
-static void launch_runs(const RunArgs &a0, hipStream_t s) {
+static void launch_runs(const RunArgs &a0, const int64_t *ids, int64_t padding, hipStream_t s) {
     RunArgs a = a0;
+    if (a.n <= kFewPlaces) {
+        hipLaunchKernelGGL((few_places_kernel<TI, TO, VEC, G>), dim3((unsigned)((a.n_rows + 255) / 256), (unsigned)((a.d + G * VEC - 1) / (G * VEC))), dim3(256),
+                           0, s, a, ids, padding);
+        return;
+    }
     a.run_blocks = (a.chunks + 256 / G - 1) / (256 / G);
     const unsigned pieces = (unsigned)((a.d + G * VEC - 1) / (G * VEC));
     const int64_t zero_blocks = (a.n_rows + 255) / 256;
@@ -415,19 +550,19 @@ static void launch_runs(const RunArgs &a0, hipStream_t s) {
 }
 
 template <class TI, class TO>
-static int launch_runs_of(const RunArgs &a, bool wide, hipStream_t s) {
+static int launch_runs_of(const RunArgs &a, const int64_t *ids, int64_t padding, bool wide, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(TI);
     const int lanes = wide ? a.d / VEC : a.d;
     if (wide) {
-        if (lanes <= 4) launch_runs<TI, TO, VEC, 4>(a, s);
-        else if (lanes <= 8) launch_runs<TI, TO, VEC, 8>(a, s);
-        else if (lanes <= 16) launch_runs<TI, TO, VEC, 16>(a, s);
-        else if (lanes <= 32) launch_runs<TI, TO, VEC, 32>(a, s);
-        else launch_runs<TI, TO, VEC, 64>(a, s);
+        if (lanes <= 4) launch_runs<TI, TO, VEC, 4>(a, ids, padding, s);
+        else if (lanes <= 8) launch_runs<TI, TO, VEC, 8>(a, ids, padding, s);
+        else if (lanes <= 16) launch_runs<TI, TO, VEC, 16>(a, ids, padding, s);
+        else if (lanes <= 32) launch_runs<TI, TO, VEC, 32>(a, ids, padding, s);
+        else launch_runs<TI, TO, VEC, 64>(a, ids, padding, s);
     } else {
-        if (lanes <= 4) launch_runs<TI, TO, 1, 4>(a, s);
-        else if (lanes <= 16) launch_runs<TI, TO, 1, 16>(a, s);
-        else launch_runs<TI, TO, 1, 64>(a, s);
+        if (lanes <= 4) launch_runs<TI, TO, 1, 4>(a, ids, padding, s);
+        else if (lanes <= 16) launch_runs<TI, TO, 1, 16>(a, ids, padding, s);
+        else launch_runs<TI, TO, 1, 64>(a, ids, padding, s);
     }
     RBG_HIP(hipGetLastError());
     return RBG_OK;
@@ -460,14 +595,22 @@ int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dty
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
         constexpr int VEC = 16 / (int)sizeof(E);
-        const int per_row = wide ? d / VEC : d;
-        const unsigned grid = (unsigned)std::min<int64_t>((n * per_row + 255) / 256, 16384);
-        if (wide)
-            hipLaunchKernelGGL((lookup_kernel<E, VEC>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n,
-                               per_row, scale, (E *)out, ldo);
-        else
-            hipLaunchKernelGGL((lookup_kernel<E, 1>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n,
-                               per_row, scale, (E *)out, ldo);
+        const bool nt = n * d * size > 32 << 20;
+        auto go = [&](auto kernel, int G) {
+            const int64_t per = 256 / G * 4;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n, d, scale,
+                               (E *)out, ldo, nt);
+        };
+        const int lanes = wide ? d / VEC : d;
+        if (wide) {
+            if (lanes <= 4) go(lookup_kernel<E, VEC, 4>, 4);
+            else if (lanes <= 16) go(lookup_kernel<E, VEC, 16>, 16);
+            else go(lookup_kernel<E, VEC, 64>, 64);
+        } else {
+            if (lanes <= 4) go(lookup_kernel<E, 1, 4>, 4);
+            else if (lanes <= 16) go(lookup_kernel<E, 1, 16>, 16);
+            else go(lookup_kernel<E, 1, 64>, 64);
+        }
         RBG_HIP(hipGetLastError());
         return (int)RBG_OK;
     });
@@ -488,7 +631,7 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
     if (int rc = check_places(n, n_rows, d)) return rc;
     if (ldg < d) return fail(RBG_ESHAPE, "d = %d, ldg = %lld", d, (long long)ldg);
     if (n_rows == 0) return RBG_OK;
-    if ((n && (!grad || !ids)) || !out || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if ((n && (!grad || !ids)) || !out || (n > kFewPlaces && !workspace)) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
     const int size = elem_size(dtype), out_size = elem_size(out_dtype);
     if (reinterpret_cast<uintptr_t>(grad) % size || reinterpret_cast<uintptr_t>(out) % out_size) return fail(RBG_EINVAL, "a tensor is not aligned to its type");
@@ -497,9 +640,12 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
     char *w = (char *)workspace;
     uint32_t *count = (uint32_t *)(w + l.count);
     uint32_t *keys = (uint32_t *)(w + l.keys), *places = (uint32_t *)(w + l.places);
-    if (n > 0 && n <= kRankMax) {
-        hipLaunchKernelGGL(rank_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
-    } else if (n > 0) {
+    if (n > kFewPlaces && n <= kRankMax) {
+        // (16, 32 and 64 places a workgroup measure alike at 8 192; fewer for fewer, so that the CUs have work)
+        if (n <= 4096) hipLaunchKernelGGL((rank_kernel<16>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+        else if (n <= 8192) hipLaunchKernelGGL((rank_kernel<32>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+        else hipLaunchKernelGGL((rank_kernel<64>), dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+    } else if (n > kRankMax) {
         int bits = 1;
         while (((int64_t)1 << bits) <= n_rows) ++bits;  // keys 0 .. n_rows
         const int passes = (bits + kMaxBits - 1) / kMaxBits, width = (bits + passes - 1) / passes;
@@ -510,20 +656,26 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
         uint32_t *to_k = passes & 1 ? keys : k2, *to_p = passes & 1 ? places : p2;
         for (int q = 0; q < passes; ++q) {
             const int64_t *src = q == 0 ? ids : nullptr;
-            hipLaunchKernelGGL(digit_count_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
+            if (l.tile_rounds == 2) hipLaunchKernelGGL((digit_count_kernel<2>), dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
+            else hipLaunchKernelGGL((digit_count_kernel<8>), dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
             hipLaunchKernelGGL(digit_prefix_kernel, dim3(1u << width), dim3(256), 0, s, hist, l.tiles, total);
-            hipLaunchKernelGGL(digit_scatter_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
-                               hist, total, to_k, to_p);
+            if (l.tile_rounds == 2)
+                hipLaunchKernelGGL((digit_scatter_kernel<2>), dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
+                                   hist, total, to_k, to_p);
+            else
+                hipLaunchKernelGGL((digit_scatter_kernel<8>), dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
+                                   hist, total, to_k, to_p);
             from_k = to_k, from_p = to_p;
             to_k = to_k == keys ? k2 : keys, to_p = to_p == places ? p2 : places;
         }
     }
     RBG_HIP(hipGetLastError());
-    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0};
+    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0,
+                    n_rows * d * out_size > 32 << 20};
     const bool wide = on_16(grad) && reinterpret_cast<uintptr_t>(out) % (16 / size * out_size) == 0 && d * size % 16 == 0 && ldg * size % 16 == 0;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
-        return out_dtype == dtype ? launch_runs_of<E, E>(a, wide, s) : launch_runs_of<E, float>(a, wide, s);
+        return out_dtype == dtype ? launch_runs_of<E, E>(a, ids, padding_idx, wide, s) : launch_runs_of<E, float>(a, ids, padding_idx, wide, s);
     });
 }
 

@@ -96,13 +96,18 @@ __device__ __forceinline__ void online(MaxSum &r, const float (&x)[N], float c) 
     r.s = s;
 }
 
-// (m, s) of chunks [c0, c1) of a row, and of its loose elements when `loose`, over the threads of a workgroup.
+// The TH threads that share a row: a workgroup, or (TH = 64) a wave of one.
+template <int TH>
+__device__ __forceinline__ int member() { return TH == kWave ? (int)(threadIdx.x & 63) : (int)threadIdx.x; }
+
+// (m, s) of chunks [c0, c1) of a row, and of its loose elements when `loose`, as far as one of its TH threads sees it.
 template <class T, int TH, int U>
 __device__ __forceinline__ MaxSum scan_row(const T *__restrict__ z, const RowShape<T> &sh, int c0, int c1, bool loose, float c) {
     constexpr int E = RowShape<T>::E;
     const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + sh.head);
     MaxSum r{-INFINITY, 0.f};
-    int i = c0 + threadIdx.x;
+    const int tid = member<TH>();
+    int i = c0 + tid;
     for (; i + (U - 1) * TH < c1; i += U * TH) {
         Vec<T, E> v[U];
 #pragma unroll
@@ -114,15 +119,22 @@ __device__ __forceinline__ MaxSum scan_row(const T *__restrict__ z, const RowSha
             for (int e = 0; e < E; ++e) x[u * E + e] = to_f32(v[u].v[e]);
         online<T>(r, x, c);
     }
-    for (; i < c1; i += TH) {
-        const Vec<T, E> v = body[i];
-        float x[E];
+    if (i < c1) {  // at most U more, all in flight at once
+        Vec<T, E> v[U];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = to_f32(v.v[e]);
-        online<T>(r, x, c);
+        for (int u = 0; u < U; ++u)
+            if (i + u * TH < c1) v[u] = body[i + u * TH];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u * TH >= c1) break;
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = to_f32(v[u].v[e]);
+            online<T>(r, x, c);
+        }
     }
-    if (loose && (int)threadIdx.x < sh.extra) {
-        const float x[1] = {to_f32(z[sh.at(threadIdx.x)])};
+    if (loose && tid < sh.extra) {
+        const float x[1] = {to_f32(z[sh.at(tid)])};
         online<T>(r, x, c);
     }
     return r;
@@ -137,18 +149,19 @@ __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &s
     const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + sh.head);
     Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
     const bool wide = on_16_dev(out);
+    const int tid = member<TH>();
     const int hb = hot - sh.head;
     const int hc = hot >= sh.head && hot < sh.tail ? hb / E : -1, he = hb - hc * E;
     for (int i0 = c0; i0 < c1; i0 += U * TH) {
         Vec<T, E> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * TH + threadIdx.x;
+            const int i = i0 + u * TH + tid;
             if (i < c1) v[u] = body[i];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * TH + threadIdx.x;
+            const int i = i0 + u * TH + tid;
             if (i >= c1) break;
             float x[E];
 #pragma unroll
@@ -167,8 +180,8 @@ __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &s
             }
         }
     }
-    if (loose && (int)threadIdx.x < sh.extra) {
-        const int j = sh.at(threadIdx.x);
+    if (loose && tid < sh.extra) {
+        const int j = sh.at(tid);
         float x = a * exp2_fast((to_f32(z[j]) - m) * c);
         if (j == hot) x += more;
         g[j] = from_f32<T>(x);
@@ -180,10 +193,11 @@ __device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, in
     constexpr int E = RowShape<T>::E;
     Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
     const bool wide = on_16_dev(out);
+    const int tid = member<TH>();
     Vec<T, E> v;
 #pragma unroll
     for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(0.f);
-    for (int i = c0 + threadIdx.x; i < c1; i += TH) {
+    for (int i = c0 + tid; i < c1; i += TH) {
         if (wide) {
             put16(out + i, &v, nt);
         } else {
@@ -191,7 +205,7 @@ __device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, in
             for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v.v[e];
         }
     }
-    if (loose && (int)threadIdx.x < sh.extra) g[sh.at(threadIdx.x)] = from_f32<T>(0.f);
+    if (loose && tid < sh.extra) g[sh.at(tid)] = from_f32<T>(0.f);
 }
 
 // Part s of S of a row's chunks.
@@ -525,26 +539,53 @@ __global__ __launch_bounds__(kWave) void logp_join_kernel(const LogpArgs a, int 
     if (threadIdx.x == 0) store_logp(a, row, there, there ? to_f32(((const T *)a.z + row * a.ldz)[t]) : 0.f, st);
 }
 
-// grad = row_g (onehot - softmax), one workgroup per row and part; row = the last one first: what the pass before read last is
-// what the caches still hold.
+// Part `part` of `parts` of a row's gradient w (onehot - softmax), by TH threads; a row of gradient 0 is not read.
 template <class T, int TH>
-__global__ __launch_bounds__(TH) void logp_grad_kernel(const void *zv, int64_t ldz, int V, const int64_t *targets, const float *stats,
-                                                       const float *row_g, void *gv, int64_t ldg, bool nt) {
-    const int64_t row = (int64_t)gridDim.y - 1 - blockIdx.y;
+__device__ __forceinline__ void grad_row(const void *zv, int64_t ldz, int V, const int64_t *targets, const float *stats, int64_t row, float w,
+                                         void *gv, int64_t ldg, int part, int parts, bool nt) {
     const int64_t t = targets[row];
     const T *z = (const T *)zv + row * ldz;
     T *g = (T *)gv + row * ldg;
     const RowShape<T> rs(z, V);
     int c0, c1;
-    part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
-    const bool loose = blockIdx.x == 0;
-    const float m = stats[2 * row], s = stats[2 * row + 1], w = row_g[row];
-    if (t < 0 || t >= V || (m == -INFINITY && s == 0.f) || w == 0.f) zero_row<T, TH>(g, rs, c0, c1, loose, nt);
+    part_of(rs.nb, part, parts, c0, c1);
+    const bool loose = part == 0;
+    bool none = t < 0 || t >= V || w == 0.f;
+    float m = 0.f, s = 0.f;
+    if (!none) {
+        m = stats[2 * row], s = stats[2 * row + 1];
+        none = m == -INFINITY && s == 0.f;
+    }
+    if (none) zero_row<T, TH>(g, rs, c0, c1, loose, nt);
     else write_row<T, TH, 4>(z, g, rs, c0, c1, loose, m, kLog2e, -w / s, (int)t, w, nt);
+}
+
+template <class T, int TH>
+__device__ __forceinline__ void clear_row(const void *zv, int64_t ldz, int V, int64_t row, void *gv, int64_t ldg) {
+    const RowShape<T> rs((const T *)zv + row * ldz, V);
+    zero_row<T, TH>((T *)gv + row * ldg, rs, 0, rs.nb, true, false);
+}
+
+// One workgroup per row and part; row = the last one first: what the pass before read last is what the caches still hold.
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void logp_grad_kernel(const void *z, int64_t ldz, int V, const int64_t *targets, const float *stats,
+                                                       const float *row_g, void *g, int64_t ldg, bool nt) {
+    const int64_t row = (int64_t)gridDim.y - 1 - blockIdx.y;
+    grad_row<T, TH>(z, ldz, V, targets, stats, row, row_g[row], g, ldg, blockIdx.x, gridDim.x, nt);
 }
 
 __device__ __forceinline__ float sigmoid_d(float h, float smoothing) {  // d loss / d margin
     return smoothing / (1.f + expf(-h)) - (1.f - smoothing) / (1.f + expf(h));
+}
+
+// -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)); a term of weight 0 is left out (its value may be infinite).
+__device__ __forceinline__ void store_pair(float h, float smoothing, float *loss, float *margin) {
+    const float l = log1pf(expf(-fabsf(h)));
+    float v = 0.f;
+    if (smoothing < 1.f) v += (1.f - smoothing) * (fmaxf(-h, 0.f) + l);
+    if (smoothing > 0.f) v += smoothing * (fmaxf(h, 0.f) + l);
+    *loss = h != h ? h : v;
+    *margin = h;
 }
 
 __device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_t m, int64_t &lo, int64_t &hi) {
@@ -573,22 +614,62 @@ __global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, con
 #pragma unroll
     for (int k = 0; k < 2; ++k) sum[k] = ((red[k][0] + red[k][1]) + (red[k][2] + red[k][3])) - (double)ref[2 * i + k];
     const float h = (float)((double)beta * (sum[0] - sum[1]));
-    if (threadIdx.x == 0) {
-        // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)); a term of weight 0 is left out (its value may be infinite)
-        const float l = log1pf(expf(-fabsf(h)));
-        float v = 0.f;
-        if (smoothing < 1.f) v += (1.f - smoothing) * (fmaxf(-h, 0.f) + l);
-        if (smoothing > 0.f) v += smoothing * (fmaxf(h, 0.f) + l);
-        if (h != h) v = h;
-        loss[i] = v;
-        margin[i] = h;
-    }
+    if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
     if constexpr (COEF) {
         const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
             for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) coef[t] = k ? -d : d;
     }
+}
+
+// Small calls in one launch: a workgroup per pair, a wave per row.  Both sums meet in LDS, and the rows, read a second time for their
+// gradient, are still in the caches.  (m, S) of a row stays with the wave that goes on to write it.
+template <class T>
+__global__ __launch_bounds__(1024) void pair_small_kernel(const LogpArgs a, int64_t m, const int64_t *offsets, const float *ref, float beta,
+                                                          float smoothing, const float *pair_w, float *loss, float *margin, void *gv, int64_t ldg) {
+    __shared__ double red[2][16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t i = blockIdx.x;
+    int64_t lo[2], hi[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        seq_of(offsets, 2 * i + k, m, lo[k], hi[k]);
+        double sum = 0.0;
+        for (int64_t row = lo[k] + w; row < hi[k]; row += 16) {
+            const int64_t t = a.targets[row];
+            if (t < 0 || t >= a.V) continue;
+            const T *z = (const T *)a.z + row * a.ldz;
+            const RowShape<T> rs(z, a.V);
+            const float zt = to_f32(z[t]);
+            const MaxSum st = wave_join(scan_row<T, kWave, 4>(z, rs, 0, rs.nb, true, kLog2e), kLog2e);
+            if (lane == 0) a.stats[2 * row] = st.m, a.stats[2 * row + 1] = st.s;
+            if (!(st.m == -INFINITY && st.s == 0.f)) sum += ((double)zt - (double)st.m) - log((double)st.s);
+        }
+        if (lane == 0) red[k][w] = sum;
+    }
+    __syncthreads();
+    double sum[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        sum[k] = 0.0;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sum[k] += red[k][q];
+        sum[k] -= (double)ref[2 * i + k];
+    }
+    const float h = (float)((double)beta * (sum[0] - sum[1]));
+    if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
+    const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        for (int64_t row = lo[k] + w; row < hi[k]; row += 16)
+            grad_row<T, kWave>(a.z, a.ldz, a.V, a.targets, a.stats, row, k ? -d : d, gv, ldg, 0, 1, false);
+    // rows in front of the first sequence and behind the last
+    const int64_t r0 = i == 0 ? 0 : hi[1], r1 = i == 0 ? lo[0] : m;
+    if (i == 0 || i + 1 == gridDim.x)
+        for (int64_t row = r0 + w; row < r1; row += 16) clear_row<T, kWave>(a.z, a.ldz, a.V, row, gv, ldg);
+    if (i == 0 && gridDim.x == 1)
+        for (int64_t row = hi[1] + w; row < m; row += 16) clear_row<T, kWave>(a.z, a.ldz, a.V, row, gv, ldg);
 }
 
 // grad_logp of every token: its sequence is found by bisection (the last one that begins at or before it and is not empty).
@@ -732,7 +813,7 @@ int rbg_distill_topk_workspace(int64_t n, int64_t V, int64_t *bytes) {
     if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
     if (n < 0 || V <= 0) return fail(RBG_ESHAPE, "n = %lld, V = %lld", (long long)n, (long long)V);
     const int S = row_parts(n, V);
-    *bytes = S > 1 ? round16(n * S * (int64_t)sizeof(MaxSum)) + round16(n * kMaxEntries * 4) : 16;
+    *bytes = S > 1 ? round16(n * S * (int64_t)sizeof(MaxSum)) + round16(n * kMaxEntries * 4) : 0;
     return RBG_OK;
 }
 
@@ -743,7 +824,7 @@ int rbg_distill_topk(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V
     if (k < 1 || k > kMaxEntries) return fail(RBG_EUNSUPPORTED, "k = %d: 1 to %d entries per row", k, kMaxEntries);
     if (!(T >= 1e-15f && T <= 1e15f)) return fail(RBG_EINVAL, "T = %g", T);  // (1 / T and T^2 stay normal numbers)
     if (n == 0) return RBG_OK;
-    if (!idx || !val || !loss || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if (!idx || !val || !loss || (!workspace && row_parts(n, V) > 1)) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
     if (grad)
         if (int rc = check_grad(z, ldz, dtype, n, V, grad, ldg)) return rc;
@@ -781,7 +862,7 @@ int rbg_token_logp_workspace(int64_t m, int64_t V, int64_t *bytes) {
     if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
     if (m < 0 || V <= 0) return fail(RBG_ESHAPE, "m = %lld, V = %lld", (long long)m, (long long)V);
     const int S = row_parts(m, V);
-    *bytes = S > 1 ? round16(m * S * (int64_t)sizeof(MaxSum)) : 16;
+    *bytes = S > 1 ? round16(m * S * (int64_t)sizeof(MaxSum)) : 0;
     return RBG_OK;
 }
 
@@ -790,7 +871,7 @@ int rbg_token_logp(const void *z, int64_t ldz, int dtype, int64_t m, int64_t V, 
     clear_error();
     if (int rc = check_rows(z, ldz, dtype, m, V)) return rc;
     if (m == 0) return RBG_OK;
-    if (!targets || !logp || !workspace) return fail(RBG_EINVAL, "NULL pointer");
+    if (!targets || !logp || (!workspace && row_parts(m, V) > 1)) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(workspace)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned");
     const LogpArgs a{z, ldz, (int)V, targets, logp, nullptr, nullptr, stats, (MaxSum *)workspace};
     return with_elem(dtype, [&](auto t) { return launch_logp<decltype(t)>(a, m, V, (hipStream_t)stream); });
@@ -858,6 +939,17 @@ int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_
     MaxSum *part = (MaxSum *)(w + 2 * round16(8 * m) + round16(4 * m));
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
+        // Up to 256 tokens, 64 and 128 KB a pair, and 1 MB in all: one launch instead of three (40 x 1 683 fp32, four pairs: 13 us a
+        // call, 19 with three).  A workgroup takes a pair's rows sixteen at a time, and the lengths are on the device: all tokens in
+        // one pair cost 16 turns of it at most (at 4 756 tokens of two pairs it would take 560 us).
+        const int64_t total = m * V * (int64_t)sizeof(E);
+        if (m && m <= 256 && m <= pairs * 64 && total <= 1 << 20 && total <= pairs << 17) {
+            const LogpArgs a{z, ldz, (int)V, targets, nullptr, nullptr, nullptr, stats, nullptr};
+            hipLaunchKernelGGL((pair_small_kernel<E>), dim3((unsigned)pairs), dim3(1024), 0, s, a, m, offsets, ref, beta, smoothing, pair_w, loss, margin,
+                               grad, ldg);
+            RBG_HIP(hipGetLastError());
+            return (int)RBG_OK;
+        }
         if (m) {
             const LogpArgs a{z, ldz, (int)V, targets, nullptr, logp, coef, stats, part};
             if (int rc = launch_logp<E>(a, m, V, s)) return rc;

@@ -75,12 +75,13 @@ def _ptr(t):
 def _bytes(fn, *sizes):
     nbytes = _lib.c_i64()
     check(getattr(lib, fn)(*sizes, ctypes.byref(nbytes)))
-    return max(nbytes.value, 16)
+    return nbytes.value
 
 
 def _workspace(of, fn, *sizes):
-    """A workspace of the call's own, on the current stream (the caching allocator hands it out in stream order)."""
-    return of.new_empty(_bytes(fn, *sizes), dtype=torch.uint8)
+    """A workspace of the call's own, on the current stream (the caching allocator hands it out in stream order); None if it needs none."""
+    nbytes = _bytes(fn, *sizes)
+    return of.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -114,7 +115,7 @@ def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=Non
         n = ids.numel()
         work = _workspace(grad, "rbg_embedding_grad_workspace", n, n_rows, d)
         _call(lib.rbg_embedding_grad, grad, grad.data_ptr(), _ld(grad), _DTYPES[grad.dtype], ids.data_ptr(), n, n_rows, d, float(scale),
-              -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _DTYPES[out_dtype], work.data_ptr())
+              -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _DTYPES[out_dtype], _ptr(work))
     return out
 
 
@@ -161,7 +162,7 @@ def _distill(logits, idx, val, temperature, row_weight, want_stats, want_grad):
     grad = logits.new_empty((n, v), dtype=logits.dtype) if want_grad else None
     work = _workspace(logits, "rbg_distill_topk_workspace", n, v)
     _call(lib.rbg_distill_topk, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], n, v, idx.data_ptr(), val.data_ptr(),
-          idx.shape[1], temperature, _ptr(row_weight), loss.data_ptr(), _ptr(stats), _ptr(grad), v, work.data_ptr())
+          idx.shape[1], temperature, _ptr(row_weight), loss.data_ptr(), _ptr(stats), _ptr(grad), v, _ptr(work))
     return loss, stats, grad
 
 
@@ -220,7 +221,7 @@ class _TokenLogp(torch.autograd.Function):
         stats = logits.new_empty((m, 2), dtype=torch.float32)
         work = _workspace(logits, "rbg_token_logp_workspace", m, v)
         _call(lib.rbg_token_logp, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(), logp.data_ptr(),
-              stats.data_ptr(), work.data_ptr())
+              stats.data_ptr(), _ptr(work))
         ctx.save_for_backward(logits, targets, stats)
         return logp
 
@@ -302,7 +303,7 @@ def preference_grad(logits, targets, offsets, ref_logp, beta=0.1, label_smoothin
     work = _workspace(logits, "rbg_preference_grad_workspace", m, v)
     _call(lib.rbg_preference_grad, logits, logits.data_ptr(), _ld(logits), _DTYPES[logits.dtype], m, v, targets.data_ptr(),
           offsets.data_ptr(), pairs, ref.data_ptr(), float(beta), float(label_smoothing), _ptr(pair_weight), loss[0].data_ptr(),
-          loss[1].data_ptr(), grad.data_ptr(), v, work.data_ptr())
+          loss[1].data_ptr(), grad.data_ptr(), v, _ptr(work))
     return loss[0], loss[1], grad
 
 
@@ -365,5 +366,5 @@ def score_int8(u, codes, scales, out_dtype=torch.float32):
         codes, ldi = _codes(codes, k)
         work = _workspace(u, "rbg_score_rows_i8_workspace", b, k)
         _call(lib.rbg_score_rows_i8, u, u.data_ptr(), _ld(u), _DTYPES[u.dtype], b, codes.data_ptr(), ldi, scales.data_ptr(), n, k,
-              out.data_ptr(), n, _DTYPES[out_dtype], work.data_ptr())
+              out.data_ptr(), n, _DTYPES[out_dtype], _ptr(work))
     return out

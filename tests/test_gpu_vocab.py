@@ -79,7 +79,7 @@ def runs_reference(grad, ids, rows, scale, padding):
             torch.bincount(ids[ok], minlength=rows)[:, None].double())
 
 
-GRAD_SHAPES = [(1, 1, 1), (2, 5, 64), (7, 3, 65), (300, 50, 64), (5000, 40, 128), (6144, 40982, 64), (4096, 1, 32), (16384, 1000, 32), (16385, 511, 24),
+GRAD_SHAPES = [(1, 1, 1), (2, 5, 64), (7, 3, 65), (100, 700, 64), (255, 3, 40), (256, 1000, 513), (257, 1000, 16), (300, 50, 64), (5000, 40, 128), (6144, 40982, 64), (4096, 1, 32), (16384, 1000, 32), (16385, 511, 24),
                (16385, 512, 8), (20000, 70000, 64), (40000, 3, 100), (50000, 300000, 16), (70001, 100, 1), (33000, 1, 4), (1000, 20, 1024), (3000, 7, 2051)]
 
 
@@ -101,7 +101,7 @@ def test_embedding_grad(rbg, cuda, dtype, n, rows, d):
         assert torch.equal(got, rbg.embedding_grad(grad, ids, rows, scale=1.7, padding_idx=padding, out_dtype=out_dtype))
 
 
-@pytest.mark.parametrize("n", [0, 1, 9, 3000, 20000])
+@pytest.mark.parametrize("n", [0, 1, 9, 256, 257, 3000, 20000])
 def test_embedding_grad_of_nothing_and_of_one_row(rbg, cuda, n):
     grad = torch.ones(n, 64, device=cuda)
     none = torch.full((n,), -1, device=cuda)
@@ -368,7 +368,7 @@ def preference_reference(lp, tol, offsets, ref, beta, smoothing):
 
 
 @pytest.mark.parametrize("dtype", ALL)
-@pytest.mark.parametrize("m,v,pairs,lead,behind", [(1, 1, 1, 0, 0), (2, 3, 1, 0, 0), (40, 1683, 4, 3, 5), (9, 50001, 2, 0, 1), (700, 513, 300, 0, 0), (600, 9001, 5, 7, 11)])
+@pytest.mark.parametrize("m,v,pairs,lead,behind", [(1, 1, 1, 0, 0), (2, 3, 1, 0, 0), (40, 1683, 4, 3, 5), (256, 33, 4, 1, 0), (130, 900, 40, 0, 30), (9, 50001, 2, 0, 1), (700, 513, 300, 0, 0), (4756, 18, 2, 0, 0), (600, 9001, 5, 7, 11)])
 @pytest.mark.parametrize("smoothing,beta", [(0.0, 0.1), (0.3, 1.0), (1.0, -0.5)])
 def test_preference(rbg, cuda, dtype, m, v, pairs, lead, behind, smoothing, beta):
     g = gen(m + pairs, cuda)

@@ -48,12 +48,12 @@ REFUSED = [
     (embedding, dict(n=-1), ESHAPE), (embedding, dict(ids=None), EINVAL), (embedding, dict(table=None), EINVAL), (embedding, dict(out=P(2)), EINVAL),
     (embedding_grad, dict(out_dtype=2), EINVAL), (embedding_grad, dict(ldg=7), ESHAPE), (embedding_grad, dict(rows=0x7fffffff), EUNSUPPORTED),
     (embedding_grad, dict(n=0x7fff0000), EUNSUPPORTED), (embedding_grad, dict(d=(1 << 20) + 1, ldg=1 << 21), EUNSUPPORTED), (embedding_grad, dict(work=P(8)), EINVAL),
-    (embedding_grad, dict(work=None), EINVAL), (embedding_grad, dict(grad=P(1)), EINVAL),
+    (embedding_grad, dict(work=None, n=1000), EINVAL), (embedding_grad, dict(grad=P(1)), EINVAL),
     (distill, dict(k=0), EUNSUPPORTED), (distill, dict(k=257), EUNSUPPORTED), (distill, dict(t=0.0), EINVAL), (distill, dict(t=float("nan")), EINVAL),
     (distill, dict(t=-1.0), EINVAL), (distill, dict(v=0), ESHAPE), (distill, dict(ldz=7), ESHAPE), (distill, dict(dtype=-1), EINVAL),
     (distill, dict(z=P(2)), EINVAL), (distill, dict(loss=None), EINVAL), (distill, dict(work=P(4)), EINVAL), (distill, dict(grad=P((1 << 20) + 32)), EINVAL),
     (distill, dict(grad=A, ldg=9), EINVAL), (distill, dict(grad=D, ldg=7), ESHAPE), (distill, dict(v=1 << 31, ldz=1 << 31), EUNSUPPORTED),
-    (logp, dict(targets=None), EINVAL), (logp, dict(v=-1), ESHAPE), (logp, dict(work=None), EINVAL),
+    (logp, dict(targets=None), EINVAL), (logp, dict(v=-1), ESHAPE), (logp, dict(work=None, v=50000, ldz=50000), EINVAL), (distill, dict(work=None, v=50000, ldz=50000), EINVAL),
     (preference, dict(beta=float("inf")), EINVAL), (preference, dict(smoothing=-0.1), EINVAL), (preference, dict(smoothing=1.5), EINVAL),
     (preference, dict(smoothing=float("nan")), EINVAL), (preference, dict(offsets=None), EINVAL), (preference, dict(pairs=-1), ESHAPE),
     (preference, dict(ref=None), EINVAL), (preference, dict(grad=None), EINVAL), (preference, dict(grad=P((1 << 20) - 32)), EINVAL),
@@ -86,7 +86,7 @@ def test_nothing_to_do_is_no_error(rbg):
 
 def test_workspaces(rbg):
     lib, n = rbg._lib.lib, ctypes.c_int64()
-    for fn, args in ((lib.rbg_embedding_grad_workspace, (5, 7, 8)), (lib.rbg_embedding_grad_workspace, (100000, 7, 8)), (lib.rbg_distill_topk_workspace, (3, 50000)),
+    for fn, args in ((lib.rbg_embedding_grad_workspace, (500, 7, 8)), (lib.rbg_embedding_grad_workspace, (100000, 7, 8)), (lib.rbg_distill_topk_workspace, (3, 50000)),
                      (lib.rbg_token_logp_workspace, (3, 50000)), (lib.rbg_score_rows_i8_workspace, (3, 500)), (lib.rbg_preference_grad_workspace, (3, 50000))):
         assert fn(*args, ctypes.byref(n)) == OK and n.value > 0 and n.value % 16 == 0
         assert fn(*args, None) == EINVAL
