@@ -22,31 +22,17 @@
 
 namespace rbg {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // ---- lookup --------------------------------------------------------------------------------------------------------------
 
-// 16 bytes of an output.  One that the L2s cannot hold anyway (`nt`) goes past them.
-template <class V>
-__device__ __forceinline__ void put(void *p, const V &v, bool nt) {
-    if constexpr (sizeof(V) % 16 == 0) {
-#pragma unroll
-        for (unsigned k = 0; k < sizeof(V) / 16; ++k) {
-            u32x4 x;
-            __builtin_memcpy(&x, (const char *)&v + 16 * k, 16);
-            u32x4 *to = reinterpret_cast<u32x4 *>(p) + k;
-            if (nt) __builtin_nontemporal_store(x, to);
-            else *to = x;
-        }
-    } else {
-        *reinterpret_cast<V *>(p) = v;
-    }
-}
+// The lane-groups below cover a row of d elements with vectors of VEC; the last vector of a row ends where the row ends and overlaps the one
+// in front of it (both hold the same values), so that rows of any width and start move 16 bytes at a time.
+template <int VEC>
+__device__ __forceinline__ int vector_at(int c, int d) { return min(c, d - VEC); }
 
 // G lanes per row, R rows of a lane-group in flight (ids, then rows, then stores).
 template <class T, int VEC, int G>
 __global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table, int64_t ldt, int64_t n_rows, const int64_t *__restrict__ ids,
-                                                     int64_t n, int d, float scale, T *__restrict__ out, int64_t ldo, bool nt) {
+                                                     int64_t n, int d, float scale, T *__restrict__ out, int64_t ldo) {
     constexpr int R = 4;
     const int sub = threadIdx.x % G;
     const int64_t i0 = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * R;
@@ -54,11 +40,12 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table
     int64_t id[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) id[r] = i0 + r < n ? ids[i0 + r] : -1;
-    for (int c = sub * VEC; c < d; c += G * VEC) {
+    for (int c0 = sub * VEC; c0 < d; c0 += G * VEC) {
+        const int c = vector_at<VEC>(c0, d);
         Vec<T, VEC> v[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (id[r] >= 0 && id[r] < n_rows) v[r] = *reinterpret_cast<const Vec<T, VEC> *>(table + id[r] * ldt + c);
+            if (id[r] >= 0 && id[r] < n_rows) v[r] = load_any<T, VEC>(table + id[r] * ldt + c);
             else
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[r].v[e] = from_f32<T>(0.f);
@@ -68,7 +55,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table
             if (i0 + r >= n) break;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[r].v[e] = from_f32<T>(scale * to_f32(v[r].v[e]));
-            put(out + (i0 + r) * ldo + c, v[r], nt);
+            store_any(out + (i0 + r) * ldo + c, v[r]);
         }
     }
 }
@@ -259,15 +246,14 @@ struct RunArgs {
     float *part;               // [chunks][2][d]: sums of the chunk's first run and of its last, where they cross a border
     uint32_t *list, *count;    // chunks whose last run starts there and goes on
     int64_t run_blocks;        // the launch's workgroups that sum; the rest zero rows
-    bool nt;                   // the output goes past the caches
 };
 
 template <class T, int VEC>
-__device__ __forceinline__ void store_row(T *p, const float (&acc)[VEC], float scale, bool nt) {
+__device__ __forceinline__ void store_row(T *p, const float (&acc)[VEC], float scale) {
     Vec<T, VEC> v;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<T>(scale * acc[e]);
-    put(p, v, nt);
+    store_any(p, v);
 }
 
 // First place of the sorted list whose key is not below v, by a whole wave: 64 probes a round.
@@ -285,21 +271,23 @@ __device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t
     return lo;
 }
 
+constexpr int kStripe = 256;  // rows that one workgroup zeroes
+
 // G lanes x VEC elements cover a piece of a row (blockIdx.y: which piece); 256 / G chunks per workgroup.
 template <class TI, class TO, int VEC, int G>
 __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     constexpr int U = G < 8 ? G : 8;  // rows in flight per lane-group
     const int sub = threadIdx.x % G, grp = threadIdx.x / G;
-    const int col = (blockIdx.y * G + sub) * VEC;
-    const bool on = col < a.d;
+    const int piece = (blockIdx.y * G + sub) * VEC, col = vector_at<VEC>(piece, a.d);
+    const bool on = piece < a.d;
     TO *out = (TO *)a.out;
     const float zero[VEC] = {};
-    if (blockIdx.x >= a.run_blocks) {  // zero the rows of a stripe of 256 that no place refers to
-        __shared__ uint32_t used[256];
+    if (blockIdx.x >= a.run_blocks) {  // zero the rows of a stripe that no place refers to
+        __shared__ uint32_t used[kStripe];
         __shared__ int64_t bounds[2];
-        const int64_t r0 = (int64_t)(blockIdx.x - a.run_blocks) * 256;
-        const int rows = (int)min<int64_t>(256, a.n_rows - r0);
-        used[threadIdx.x] = 0;
+        const int64_t r0 = (int64_t)(blockIdx.x - a.run_blocks) * kStripe;
+        const int rows = (int)min<int64_t>(kStripe, a.n_rows - r0);
+        if (threadIdx.x < kStripe) used[threadIdx.x] = 0;
         if (threadIdx.x < 128) {
             const int w = threadIdx.x >> 6;
             const int64_t at = first_not_below(a.keys, a.n, (uint32_t)(r0 + w * rows));
@@ -310,7 +298,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
         __syncthreads();
         if (on)
             for (int q = grp; q < rows; q += 256 / G)
-                if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f, a.nt);
+                if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f);
         return;
     }
     const int64_t c = (int64_t)blockIdx.x * (256 / G) + grp;
@@ -336,7 +324,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
         for (int u = 0; u < U; ++u) {
             key[u] = __shfl(my_key, u, G);
             const uint32_t place = __shfl(my_place, u, G);
-            if (key[u] != none && on) v[u] = *reinterpret_cast<const Vec<TI, VEC> *>(grad + (int64_t)place * a.ldg + col);
+            if (key[u] != none && on) v[u] = load_any<TI, VEC>(grad + (int64_t)place * a.ldg + col);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -348,7 +336,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) to[e] = acc[e];
                     } else {
-                        store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale, a.nt);
+                        store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale);
                     }
                 }
                 run = key[u];
@@ -365,7 +353,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     if (run == none) return;
     const bool goes_on = run == behind;
     if (!first && !goes_on) {
-        if (on) store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale, a.nt);
+        if (on) store_row<TO, VEC>(out + (int64_t)run * a.d + col, acc, a.scale);
         return;
     }
     if (on) {
@@ -416,8 +404,8 @@ __global__ __launch_bounds__(256) void few_places_kernel(const RunArgs a, const 
     }
     __syncthreads();
     const int sub = i % G, grp = i / G, m = (int)found;
-    const int col = (blockIdx.y * G + sub) * VEC;
-    if (col >= a.d) return;
+    const int piece = (blockIdx.y * G + sub) * VEC, col = vector_at<VEC>(piece, a.d);
+    if (piece >= a.d) return;
     const TI *grad = (const TI *)a.grad;
     TO *out = (TO *)a.out;
     const float zero[VEC] = {};
@@ -431,17 +419,17 @@ __global__ __launch_bounds__(256) void few_places_kernel(const RunArgs a, const 
             Vec<TI, VEC> v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (p + u < end) v[u] = *reinterpret_cast<const Vec<TI, VEC> *>(grad + (int64_t)place_of[p + u] * a.ldg + col);
+                if (p + u < end) v[u] = load_any<TI, VEC>(grad + (int64_t)place_of[p + u] * a.ldg + col);
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (p + u < end)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) acc[e] += to_f32(v[u].v[e]);
         }
-        store_row<TO, VEC>(out + (r0 + run) * a.d + col, acc, a.scale, a.nt);
+        store_row<TO, VEC>(out + (r0 + run) * a.d + col, acc, a.scale);
     }
     for (int q = grp; q < rows; q += 256 / G)
-        if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f, a.nt);
+        if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f);
 }
 
 // Runs over several chunks: the last sum of the chunk they start in, then the first sums of the chunks they reach into.
@@ -450,8 +438,8 @@ __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
     constexpr int N = 256 / G;
     __shared__ float sums[256 * VEC];
     const int sub = threadIdx.x % G, grp = threadIdx.x / G;
-    const int col = (blockIdx.y * G + sub) * VEC;
-    const bool on = col < a.d;
+    const int piece = (blockIdx.y * G + sub) * VEC, col = vector_at<VEC>(piece, a.d);
+    const bool on = piece < a.d;
     const uint32_t todo = *a.count;
     for (uint32_t t = blockIdx.x; t < todo; t += gridDim.x) {
         const int64_t c = a.list[t];
@@ -485,7 +473,7 @@ __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
             for (int q = 0; q < N; ++q)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] += sums[(q * G + sub) * VEC + e];
-            store_row<TO, VEC>((TO *)a.out + (int64_t)key * a.d + col, acc, a.scale, a.nt);
+            store_row<TO, VEC>((TO *)a.out + (int64_t)key * a.d + col, acc, a.scale);
         }
         __syncthreads();
     }
@@ -543,7 +531,7 @@ static void launch_runs(const RunArgs &a0, const int64_t *ids, int64_t padding, 
     }
     a.run_blocks = (a.chunks + 256 / G - 1) / (256 / G);
     const unsigned pieces = (unsigned)((a.d + G * VEC - 1) / (G * VEC));
-    const int64_t zero_blocks = (a.n_rows + 255) / 256;
+    const int64_t zero_blocks = (a.n_rows + kStripe - 1) / kStripe;
     hipLaunchKernelGGL((run_sum_kernel<TI, TO, VEC, G>), dim3((unsigned)(a.run_blocks + zero_blocks), pieces), dim3(256), 0, s, a);
     if (a.chunks > 1)
         hipLaunchKernelGGL((run_join_kernel<TO, VEC, G>), dim3((unsigned)std::min<int64_t>(a.chunks, 1024), pieces), dim3(256), 0, s, a);
@@ -552,7 +540,7 @@ static void launch_runs(const RunArgs &a0, const int64_t *ids, int64_t padding, 
 template <class TI, class TO>
 static int launch_runs_of(const RunArgs &a, const int64_t *ids, int64_t padding, bool wide, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(TI);
-    const int lanes = wide ? a.d / VEC : a.d;
+    const int lanes = wide ? (a.d + VEC - 1) / VEC : a.d;
     if (wide) {
         if (lanes <= 4) launch_runs<TI, TO, VEC, 4>(a, ids, padding, s);
         else if (lanes <= 8) launch_runs<TI, TO, VEC, 8>(a, ids, padding, s);
@@ -560,9 +548,7 @@ static int launch_runs_of(const RunArgs &a, const int64_t *ids, int64_t padding,
         else if (lanes <= 32) launch_runs<TI, TO, VEC, 32>(a, ids, padding, s);
         else launch_runs<TI, TO, VEC, 64>(a, ids, padding, s);
     } else {
-        if (lanes <= 4) launch_runs<TI, TO, 1, 4>(a, ids, padding, s);
-        else if (lanes <= 16) launch_runs<TI, TO, 1, 16>(a, ids, padding, s);
-        else launch_runs<TI, TO, 1, 64>(a, ids, padding, s);
+        launch_runs<TI, TO, 1, 8>(a, ids, padding, s);  // rows of less than 16 bytes: at most seven elements
     }
     RBG_HIP(hipGetLastError());
     return RBG_OK;
@@ -591,25 +577,22 @@ int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dty
     if ((n_rows && !table) || !ids || !out) return fail(RBG_EINVAL, "NULL pointer");
     const int size = elem_size(dtype);
     if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) % size) return fail(RBG_EINVAL, "a table is not aligned to its type");
-    const bool wide = on_16(table) && on_16(out) && d * size % 16 == 0 && ldt * size % 16 == 0 && ldo * size % 16 == 0;
+    const bool wide = d * size >= 16;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
         constexpr int VEC = 16 / (int)sizeof(E);
-        const bool nt = n * d * size > 32 << 20;
         auto go = [&](auto kernel, int G) {
             const int64_t per = 256 / G * 4;
             hipLaunchKernelGGL(kernel, dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n, d, scale,
-                               (E *)out, ldo, nt);
+                               (E *)out, ldo);
         };
-        const int lanes = wide ? d / VEC : d;
+        const int lanes = wide ? (d + VEC - 1) / VEC : d;
         if (wide) {
             if (lanes <= 4) go(lookup_kernel<E, VEC, 4>, 4);
             else if (lanes <= 16) go(lookup_kernel<E, VEC, 16>, 16);
             else go(lookup_kernel<E, VEC, 64>, 64);
         } else {
-            if (lanes <= 4) go(lookup_kernel<E, 1, 4>, 4);
-            else if (lanes <= 16) go(lookup_kernel<E, 1, 16>, 16);
-            else go(lookup_kernel<E, 1, 64>, 64);
+            go(lookup_kernel<E, 1, 8>, 8);  // rows of less than 16 bytes: at most seven elements
         }
         RBG_HIP(hipGetLastError());
         return (int)RBG_OK;
@@ -670,9 +653,8 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
         }
     }
     RBG_HIP(hipGetLastError());
-    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0,
-                    n_rows * d * out_size > 32 << 20};
-    const bool wide = on_16(grad) && reinterpret_cast<uintptr_t>(out) % (16 / size * out_size) == 0 && d * size % 16 == 0 && ldg * size % 16 == 0;
+    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0};
+    const bool wide = d * size >= 16;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
         return out_dtype == dtype ? launch_runs_of<E, E>(a, ids, padding_idx, wide, s) : launch_runs_of<E, float>(a, ids, padding_idx, wide, s);

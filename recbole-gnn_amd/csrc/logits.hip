@@ -37,14 +37,15 @@ struct RowShape {
     __device__ __forceinline__ int at(int x) const { return x < head ? x : tail + (x - head); }
 };
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-// 16 bytes of a gradient.  One that the L2s cannot hold anyway (`nt`) goes past them: written back line by line it would compete with the
-// logits still to be read (2048 x 40 982 bf16, value and gradient: 91.6 us with plain stores, 73.8 us).
-__device__ __forceinline__ void put16(void *p, const void *v, bool nt) {
+// 16 bytes of a gradient.  Rows that a workgroup writes (NT) go past the caches: what these hold is then logits, of which a second reader
+// finds more (value and gradient of the preference loss: 172 us with plain stores and 139 us past the caches at 4 096 x 40 982 bf16, 107
+// and 86 at 1 200 x 40 001 fp32; of the distillation 77 and 73 at 2 048 x 40 982 bf16; alike at 600 x 40 001 bf16).  Compile-time:
+// with both kinds of store behind a condition the compiler makes one of them, the plain one.
+template <bool NT>
+__device__ __forceinline__ void put16(void *p, const void *v) {
     u32x4 x;
     __builtin_memcpy(&x, v, 16);
-    if (nt) __builtin_nontemporal_store(x, reinterpret_cast<u32x4 *>(p));
+    if constexpr (NT) __builtin_nontemporal_store(x, reinterpret_cast<u32x4 *>(p));
     else *reinterpret_cast<u32x4 *>(p) = x;
 }
 
@@ -144,7 +145,7 @@ __device__ __forceinline__ MaxSum scan_row(const T *__restrict__ z, const RowSha
 // z and g may be the same row: an element is read and written by the same thread.
 template <class T, int TH, int U>
 __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &sh, int c0, int c1, bool loose, float m, float c, float a,
-                                          int hot, float more, bool nt) {
+                                          int hot, float more) {
     constexpr int E = RowShape<T>::E;
     const Vec<T, E> *body = reinterpret_cast<const Vec<T, E> *>(z + sh.head);
     Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
@@ -173,7 +174,7 @@ __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &s
 #pragma unroll
             for (int e = 0; e < E; ++e) v[u].v[e] = from_f32<T>(x[e]);
             if (wide) {
-                put16(out + i, &v[u], nt);
+                put16<(TH > kWave)>(out + i, &v[u]);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v[u].v[e];
@@ -189,7 +190,7 @@ __device__ __forceinline__ void write_row(const T *z, T *g, const RowShape<T> &s
 }
 
 template <class T, int TH>
-__device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, int c1, bool loose, bool nt) {
+__device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, int c1, bool loose) {
     constexpr int E = RowShape<T>::E;
     Vec<T, E> *out = reinterpret_cast<Vec<T, E> *>(g + sh.head);
     const bool wide = on_16_dev(out);
@@ -199,7 +200,7 @@ __device__ __forceinline__ void zero_row(T *g, const RowShape<T> &sh, int c0, in
     for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(0.f);
     for (int i = c0 + tid; i < c1; i += TH) {
         if (wide) {
-            put16(out + i, &v, nt);
+            put16<(TH > kWave)>(out + i, &v);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) g[sh.head + i * E + e] = v.v[e];
@@ -229,7 +230,6 @@ struct DistillArgs {
     int64_t ldg;
     MaxSum *part;  // [n][S] when a row is split
     float *zt;     // [n][k] when a row is split: the entries' logits (the gradient may overwrite them)
-    bool nt;       // the gradient goes past the caches
 };
 
 struct Entries {
@@ -380,9 +380,8 @@ __global__ __launch_bounds__(TH, NC <= 12 ? 5 : 4) void distill_row_kernel(const
     const MaxSum st = block_join<TH>(r, a.c, sh.red);
     if constexpr (TH == kWave) __syncthreads();  // (block_join's own barrier hands over the entries elsewhere)
     entries_loss(a, row, sh, st);                // (the other waves are storing meanwhile: at the end it would prolong the workgroup)
-    const bool nt = TH >= 512 || a.nt;           // (512 threads: rows of over 16 KB, and at least 512 of them)
     if (distill_empty(sh, st)) {
-        zero_row<T, TH>(g, rs, 0, rs.nb, true, nt);
+        zero_row<T, TH>(g, rs, 0, rs.nb, true);
     } else {
         const float w = a.row_w ? a.row_w[row] : 1.f;
         const float s = w * a.T / st.s;
@@ -396,7 +395,7 @@ __global__ __launch_bounds__(TH, NC <= 12 ? 5 : 4) void distill_row_kernel(const
 #pragma unroll
             for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(s * exp2_fast((to_f32(as_elems<T, E>(v[u]).v[e]) - st.m) * a.c));
             if (wide) {
-                put16(out + i, &o, nt);
+                put16<(TH > kWave)>(out + i, &o);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) g[rs.head + i * E + e] = o.v[e];
@@ -421,11 +420,11 @@ __global__ __launch_bounds__(TH) void distill_long_kernel(const DistillArgs a) {
     __syncthreads();
     entries_loss(a, row, sh, st);
     if (distill_empty(sh, st)) {
-        zero_row<T, TH>(g, rs, 0, rs.nb, true, a.nt);
+        zero_row<T, TH>(g, rs, 0, rs.nb, true);
         return;
     }
     const float w = a.row_w ? a.row_w[row] : 1.f;
-    write_row<T, TH, 4>(z, g, rs, 0, rs.nb, true, st.m, a.c, w * a.T / st.s, -1, 0.f, a.nt);
+    write_row<T, TH, 4>(z, g, rs, 0, rs.nb, true, st.m, a.c, w * a.T / st.s, -1, 0.f);
     __syncthreads();
     fix_entries<T, TH>(a, g, rs, 0, rs.nb, true, sh, st, w);
 }
@@ -476,11 +475,11 @@ __global__ __launch_bounds__(TH) void distill_grad_kernel(const DistillArgs a) {
     part_of(rs.nb, blockIdx.x, gridDim.x, c0, c1);
     const bool loose = blockIdx.x == 0;
     if (distill_empty(sh, st)) {
-        zero_row<T, TH>(g, rs, c0, c1, loose, a.nt);
+        zero_row<T, TH>(g, rs, c0, c1, loose);
         return;
     }
     const float w = a.row_w ? a.row_w[row] : 1.f;
-    write_row<T, TH, 4>(z, g, rs, c0, c1, loose, st.m, a.c, w * a.T / st.s, -1, 0.f, a.nt);
+    write_row<T, TH, 4>(z, g, rs, c0, c1, loose, st.m, a.c, w * a.T / st.s, -1, 0.f);
     __syncthreads();
     fix_entries<T, TH>(a, g, rs, c0, c1, loose, sh, st, w);
 }
@@ -542,7 +541,7 @@ __global__ __launch_bounds__(kWave) void logp_join_kernel(const LogpArgs a, int 
 // Part `part` of `parts` of a row's gradient w (onehot - softmax), by TH threads; a row of gradient 0 is not read.
 template <class T, int TH>
 __device__ __forceinline__ void grad_row(const void *zv, int64_t ldz, int V, const int64_t *targets, const float *stats, int64_t row, float w,
-                                         void *gv, int64_t ldg, int part, int parts, bool nt) {
+                                         void *gv, int64_t ldg, int part, int parts) {
     const int64_t t = targets[row];
     const T *z = (const T *)zv + row * ldz;
     T *g = (T *)gv + row * ldg;
@@ -556,22 +555,22 @@ __device__ __forceinline__ void grad_row(const void *zv, int64_t ldz, int V, con
         m = stats[2 * row], s = stats[2 * row + 1];
         none = m == -INFINITY && s == 0.f;
     }
-    if (none) zero_row<T, TH>(g, rs, c0, c1, loose, nt);
-    else write_row<T, TH, 4>(z, g, rs, c0, c1, loose, m, kLog2e, -w / s, (int)t, w, nt);
+    if (none) zero_row<T, TH>(g, rs, c0, c1, loose);
+    else write_row<T, TH, 4>(z, g, rs, c0, c1, loose, m, kLog2e, -w / s, (int)t, w);
 }
 
 template <class T, int TH>
 __device__ __forceinline__ void clear_row(const void *zv, int64_t ldz, int V, int64_t row, void *gv, int64_t ldg) {
     const RowShape<T> rs((const T *)zv + row * ldz, V);
-    zero_row<T, TH>((T *)gv + row * ldg, rs, 0, rs.nb, true, false);
+    zero_row<T, TH>((T *)gv + row * ldg, rs, 0, rs.nb, true);
 }
 
 // One workgroup per row and part; row = the last one first: what the pass before read last is what the caches still hold.
 template <class T, int TH>
 __global__ __launch_bounds__(TH) void logp_grad_kernel(const void *z, int64_t ldz, int V, const int64_t *targets, const float *stats,
-                                                       const float *row_g, void *g, int64_t ldg, bool nt) {
+                                                       const float *row_g, void *g, int64_t ldg) {
     const int64_t row = (int64_t)gridDim.y - 1 - blockIdx.y;
-    grad_row<T, TH>(z, ldz, V, targets, stats, row, row_g[row], g, ldg, blockIdx.x, gridDim.x, nt);
+    grad_row<T, TH>(z, ldz, V, targets, stats, row, row_g[row], g, ldg, blockIdx.x, gridDim.x);
 }
 
 __device__ __forceinline__ float sigmoid_d(float h, float smoothing) {  // d loss / d margin
@@ -663,7 +662,7 @@ __global__ __launch_bounds__(1024) void pair_small_kernel(const LogpArgs a, int6
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         for (int64_t row = lo[k] + w; row < hi[k]; row += 16)
-            grad_row<T, kWave>(a.z, a.ldz, a.V, a.targets, a.stats, row, k ? -d : d, gv, ldg, 0, 1, false);
+            grad_row<T, kWave>(a.z, a.ldz, a.V, a.targets, a.stats, row, k ? -d : d, gv, ldg, 0, 1);
     // rows in front of the first sequence and behind the last
     const int64_t r0 = i == 0 ? 0 : hi[1], r1 = i == 0 ? lo[0] : m;
     if (i == 0 || i + 1 == gridDim.x)
@@ -707,9 +706,6 @@ static int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
 
 // Workgroups per row of a pass that needs nothing from the rest of the row: 256 threads x 4 chunks each.
 static int grad_parts(int64_t V, int elem) { return (int)std::max<int64_t>(1, std::min<int64_t>((V * elem + 16383) / 16384, 1024)); }
-
-// A gradient of more than the eight L2s' 32 MB.
-static bool past_caches(int64_t n, int64_t V, int elem) { return n * V * elem > 32 << 20; }
 
 static int check_rows(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V) {
     if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
@@ -780,16 +776,15 @@ static int launch_logp_grad(const T *z, int64_t ldz, int64_t m, int64_t V, const
                             T *g, int64_t ldg, hipStream_t s) {
     const int S = grad_parts(V, sizeof(T));
     const int64_t slices = (m + kMaxGridY - 1) / kMaxGridY;
-    const bool nt = past_caches(m, V, sizeof(T));
     for (int64_t k = slices - 1; k >= 0; --k) {
         const int64_t r0 = k * kMaxGridY, cnt = std::min(kMaxGridY, m - r0);
         const dim3 grid(S, (unsigned)cnt);
         if (V * (int64_t)sizeof(T) <= 4096)
             hipLaunchKernelGGL((logp_grad_kernel<T, 64>), grid, dim3(64), 0, s, z + r0 * ldz, ldz, (int)V, targets + r0, stats + 2 * r0,
-                               row_g + r0, g + r0 * ldg, ldg, nt);
+                               row_g + r0, g + r0 * ldg, ldg);
         else
             hipLaunchKernelGGL((logp_grad_kernel<T, 256>), grid, dim3(256), 0, s, z + r0 * ldz, ldz, (int)V, targets + r0, stats + 2 * r0,
-                               row_g + r0, g + r0 * ldg, ldg, nt);
+                               row_g + r0, g + r0 * ldg, ldg);
     }
     RBG_HIP(hipGetLastError());
     return RBG_OK;
@@ -830,7 +825,7 @@ int rbg_distill_topk(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V
         if (int rc = check_grad(z, ldz, dtype, n, V, grad, ldg)) return rc;
     const int S = row_parts(n, V);
     DistillArgs a{z, ldz, (int)V, k, idx, val, (float)(1.4426950408889634 / (double)T), T, row_w, loss, stats, grad, ldg, (MaxSum *)workspace,
-                  (float *)((char *)workspace + round16(n * S * (int64_t)sizeof(MaxSum))), past_caches(n, V, elem_size(dtype))};
+                  (float *)((char *)workspace + round16(n * S * (int64_t)sizeof(MaxSum)))};
     return with_elem(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, V, (hipStream_t)stream); });
 }
 
@@ -848,7 +843,7 @@ int rbg_distill_topk_backward(const void *z, int64_t ldz, int dtype, int64_t n, 
         typedef decltype(t) E;
         for (int64_t r0 = 0; r0 < n; r0 += kMaxGridY) {
             const DistillArgs a{(const E *)z + r0 * ldz, ldz, (int)V, k, idx + r0 * k, val + r0 * k, (float)(1.4426950408889634 / (double)T), T,
-                                row_w ? row_w + r0 : nullptr, nullptr, const_cast<float *>(stats) + 2 * r0, (E *)grad + r0 * ldg, ldg, nullptr, nullptr, past_caches(n, V, elem_size(dtype))};
+                                row_w ? row_w + r0 : nullptr, nullptr, const_cast<float *>(stats) + 2 * r0, (E *)grad + r0 * ldg, ldg, nullptr, nullptr};
             const dim3 grid(S, (unsigned)std::min(kMaxGridY, n - r0));
             hipLaunchKernelGGL((distill_grad_kernel<E, 256, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
         }

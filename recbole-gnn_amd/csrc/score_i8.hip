@@ -37,7 +37,7 @@ __device__ __forceinline__ float magnitude(float x) {  // NaN counts as infinite
     return v < INFINITY ? v : INFINITY;
 }
 
-// Rows that start on 16 bytes: G lanes per row hold NC vectors each, read once.
+// G lanes per row hold NC vectors each, read once.
 template <class T, int G, int NC>
 __global__ __launch_bounds__(256) void quantize_kernel(const T *__restrict__ x, int64_t ldx, int64_t n, int K, int8_t *__restrict__ codes,
                                                        int ldc, float *__restrict__ scale) {
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *__restrict__ x, 
     for (int u = 0; u < NC; ++u) {
         const int c = (u * G + sub) * E;
         if (c + E <= K) {
-            v[u] = *reinterpret_cast<const Vec<T, E> *>(p + c);
+            v[u] = load_any<T, E>(p + c);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) v[u].v[e] = c + e < K ? p[c + e] : from_f32<T>(0.f);
@@ -89,9 +89,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *__restrict__ x, 
     }
 }
 
-// Rows that start anywhere, or are too long for that: one workgroup per row, which it reads twice.
+// Longer rows: one workgroup per row, which it reads twice.
 template <class T>
-__global__ __launch_bounds__(256) void quantize_any_kernel(const T *__restrict__ x, int64_t ldx, int64_t K, int8_t *__restrict__ codes, int64_t ldc,
+__global__ __launch_bounds__(256) void quantize_long_kernel(const T *__restrict__ x, int64_t ldx, int64_t K, int8_t *__restrict__ codes, int64_t ldc,
                                                            float *__restrict__ scale) {
     __shared__ float red[4];
     const int64_t row = blockIdx.x;
@@ -117,13 +117,12 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(const T *__restrict__
 template <class T>
 static int launch_quantize(const T *x, int64_t ldx, int64_t n, int64_t K, int8_t *codes, int64_t ldc, float *scale, hipStream_t s) {
     constexpr int E = 16 / (int)sizeof(T);
-    const bool wide = on_16(x) && ldx * (int64_t)sizeof(T) % 16 == 0;
     auto blocks = [&](int per) { return dim3((unsigned)((n + per - 1) / per)); };
-    if (wide && ldc <= 32 * E) hipLaunchKernelGGL((quantize_kernel<T, 32, 1>), blocks(8), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
-    else if (wide && ldc <= 128 * E) hipLaunchKernelGGL((quantize_kernel<T, 64, 2>), blocks(4), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
-    else if (wide && ldc <= 1024 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 4>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
-    else if (wide && ldc <= 4096 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 16>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
-    else hipLaunchKernelGGL((quantize_any_kernel<T>), blocks(1), dim3(256), 0, s, x, ldx, K, codes, ldc, scale);
+    if (ldc <= 32 * E) hipLaunchKernelGGL((quantize_kernel<T, 32, 1>), blocks(8), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else if (ldc <= 128 * E) hipLaunchKernelGGL((quantize_kernel<T, 64, 2>), blocks(4), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else if (ldc <= 1024 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 4>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else if (ldc <= 4096 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 16>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
+    else hipLaunchKernelGGL((quantize_long_kernel<T>), blocks(1), dim3(256), 0, s, x, ldx, K, codes, ldc, scale);
     RBG_HIP(hipGetLastError());
     return RBG_OK;
 }

@@ -17,11 +17,22 @@ inline int elem_size(int dtype) { return dtype == RBG_F32 ? 4 : 2; }
 __device__ __forceinline__ bool on_16_dev(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// N consecutive elements moved by one load or store; the loads and stores below state the alignment they rely on.
+// N consecutive elements moved by one load or store (of 16 bytes at most; longer ones by several).
 template <class T, int N>
 struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The same from and to any element boundary: global memory takes 16-byte accesses at every address of an element on this target.
+template <class T, int N>
+__device__ __forceinline__ Vec<T, N> load_any(const T *p) {
+    Vec<T, N> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_any(T *p, const Vec<T, N> &v) { __builtin_memcpy(p, &v, sizeof(v)); }
 
 // All arithmetic is in 32 bits; a store rounds once, to nearest even (what the casts compile to on gfx950).
 template <class T>
