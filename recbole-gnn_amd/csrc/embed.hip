@@ -11,12 +11,14 @@
 // row of the gradient is written once.
 //
 // The sort: up to kRankMax places, a place's rank is counted outright — the number of (id, place) pairs in front of it — from the
-// ids staged in LDS: N^2 compares, all independent, in one launch.  Above, least-significant-digit radix passes of
-// up to nine bits, three launches each (digit counts per tile, their prefix per digit, a stable scatter).
+// ids staged in LDS: N^2 compares, 64 to an instruction, in one launch.  Above, least-significant-digit radix passes of
+// up to nine bits: to kMoveMax places one launch each, which counts the next pass's digits as it goes (and one launch for the first
+// pass's); beyond, three each (digit counts per tile, their prefix per digit, a stable scatter).
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vocab_common.h"
 
@@ -71,53 +73,191 @@ __device__ __forceinline__ uint32_t key_of(const int64_t *ids, int64_t i, int64_
     return id >= 0 && id < n_rows && id != padding ? (uint32_t)id : (uint32_t)n_rows;
 }
 
-// Rank by counting: a workgroup ranks P places.  Its 64-lane waves hold them 64 / P times over; wave and copy say which part of the
-// places a lane counts over, out of LDS: two instructions for 64 pairs, since all but the workgroup's own places lie wholly in front of or
-// wholly behind the ranked ones.
-template <int P>
+// Rank by counting: a workgroup of 16 waves ranks 16 Q places, a wave Q of them.  The wave holds its places' keys in scalar registers and 64
+// other places' in a vector register: one compare for 64 pairs, and a count of its bits.  Every second place's bits are counted by the
+// scalar unit, which the CU's 16 waves share, the others lane by lane.  Only the step that holds the wave's own places
+// looks at positions: all others lie wholly in front of them (an equal key counts) or wholly behind (it does not).
+template <int Q>
 __global__ __launch_bounds__(1024) void rank_kernel(const int64_t *__restrict__ ids, int n, int64_t n_rows, int64_t padding,
                                                     uint32_t *__restrict__ keys, uint32_t *__restrict__ places, uint32_t *count) {
-    constexpr int PARTS = 16 * (64 / P);
-    __shared__ __align__(16) uint32_t all[kRankMax];
-    __shared__ uint32_t before[PARTS][P];
-    const int n4 = (n + 3) & ~3;
+    constexpr int U = 8;  // steps in flight
+    __shared__ uint32_t all[kRankMax];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n64 = (n + 63) & ~63;
 #pragma unroll 8
-    for (int j = threadIdx.x; j < n4; j += 1024) all[j] = j < n ? key_of(ids, j, n_rows, padding) : 0xffffffffu;
+    for (int j = threadIdx.x; j < n64; j += 1024) all[j] = j < n ? key_of(ids, j, n_rows, padding) : 0xffffffffu;
     if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
-    const int own = threadIdx.x % P, part = threadIdx.x / P;
-    const int i0 = blockIdx.x * P, i = i0 + own;
-    const uint32_t mine = i < n ? all[i] : 0u;
-    // of equal ids those in front come first: key <= mine for j < i, key < mine behind (parts an odd number of 16-byte pieces long: a wave's
-    // copies then read different banks)
-    const int per = ((n4 / 4 + PARTS - 1) / PARTS | 1) * 4, j0 = min(part * per, n4), j1 = min(j0 + per, n4);
-    uint32_t r = 0;
-    int j = j0;
-    const int ja = min(j1, i0), jb = min(j1, i0 + P);
-#pragma unroll 8
-    for (; j < ja; j += 4) {
-        const uint4 k = *reinterpret_cast<const uint4 *>(all + j);
-        r += k.x <= mine, r += k.y <= mine, r += k.z <= mine, r += k.w <= mine;
+    const int i0 = (blockIdx.x * 16 + w) * Q;
+    if (i0 >= n) return;
+    uint32_t mine[Q], rank[Q], part[Q];  // (a wave's count of a place, or its lanes' counts)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        mine[q] = __builtin_amdgcn_readfirstlane(all[min(i0 + q, n - 1)]);
+        rank[q] = part[q] = 0;
     }
-    for (; j < jb; ++j) r += all[j] < mine || (all[j] == mine && j < i);
-#pragma unroll 8
-    for (; j < j1; j += 4) {
-        const uint4 k = *reinterpret_cast<const uint4 *>(all + j);
-        r += k.x < mine, r += k.y < mine, r += k.z < mine, r += k.w < mine;
+    auto step = [&](uint32_t k, auto ahead) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const bool in_front = ahead.value ? k <= mine[q] : k < mine[q];
+            if (q & 1) part[q] += in_front;
+            else rank[q] += __popcll(__ballot(in_front));
+        }
+    };
+    auto steps = [&](int from, int to, auto ahead) {  // places [from, to), both multiples of 64
+        int j = from;
+        for (; j + 64 * U <= to; j += 64 * U) {
+            uint32_t k[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = all[j + 64 * u + lane];
+#pragma unroll
+            for (int u = 0; u < U; ++u) step(k[u], ahead);
+        }
+        for (; j < to; j += 64) step(all[j + lane], ahead);
+    };
+    const int own = i0 & ~63;  // (64 is a multiple of Q: one step holds all of the wave's places)
+    steps(0, own, std::true_type{});
+    {
+        const uint32_t k = all[own + lane];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) rank[q] += __popcll(__ballot(k < mine[q] || (k == mine[q] && own + lane < i0 + q)));
     }
-    before[part][own] = r;
-    __syncthreads();
-    if (threadIdx.x < P && i < n) {
-        uint32_t rank = 0;
-#pragma unroll 16
-        for (int q = 0; q < PARTS; ++q) rank += before[q][own];
-        keys[rank] = mine;
-        places[rank] = (uint32_t)i;
+    steps(own + 64, n64, std::false_type{});
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        if (q & 1)
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) part[q] += __shfl_xor(part[q], o);
+        const uint32_t r = rank[q] + (q & 1 ? part[q] : 0u);
+        if (lane == 0 && i0 + q < n) keys[r] = mine[q], places[r] = (uint32_t)(i0 + q);
     }
 }
 
-// Radix pass, first launch: how often each digit occurs in each tile -> hist[digit][tile].  (ids: the first pass.)
-template <int R>  // a tile is 256 R places
+// A wave's rank of each of its R x 64 places among those with the same digit, in order; slots[digit] counts them.
+template <int R>
+__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[R], const bool (&there)[R], int bits, uint32_t *slots, uint32_t (&rank)[R]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        unsigned long long same = __ballot(there[u]);
+        for (int b = 0; b < bits; ++b) {
+            const bool set = (digit[u] >> b) & 1u;
+            const unsigned long long one = __ballot(set);
+            same &= set ? one : ~one;
+        }
+        const int ahead = __popcll(same & ((1ull << lane) - 1ull));
+        volatile uint32_t *slot = &slots[digit[u]];
+        const uint32_t before = *slot;  // (a wave's LDS accesses are served in the order it issues them)
+        rank[u] = before + ahead;
+        if (there[u] && ahead == 0) *slot = before + __popcll(same);
+    }
+}
+
+// The exclusive prefix of one value per thread over a workgroup of TH threads; `part`: TH / 64 entries of LDS.
+template <int TH>
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *part) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) part[w] = x;
+    __syncthreads();
+    uint32_t r = x - v;
+    for (int q = 0; q < w; ++q) r += part[q];
+    return r;
+}
+
+// One launch per pass.  Tiles of 2 048 places, counts[pass][tile][digit].
+constexpr int kBins = 1 << kMaxBits, kMoveTile = 2048, kMoveMax = 1 << 16, kMaxPasses = 4;
+constexpr int kMoveTiles = kMoveMax / kMoveTile;
+
+// The first pass's counts; the later passes' are cleared.
+__global__ __launch_bounds__(512) void move_count_kernel(const int64_t *ids, int n, int64_t n_rows, int64_t padding, int bits, int passes,
+                                                         uint32_t *counts, uint32_t *count) {
+    __shared__ uint32_t h[kBins];
+    h[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMoveTile / 512; ++u) {
+        const int i = blockIdx.x * kMoveTile + u * 512 + threadIdx.x;
+        if (i < n) atomicAdd(&h[key_of(ids, i, n_rows, padding) & ((1u << bits) - 1)], 1u);
+    }
+    __syncthreads();
+    counts[blockIdx.x * kBins + threadIdx.x] = h[threadIdx.x];
+    for (int q = 1; q < passes; ++q) counts[((int64_t)q * gridDim.x + blockIdx.x) * kBins + threadIdx.x] = 0;
+}
+
+// A pass: a place moves to (places of smaller digits) + (of its digit in earlier tiles) + (of its digit before it here).  A thread per
+// digit adds up the tiles' counts, which are few.  COUNT: the next pass's counts are taken where the places arrive, first in LDS: a place
+// in every 50 may be the same row's, and adding each to memory by itself takes 45 us of a pass of 65 536, this way 3.
+template <bool COUNT>
+__global__ __launch_bounds__(512) void move_kernel(const int64_t *ids, const uint32_t *keys, const uint32_t *places, int n, int64_t n_rows,
+                                                   int64_t padding, int shift, int bits, const uint32_t *counts, uint32_t *next_counts,
+                                                   uint32_t *keys_out, uint32_t *places_out) {
+    constexpr int R = kMoveTile / 512;
+    __shared__ uint32_t at[8][kBins];  // places of a digit in each wave's eighth, then where the next one goes
+    __shared__ uint32_t part[8];
+    __shared__ uint32_t arrive[COUNT ? kMoveTiles : 1][kBins];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint32_t mask = (1u << bits) - 1;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) at[q][threadIdx.x] = 0;
+    if constexpr (COUNT)
+        for (int t = 0; t < (int)gridDim.x; ++t) arrive[t][threadIdx.x] = 0;
+    __syncthreads();
+    const int i0 = blockIdx.x * kMoveTile + w * (64 * R);
+    uint32_t key[R], digit[R], rank[R];
+    bool there[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int i = i0 + u * 64 + lane;
+        there[u] = i < n;
+        key[u] = there[u] ? (ids ? key_of(ids, i, n_rows, padding) : keys[i]) : 0u;
+        digit[u] = (key[u] >> shift) & mask;
+    }
+    uint32_t total = 0, before = 0;
+    for (int t0 = 0; t0 < (int)gridDim.x; t0 += 16) {
+        uint32_t c[16];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) c[t] = t0 + t < (int)gridDim.x ? counts[(t0 + t) * kBins + threadIdx.x] : 0u;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            total += c[t];
+            before += t0 + t < (int)blockIdx.x ? c[t] : 0u;
+        }
+    }
+    wave_ranks<R>(digit, there, bits, at[w], rank);
+    uint32_t go = block_prefix<512>(total, part) + before;  // (its barrier also ends the counting)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const uint32_t c = at[q][threadIdx.x];
+        at[q][threadIdx.x] = go;
+        go += c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        if (!there[u]) continue;
+        const uint32_t to = at[w][digit[u]] + rank[u];
+        keys_out[to] = key[u];
+        places_out[to] = places ? places[i0 + u * 64 + lane] : (uint32_t)(i0 + u * 64 + lane);
+        if constexpr (COUNT) atomicAdd(&arrive[to / kMoveTile][(key[u] >> (shift + bits)) & mask], 1u);
+    }
+    if constexpr (COUNT) {  // (integer sums: the order of the additions does not show)
+        __syncthreads();
+        for (int t = 0; t < (int)gridDim.x; ++t) {
+            const uint32_t c = arrive[t][threadIdx.x];
+            if (c) atomicAdd(&next_counts[t * kBins + threadIdx.x], c);
+        }
+    }
+}
+
+// Three launches per pass.  First: how often each digit occurs in each tile -> hist[digit][tile].  (ids: the first pass.)
+constexpr int kTile = 2048;
 __global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, const uint32_t *keys, int64_t n, int64_t n_rows, int64_t padding,
                                                           int shift, int bits, uint32_t *hist, uint32_t *count) {
     __shared__ uint32_t h[1 << kMaxBits];
@@ -125,9 +265,9 @@ __global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, co
     for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
-    const int64_t i0 = (int64_t)blockIdx.x * (256 * R);
+    const int64_t i0 = (int64_t)blockIdx.x * kTile;
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
+    for (int u = 0; u < kTile / 256; ++u) {
         const int64_t i = i0 + u * 256 + threadIdx.x;
         if (i < n) {
             const uint32_t k = ids ? key_of(ids, i, n_rows, padding) : keys[i];
@@ -142,22 +282,12 @@ __global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, co
 __global__ __launch_bounds__(256) void digit_prefix_kernel(uint32_t *hist, int tiles, uint32_t *total) {
     __shared__ uint32_t part[4];
     uint32_t *h = hist + (int64_t)blockIdx.x * tiles;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint32_t run = 0;
     for (int t0 = 0; t0 < tiles; t0 += 256) {
         const int t = t0 + threadIdx.x;
         const uint32_t v = t < tiles ? h[t] : 0u;
-        uint32_t x = v;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t y = __shfl_up(x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 63) part[w] = x;
-        __syncthreads();
-        uint32_t base = run;
-        for (int q = 0; q < w; ++q) base += part[q];
-        if (t < tiles) h[t] = base + x - v;
+        const uint32_t ahead = block_prefix<256>(v, part);
+        if (t < tiles) h[t] = run + ahead;
         run += part[0] + part[1] + part[2] + part[3];
         __syncthreads();
     }
@@ -165,7 +295,6 @@ __global__ __launch_bounds__(256) void digit_prefix_kernel(uint32_t *hist, int t
 }
 
 // Third launch: every place moves to (places of smaller digits) + (of its digit in earlier tiles) + (of its digit before it here).
-template <int R>
 __global__ __launch_bounds__(256) void digit_scatter_kernel(const int64_t *ids, const uint32_t *keys, const uint32_t *places, int64_t n,
                                                             int64_t n_rows, int64_t padding, int shift, int bits, const uint32_t *hist,
                                                             const uint32_t *total, uint32_t *keys_out, uint32_t *places_out) {
@@ -174,39 +303,23 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(const int64_t *ids, 
     const int bins = 1 << bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     for (int d = threadIdx.x; d < 4 * (1 << kMaxBits); d += 256) (&at[0][0])[d] = 0;
     __syncthreads();
-    const int64_t i0 = (int64_t)blockIdx.x * (256 * R) + w * (64 * R);
-    uint32_t key[R], rank[R];
+    constexpr int R = kTile / 256;
+    const int64_t i0 = (int64_t)blockIdx.x * kTile + w * (64 * R);
+    uint32_t key[R], digit[R], rank[R];
+    bool there[R];
 #pragma unroll
     for (int u = 0; u < R; ++u) {
         const int64_t i = i0 + u * 64 + lane;
-        const bool there = i < n;
-        key[u] = there ? (ids ? key_of(ids, i, n_rows, padding) : keys[i]) : 0u;
-        const uint32_t d = (key[u] >> shift) & (bins - 1);
-        unsigned long long same = __ballot(there);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long one = __ballot((d >> b) & 1u);
-            same &= (d >> b) & 1u ? one : ~one;
-        }
-        const int ahead = __popcll(same & ((1ull << lane) - 1ull));
-        volatile uint32_t *slot = &at[w][d];
-        const uint32_t old = *slot;       // (a wave's LDS accesses are served in the order it issues them)
-        rank[u] = old + ahead;
-        if (there && ahead == 0) *slot = old + __popcll(same);
+        there[u] = i < n;
+        key[u] = there[u] ? (ids ? key_of(ids, i, n_rows, padding) : keys[i]) : 0u;
+        digit[u] = (key[u] >> shift) & (bins - 1);
     }
+    wave_ranks<R>(digit, there, bits, at[w], rank);
     __syncthreads();
     // start of each digit: exclusive prefix of the totals, two digits per thread
     const uint32_t a = 2 * threadIdx.x < (unsigned)bins ? total[2 * threadIdx.x] : 0u;
     const uint32_t b = 2 * threadIdx.x + 1 < (unsigned)bins ? total[2 * threadIdx.x + 1] : 0u;
-    uint32_t x = a + b;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 63) part[w] = x;
-    __syncthreads();
-    uint32_t first = x - a - b;
-    for (int q = 0; q < w; ++q) first += part[q];
+    const uint32_t first = block_prefix<256>(a + b, part);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int d = 2 * threadIdx.x + k;
@@ -225,7 +338,7 @@ __global__ __launch_bounds__(256) void digit_scatter_kernel(const int64_t *ids, 
     for (int u = 0; u < R; ++u) {
         const int64_t i = i0 + u * 64 + lane;
         if (i < n) {
-            const uint32_t to = at[w][(key[u] >> shift) & (bins - 1)] + rank[u];
+            const uint32_t to = at[w][digit[u]] + rank[u];
             keys_out[to] = key[u];
             places_out[to] = places ? places[i] : (uint32_t)i;
         }
@@ -256,14 +369,14 @@ __device__ __forceinline__ void store_row(T *p, const float (&acc)[VEC], float s
     store_any(p, v);
 }
 
-// First place of the sorted list whose key is not below v, by a whole wave: 64 probes a round.
-__device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t n, uint32_t v) {
+// The first of n sorted keys, `stride` apart, that is not below v, by a whole wave: 64 probes a round.
+__device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t n, uint32_t v, int stride = 1) {
     const int lane = threadIdx.x & 63;
     int64_t lo = 0, cnt = n;  // the answer is in [lo, lo + cnt]
     while (cnt > 0) {
         const int64_t step = (cnt + 63) / 64;
         const int64_t at = lo + (lane + 1) * step - 1;
-        const int below = __popcll(__ballot(at < lo + cnt && keys[at] < v));  // probes 0 .. below - 1 are below v
+        const int below = __popcll(__ballot(at < lo + cnt && keys[at * stride] < v));  // probes 0 .. below - 1 are below v
         const int64_t end = lo + cnt;
         lo += below * step;
         cnt = min(step - 1, end - lo);
@@ -294,7 +407,18 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
             if ((threadIdx.x & 63) == 0) bounds[w] = at;
         }
         __syncthreads();
-        for (int64_t p = bounds[0] + threadIdx.x; p < bounds[1]; p += 256) used[a.keys[p] - (uint32_t)r0] = 1;
+        if (bounds[1] - bounds[0] <= 4096) {
+            for (int64_t p = bounds[0] + threadIdx.x; p < bounds[1]; p += 256) used[a.keys[p] - (uint32_t)r0] = 1;
+        } else if ((int)threadIdx.x < rows) {  // long runs: each row looks for itself
+            int64_t lo = bounds[0], hi = bounds[1];
+            const uint32_t key = (uint32_t)(r0 + threadIdx.x);
+            while (lo < hi) {
+                const int64_t mid = (lo + hi) >> 1;
+                if (a.keys[mid] < key) lo = mid + 1;
+                else hi = mid;
+            }
+            used[threadIdx.x] = lo < bounds[1] && a.keys[lo] == key;
+        }
         __syncthreads();
         if (on)
             for (int q = grp; q < rows; q += 256 / G)
@@ -444,20 +568,14 @@ __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
     for (uint32_t t = blockIdx.x; t < todo; t += gridDim.x) {
         const int64_t c = a.list[t];
         const uint32_t key = a.keys[(c + 1) * a.chunk];
-        int64_t last = c + 1;  // the last chunk that starts with the run's key
-        for (;;) {
-            const int64_t q = last + 1 + (threadIdx.x & 63);
-            const unsigned long long same = __ballot(q < a.chunks && a.keys[q * a.chunk] == key);
-            const int more = ~same ? __builtin_ctzll(~same) : 64;
-            last += more;
-            if (more < 64) break;
-        }
+        // the last chunk that starts with the run's key
+        const int64_t last = c + first_not_below(a.keys + (c + 1) * a.chunk, a.chunks - c - 1, key + 1u, a.chunk);
         // parts c, c + 1, .., last: an equal piece for each lane-group, the pieces joined in order
         const int64_t cnt = last - c + 1, per = (cnt + N - 1) / N;
         const int64_t q0 = c + grp * per, q1 = min(q0 + per, last + 1);
         float acc[VEC] = {};
         if (on) {
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t q = q0; q < q1; ++q) {
                 const float *from = a.part + (2 * q + (q == c ? 1 : 0)) * a.d + col;
 #pragma unroll
@@ -491,7 +609,7 @@ static int chunk_of(int64_t n, int d) {
 
 struct Layout {
     int64_t keys, places, keys2, places2, hist, total, part, list, count, bytes;
-    int chunk, tiles, tile_rounds;
+    int chunk, tiles;
     int64_t chunks;
 };
 
@@ -499,8 +617,7 @@ static Layout layout_of(int64_t n, int d) {
     Layout l{};
     l.chunk = chunk_of(n, d);
     l.chunks = (n + l.chunk - 1) / l.chunk;
-    l.tile_rounds = n <= 1 << 19 ? 2 : 8;  // (at 65 536 places 32 tiles of 2 048 leave most CUs idle: 12 us a scatter)
-    l.tiles = (int)((n + 256 * l.tile_rounds - 1) / (256 * l.tile_rounds));
+    l.tiles = (int)((n + kTile - 1) / kTile);
     int64_t at = 0;
     auto take = [&](int64_t b) {
         const int64_t r = at;
@@ -512,8 +629,8 @@ static Layout layout_of(int64_t n, int d) {
     l.keys = take(4 * n), l.places = take(4 * n);
     if (n > kRankMax) {
         l.keys2 = take(4 * n), l.places2 = take(4 * n);
-        l.hist = take(4ll * (1 << kMaxBits) * l.tiles);
-        l.total = take(4 << kMaxBits);
+        l.hist = take(4ll * kBins * l.tiles * (n <= kMoveMax ? kMaxPasses : 1));
+        l.total = take(4 * kBins);
     }
     l.list = take(4 * l.chunks);
     l.part = take(4ll * 2 * l.chunks * d);
@@ -624,10 +741,10 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
     uint32_t *count = (uint32_t *)(w + l.count);
     uint32_t *keys = (uint32_t *)(w + l.keys), *places = (uint32_t *)(w + l.places);
     if (n > kFewPlaces && n <= kRankMax) {
-        // (16, 32 and 64 places a workgroup measure alike at 8 192; fewer for fewer, so that the CUs have work)
-        if (n <= 4096) hipLaunchKernelGGL((rank_kernel<16>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
-        else if (n <= 8192) hipLaunchKernelGGL((rank_kernel<32>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
-        else hipLaunchKernelGGL((rank_kernel<64>), dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+        // places per wave: few where there are few, so that every CU has a workgroup
+        if (n <= 4096) hipLaunchKernelGGL((rank_kernel<1>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+        else if (n <= 8192) hipLaunchKernelGGL((rank_kernel<2>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+        else hipLaunchKernelGGL((rank_kernel<4>), dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
     } else if (n > kRankMax) {
         int bits = 1;
         while (((int64_t)1 << bits) <= n_rows) ++bits;  // keys 0 .. n_rows
@@ -635,19 +752,25 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
         uint32_t *k2 = (uint32_t *)(w + l.keys2), *p2 = (uint32_t *)(w + l.places2);
         uint32_t *hist = (uint32_t *)(w + l.hist), *total = (uint32_t *)(w + l.total);
         const uint32_t *from_k = nullptr, *from_p = nullptr;
+        if (n <= kMoveMax) hipLaunchKernelGGL(move_count_kernel, dim3(l.tiles), dim3(512), 0, s, ids, (int)n, n_rows, padding_idx, width, passes, hist, count);
         // the last pass ends in (keys, places)
         uint32_t *to_k = passes & 1 ? keys : k2, *to_p = passes & 1 ? places : p2;
         for (int q = 0; q < passes; ++q) {
             const int64_t *src = q == 0 ? ids : nullptr;
-            if (l.tile_rounds == 2) hipLaunchKernelGGL((digit_count_kernel<2>), dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
-            else hipLaunchKernelGGL((digit_count_kernel<8>), dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
-            hipLaunchKernelGGL(digit_prefix_kernel, dim3(1u << width), dim3(256), 0, s, hist, l.tiles, total);
-            if (l.tile_rounds == 2)
-                hipLaunchKernelGGL((digit_scatter_kernel<2>), dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
+            if (n <= kMoveMax) {
+                uint32_t *counts = hist + (int64_t)q * l.tiles * kBins, *next = counts + (int64_t)l.tiles * kBins;
+                if (q + 1 < passes)
+                    hipLaunchKernelGGL((move_kernel<true>), dim3(l.tiles), dim3(512), 0, s, src, from_k, from_p, (int)n, n_rows, padding_idx, q * width, width,
+                                       counts, next, to_k, to_p);
+                else
+                    hipLaunchKernelGGL((move_kernel<false>), dim3(l.tiles), dim3(512), 0, s, src, from_k, from_p, (int)n, n_rows, padding_idx, q * width, width,
+                                       counts, nullptr, to_k, to_p);
+            } else {
+                hipLaunchKernelGGL(digit_count_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
+                hipLaunchKernelGGL(digit_prefix_kernel, dim3(1u << width), dim3(256), 0, s, hist, l.tiles, total);
+                hipLaunchKernelGGL(digit_scatter_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
                                    hist, total, to_k, to_p);
-            else
-                hipLaunchKernelGGL((digit_scatter_kernel<8>), dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
-                                   hist, total, to_k, to_p);
+            }
             from_k = to_k, from_p = to_p;
             to_k = to_k == keys ? k2 : keys, to_p = to_p == places ? p2 : places;
         }

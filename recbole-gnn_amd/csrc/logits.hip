@@ -934,11 +934,12 @@ int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_
     MaxSum *part = (MaxSum *)(w + 2 * round16(8 * m) + round16(4 * m));
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
-        // Up to 256 tokens, 64 and 128 KB a pair, and 1 MB in all: one launch instead of three (40 x 1 683 fp32, four pairs: 13 us a
-        // call, 19 with three).  A workgroup takes a pair's rows sixteen at a time, and the lengths are on the device: all tokens in
-        // one pair cost 16 turns of it at most (at 4 756 tokens of two pairs it would take 560 us).
+        // Up to 256 tokens, 64 and 128 KB a pair, rows of 16 KB and 1 MB in all: one launch instead of three (40 x 1 683 fp32, four
+        // pairs: 13 us a call, 19 with three).  A workgroup takes a pair's rows sixteen at a time, a wave each, and the lengths are on the
+        // device: all tokens in one pair cost 16 turns of it at most (4 756 tokens of two pairs would take 560 us), and a wave
+        // reads a row of 16 KB in four turns (one of 500 KB would take 80 us).
         const int64_t total = m * V * (int64_t)sizeof(E);
-        if (m && m <= 256 && m <= pairs * 64 && total <= 1 << 20 && total <= pairs << 17) {
+        if (m && m <= 256 && m <= pairs * 64 && V * (int64_t)sizeof(E) <= 16 << 10 && total <= 1 << 20 && total <= pairs << 17) {
             const LogpArgs a{z, ldz, (int)V, targets, nullptr, nullptr, nullptr, stats, nullptr};
             hipLaunchKernelGGL((pair_small_kernel<E>), dim3((unsigned)pairs), dim3(1024), 0, s, a, m, offsets, ref, beta, smoothing, pair_w, loss, margin,
                                grad, ldg);

@@ -317,9 +317,9 @@ static int launch_short(const ScoreArgs &a, hipStream_t s) {
     return panels * lines >= 1024 ? launch_short<TO, KS, 2048>(a, 512, s) : launch_short<TO, KS, 512>(a, 1024, s);
 }
 
-// Few users (B <= 16 UT): the table is read once and everything else is small.  16 x 16 tiles straight from the rows, no staging: a
-// wave's load touches 64 bytes of each of 16 items' rows.  KW waves of a workgroup share 16 IT items and split K (their sums meet in LDS);
-// the other 4 / KW have items of their own.
+// Few users (B <= 16 UT), or too few scores for the tiles below: 16 x 16 tiles straight from the rows, no staging: a wave's load touches
+// 64 bytes of each of 16 items' rows.  A workgroup has 16 UT users (blockIdx.y) and KW of its waves share 16 IT items and split K (their
+// sums meet in LDS); the other 4 / KW have items of their own.
 // TU other than void: the users' rows are a.u, of that type and at most kOwnCodes values in all; every workgroup makes their codes for
 // itself in LDS, and the call is one launch.
 constexpr int kOwnCodes = 8192;
@@ -333,12 +333,12 @@ __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
     __shared__ float own_su[16];
     const int pitch = (a.kc + 3) / 4 * 64 + 16;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-    const int64_t j0 = ((int64_t)blockIdx.x * (4 / KW) + w / KW) * (16 * IT);
+    const int64_t j0 = ((int64_t)blockIdx.x * (4 / KW) + w / KW) * (16 * IT), b0 = (int64_t)blockIdx.y * (16 * UT);
     const i32x4 *pu[UT], *pi[IT];
 #pragma unroll
     for (int x = 0; x < UT; ++x) {
         if constexpr (OWN) pu[x] = reinterpret_cast<const i32x4 *>(own + min<int>(m, (int)a.B - 1) * pitch);
-        else pu[x] = reinterpret_cast<const i32x4 *>(a.qu + min<int64_t>(16 * x + m, a.B - 1) * a.ldu);
+        else pu[x] = reinterpret_cast<const i32x4 *>(a.qu + min<int64_t>(b0 + 16 * x + m, a.B - 1) * a.ldu);
     }
 #pragma unroll
     for (int y = 0; y < IT; ++y) pi[y] = reinterpret_cast<const i32x4 *>(a.qi + min<int64_t>(j0 + 16 * y + m, a.n - 1) * a.ldi);
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
         for (int x = 0; x < UT; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int64_t b = 16 * x + 4 * g + r;
+                const int64_t b = b0 + 16 * x + 4 * g + r;
                 if (b < a.B) S[b * a.lds + j] = from_f32<TO>((float)acc[x][y][r] * su[b] * si);
             }
     }
@@ -411,11 +411,13 @@ __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
 
 template <class TO, class TU, int UT>
 static int launch_few(const ScoreArgs &a, hipStream_t s) {
+    const unsigned gy = (unsigned)((a.B + 16 * UT - 1) / (16 * UT));  // (a few)
+    auto blocks = [&](int per) { return dim3((unsigned)((a.n + per - 1) / per), gy); };
     if (a.kc >= 64) {  // 1 KB and more of a row: four waves share it
-        if (a.n <= 16 * 2048) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), dim3((unsigned)((a.n + 31) / 32)), dim3(256), 0, s, a);
+        if (a.n * gy <= 16 * 2048) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), blocks(16), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), blocks(32), dim3(256), 0, s, a);
     } else {
-        hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 1>), dim3((unsigned)((a.n + 127) / 128)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 1>), blocks(128), dim3(256), 0, s, a);
     }
     RBG_HIP(hipGetLastError());
     return RBG_OK;
@@ -578,9 +580,12 @@ static int launch_score(const ScoreArgs &a, hipStream_t s) {
     if (a.kc <= 8) return launch_short<TO, 4>(a, s);
     if (a.B <= 32) return launch_few<TO, void, 2>(a, s);
     if (a.B <= 64) return launch_few<TO, void, 4>(a, s);
-    const int64_t gx = (a.n + 255) / 256, gw = (a.B + 255) / 256;
-    if (gx * gw >= 192 && gx * gw < (1 << 30) && a.ldu <= 1 << 23 && a.ldi <= 1 << 23) {  // (32-bit offsets inside a tile)
-        hipLaunchKernelGGL((score_i8_wide_kernel<TO>), dim3((unsigned)(gx * gw)), dim3(256), 0, s, a, (int)gx, (int)gw);
+    const int64_t wide = ((a.n + 255) / 256) * ((a.B + 255) / 256), small = ((a.n + 127) / 128) * ((a.B + 127) / 128);
+    if (small < 128 && a.kc > 16) return launch_few<TO, void, 4>(a, s);  // (64 x 16 tiles, K over four waves: many times the workgroups)
+    // Rounds of 256 x 256 tiles (one per CU) against 128 x 128 ones, whose products cost 1.37 times as much (690 and 505 us at 4096 x
+    // 16 384 x 8192) but which waste less of the last round and of the edges.  (32-bit offsets inside a wide tile.)
+    if ((wide + 255) / 256 * 4 <= 1.37 * small / 256 && wide < (1 << 30) && a.ldu <= 1 << 23 && a.ldi <= 1 << 23) {
+        hipLaunchKernelGGL((score_i8_wide_kernel<TO>), dim3((unsigned)wide), dim3(256), 0, s, a, (int)((a.n + 255) / 256), (int)((a.B + 255) / 256));
         RBG_HIP(hipGetLastError());
         return RBG_OK;
     }

@@ -80,7 +80,7 @@ def runs_reference(grad, ids, rows, scale, padding):
 
 
 GRAD_SHAPES = [(1, 1, 1), (2, 5, 64), (7, 3, 65), (100, 700, 64), (255, 3, 40), (256, 1000, 513), (257, 1000, 16), (300, 50, 64), (5000, 40, 128), (6144, 40982, 64), (4096, 1, 32), (16384, 1000, 32), (16385, 511, 24),
-               (16385, 512, 8), (20000, 70000, 64), (40000, 3, 100), (50000, 300000, 16), (70001, 100, 1), (33000, 1, 4), (1000, 20, 1024), (3000, 7, 2051)]
+               (16385, 512, 8), (20000, 70000, 64), (40000, 3, 100), (50000, 300000, 16), (70001, 100, 1), (33000, 1, 4), (65536, 140000, 3), (65537, 777, 4), (131072, 300, 2), (150000, 600000, 2), (1000, 20, 1024), (3000, 7, 2051)]
 
 
 @pytest.mark.parametrize("n,rows,d", GRAD_SHAPES)
