@@ -758,12 +758,12 @@ int rbg_quantize_rows_i8(const void *x, int64_t ldx, int dtype, int64_t n, int64
 
 /* The scores of rbg_score_f32 from rows in 8 bits: S[b, j] = su[b] si[j] sum_k qu[b, k] qi[j, k], the sum exact in 32-bit integers
  * (1 <= K <= 131071).  qu [B, ldu]: ldu % 128 == 0, columns [K, ldu) zero (what rbg_quantize_rows_i8 writes); qi [n, ldi]:
- * ldi % 16 == 0, any value in columns [K, K rounded up to 16), which have to be there for the last row too.  qu, qi 16-byte aligned.
- * S [B, lds] of out_dtype, rounded once from 32 bits. */
+ * ldi % 16 == 0, any value in columns [K, K rounded up to 16), which have to be there for the last row too.  qu, qi 16-byte aligned;
+ * ldu, ldi <= 2^23.  S [B, lds] of out_dtype, rounded once from 32 bits. */
 int rbg_score_i8(const int8_t *qu, int64_t ldu, const float *su, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n,
                  int64_t K, void *S, int64_t lds, int out_dtype, void *stream);
 
-/* Both in one call: the rows u [B, K] of `dtype` are quantized (rbg_quantize_rows_i8) and scored (rbg_score_i8); for up to 16 rows of 8 192
+/* Both in one call: the rows u [B, K] of `dtype` are quantized (rbg_quantize_rows_i8) and scored (rbg_score_i8); for up to 16 rows of 2 048
  * values in all it is one launch.  `workspace`: rbg_score_rows_i8_workspace(B, K) bytes, 16-byte aligned. */
 int rbg_score_rows_i8_workspace(int64_t B, int64_t K, int64_t *bytes);
 int rbg_score_rows_i8(const void *u, int64_t ldu, int dtype, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n, int64_t K,

@@ -141,74 +141,6 @@ struct ScoreArgs {
     int K;
 };
 
-// A 128 x 128 tile of S per workgroup of four waves (64 x 64 each: 2 x 2 tiles of 32 x 32); K in steps of 128 bytes, both
-// operands' steps staged in LDS (rows of 128 bytes; 16-byte chunk c of row r at slot c ^ (r / 2 % 8), so that any 16 rows a
-// fragment read touches spread over the banks), the next step in flight in registers.
-template <class TO>
-__global__ __launch_bounds__(256) void score_i8_kernel(const ScoreArgs a) {
-    __shared__ i32x4 lu[128 * 8], li[128 * 8];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t b0 = (int64_t)blockIdx.y * 128, j0 = (int64_t)blockIdx.x * 128;
-    const int steps = (a.kc + 7) / 8;
-    // this thread stages chunk (tid & 7) of rows tid / 8 + 32 q
-    const int sc = threadIdx.x & 7, sr = threadIdx.x >> 3;
-    const i32x4 *pu[4], *pi[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        pu[q] = reinterpret_cast<const i32x4 *>(a.qu + min(b0 + sr + 32 * q, a.B - 1) * a.ldu);
-        pi[q] = reinterpret_cast<const i32x4 *>(a.qi + min(j0 + sr + 32 * q, a.n - 1) * a.ldi);
-    }
-    i32x4 ru[4], ri[4];
-    auto fetch = [&](int t) {
-        const int c = t * 8 + sc;
-        const int ci = min(c, a.kc - 1);  // behind the row's end the users' codes are zero
-#pragma unroll
-        for (int q = 0; q < 4; ++q) ru[q] = pu[q][c], ri[q] = pi[q][ci];
-    };
-    i32x16 acc[2][2] = {};
-    fetch(0);
-    const int m = lane & 31, h = lane >> 5, wu = (w >> 1) * 64, wi = (w & 1) * 64;
-    for (int t = 0; t < steps; ++t) {
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int r = sr + 32 * q;
-            lu[r * 8 + (sc ^ ((r >> 1) & 7))] = ru[q];
-            li[r * 8 + (sc ^ ((r >> 1) & 7))] = ri[q];
-        }
-        __syncthreads();
-        if (t + 1 < steps) fetch(t + 1);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            i32x4 fu[2], fi[2];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int r = 32 * q + m, c = (2 * k + h) ^ ((r >> 1) & 7);
-                fu[q] = lu[(wu + r) * 8 + c];
-                fi[q] = li[(wi + r) * 8 + c];
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fu[x], fi[y], acc[x][y], 0, 0, 0);
-        }
-    }
-    TO *S = (TO *)a.S;
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-        const int64_t j = j0 + wi + 32 * y + m;
-        if (j >= a.n) continue;
-        const float si = a.si[j];
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t b = b0 + wu + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * h;
-                if (b < a.B) S[b * a.lds + j] = from_f32<TO>((float)acc[x][y][r] * a.su[b] * si);
-            }
-    }
-}
-
 // Short rows (K <= 32 KS): the scores are written at the rate of the stores and everything else has to hide behind them.  A workgroup
 // keeps 32 users' codes in registers and walks item tiles of TB bytes of scores per row: each wave multiplies 32 items' codes at a time,
 // taken straight from the table, and puts its scores into LDS, every row shifted by its distance from a 128-byte line.  Whole lines then
@@ -321,12 +253,13 @@ static int launch_short(const ScoreArgs &a, hipStream_t s) {
 // 64 bytes of each of 16 items' rows.  A workgroup has 16 UT users (blockIdx.y) and KW of its waves share 16 IT items and split K (their
 // sums meet in LDS); the other 4 / KW have items of their own.
 // TU other than void: the users' rows are a.u, of that type and at most kOwnCodes values in all; every workgroup makes their codes for
-// itself in LDS, and the call is one launch.
-constexpr int kOwnCodes = 8192;
+// itself in LDS, and the call is one launch.  (At 8 192 values that takes longer than everything else: 357 us for one user of 131 072
+// items x 8 192, 198 with the codes made first.)
+constexpr int kOwnCodes = 2048;
 
 template <class TO, class TU, int UT, int IT, int KW>
 __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
-    constexpr int U = 4;  // steps of 64 bytes in flight
+    constexpr int U = UT * IT >= 8 ? 2 : 4;  // steps of 64 bytes in flight
     constexpr bool OWN = !std::is_void_v<TU>;
     // a row of codes: K rounded up to 64, and 16 more bytes so that the 16 rows of a fragment spread over the banks
     __shared__ alignas(16) int8_t own[OWN ? kOwnCodes + 16 * 80 : 16];
@@ -414,8 +347,10 @@ static int launch_few(const ScoreArgs &a, hipStream_t s) {
     const unsigned gy = (unsigned)((a.B + 16 * UT - 1) / (16 * UT));  // (a few)
     auto blocks = [&](int per) { return dim3((unsigned)((a.n + per - 1) / per), gy); };
     if (a.kc >= 64) {  // 1 KB and more of a row: four waves share it
+        // more items per wave read the users' codes less often, but leave fewer waves
         if (a.n * gy <= 16 * 2048) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), blocks(16), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), blocks(32), dim3(256), 0, s, a);
+        else if (a.n * gy <= 64 * 1024 || a.kc < 128) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), blocks(32), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 4, 4>), blocks(64), dim3(256), 0, s, a);
     } else {
         hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 1>), blocks(128), dim3(256), 0, s, a);
     }
@@ -434,28 +369,30 @@ __device__ __forceinline__ void dma16(const void *base, uint32_t off, unsigned d
         : "memory");
 }
 
-// Large products: a 256 x 256 tile of S per workgroup, one wave per SIMD with 128 x 128 of it (4 x 4 accumulators of 32 x 32), K in
-// steps of 128 bytes through two LDS stages of 64 KB that LDS-DMA fills.  A step is four slices of 32 bytes: while a slice's
-// sixteen products run, the next slice's eight fragments are read; the barrier that hands over a stage stands in front of the last
-// slice's products, so that the next stage's first fragments arrive under them.  Chunk c of row r lies at slot c ^ (r / 2 % 8): any 16 rows' fragments cover the 64 banks.
-template <class TO>
-__global__ __launch_bounds__(256, 1) void score_i8_wide_kernel(const ScoreArgs a, int gx, int gy) {
-    constexpr int STAGE = 2 * 256 * 128;
+// Large products: a 64 W x 64 W tile of S per workgroup (W = 4, or 2 where that leaves CUs without one), one wave per SIMD with a quarter
+// of it (W x W accumulators of 32 x 32), K in steps of 128 bytes through two LDS stages that LDS-DMA fills.  A step is four slices of
+// 32 bytes: while a slice's W W products run, the next slice's 2 W fragments are read; the barrier that hands over a stage
+// stands in front of the last slice's products, so that the next stage's first fragments arrive under them and the old stage's
+// refill goes out between them.  Chunk c of row r lies at slot c ^ (r / 2 % 8): any 16 rows' fragments cover the 64 banks.
+template <class TO, int W>
+__global__ __launch_bounds__(256, W == 4 ? 1 : 2) void score_i8_tile_kernel(const ScoreArgs a, int gx, int gy) {
+    constexpr int SIDE = 64 * W, STAGE = 2 * SIDE * 128;
     __shared__ alignas(16) int8_t lds[2 * STAGE];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, h = lane >> 5;
     // workgroup i runs on XCD i % 8: give each XCD a run of tiles, four user tiles deep, so that its L2 sees few rows at a time
     const int total = gx * gy, q8 = total / 8, r8 = total % 8, xcd = blockIdx.x % 8;
     const int t = xcd * q8 + min(xcd, r8) + blockIdx.x / 8;
     const int group = t / (4 * gx), y0 = group * 4, deep = min(4, gy - y0), in = t - group * 4 * gx;
-    const int64_t b0 = (int64_t)(y0 + in % deep) * 256, j0 = (int64_t)(in / deep) * 256;
+    // (the quotients come out of vector registers: told to be the same in all lanes, the operands' bases below are scalar)
+    const int64_t b0 = (int64_t)__builtin_amdgcn_readfirstlane(y0 + in % deep) * SIDE, j0 = (int64_t)__builtin_amdgcn_readfirstlane(in / deep) * SIDE;
     const int steps = (a.kc + 7) / 8;
-    // this wave fills rows 64 w .. 64 w + 63 of both operands, eight rows per request
-    const int sc = (lane & 7) ^ (lane >> 4);  // its chunk in rows of an even q; ^ 4 in those of an odd one
+    // this wave fills rows 16 W w .. 16 W w + 16 W - 1 of both operands, eight rows per request
+    const int sc = (lane & 7) ^ (lane >> 4);  // its chunk in rows of an even request; ^ 4 in those of an odd one
     const int8_t *bu = a.qu + b0 * a.ldu, *bi = a.qi + j0 * a.ldi;
-    uint32_t ou[8], oi[8];
+    uint32_t ou[2 * W], oi[2 * W];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const int r = 64 * w + 8 * q + (lane >> 3);
+    for (int q = 0; q < 2 * W; ++q) {
+        const int r = 16 * W * w + 8 * q + (lane >> 3);
         ou[q] = (uint32_t)(min<int64_t>(r, a.B - 1 - b0) * a.ldu) + 16 * (sc ^ (q & 1) * 4);
         oi[q] = (uint32_t)(min<int64_t>(r, a.n - 1 - j0) * a.ldi) + 16 * (sc ^ (q & 1) * 4);
     }
@@ -463,45 +400,45 @@ __global__ __launch_bounds__(256, 1) void score_i8_wide_kernel(const ScoreArgs a
     // behind a row's end: the users' codes are zero there, the items' row ends at its last whole chunk
     const int last = a.kc - 1 - 8 * (steps - 1);
     const uint32_t back[2] = {16u * (uint32_t)max(0, sc - last), 16u * (uint32_t)max(0, (sc ^ 4) - last)};
-    auto fill = [&](int step, auto part) {  // a quarter of a stage: two requests for either operand
-        const unsigned to = lds0 + (step & 1) * STAGE + w * 8192;
-        const int8_t *pu = bu + (int64_t)step * 128, *pi = bi + (int64_t)step * 128;
+    auto fill = [&](int step, auto part) {  // a W-th of a stage: two requests for either operand
+        const unsigned to = lds0 + (step & 1) * STAGE + w * (W * 2048);
+        const uint32_t at = (uint32_t)step * 128;
         const bool end = step + 1 == steps;
         constexpr int q = 2 * decltype(part)::value;
-        dma16(pu, ou[q], to + q * 1024);
-        dma16(pu, ou[q + 1], to + q * 1024 + 1024);
-        dma16(pi, oi[q] - (end ? back[0] : 0u), to + STAGE / 2 + q * 1024);
-        dma16(pi, oi[q + 1] - (end ? back[1] : 0u), to + STAGE / 2 + q * 1024 + 1024);
+        dma16(bu, ou[q] + at, to + q * 1024);
+        dma16(bu, ou[q + 1] + at, to + q * 1024 + 1024);
+        dma16(bi, oi[q] + at - (end ? back[0] : 0u), to + STAGE / 2 + q * 1024);
+        dma16(bi, oi[q + 1] + at - (end ? back[1] : 0u), to + STAGE / 2 + q * 1024 + 1024);
     };
-    constexpr std::integral_constant<int, 0> p0;
-    constexpr std::integral_constant<int, 1> p1;
-    constexpr std::integral_constant<int, 2> p2;
-    constexpr std::integral_constant<int, 3> p3;
-    auto fill_all = [&](int step) { fill(step, p0), fill(step, p1), fill(step, p2), fill(step, p3); };
-    i32x16 acc[4][4] = {};
-    i32x4 f0[8], f1[8];
-    const int wu = (w >> 1) * 128, wi = (w & 1) * 128;
-    auto read = [&](i32x4(&to)[8], int step, int k) {
+    auto each = [](auto f) {
+        f(std::integral_constant<int, 0>{});
+        f(std::integral_constant<int, 1>{});
+        if constexpr (W == 4) f(std::integral_constant<int, 2>{}), f(std::integral_constant<int, 3>{});
+    };
+    i32x16 acc[W][W] = {};
+    i32x4 f0[2 * W], f1[2 * W];
+    const int wu = (w >> 1) * (32 * W), wi = (w & 1) * (32 * W);
+    auto read = [&](i32x4(&to)[2 * W], int step, int k) {
         const int8_t *from = lds + (step & 1) * STAGE + (((2 * k + h) ^ ((m >> 1) & 7)) * 16);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) to[x] = *reinterpret_cast<const i32x4 *>(from + (wu + 32 * x + m) * 128);
+        for (int x = 0; x < W; ++x) to[x] = *reinterpret_cast<const i32x4 *>(from + (wu + 32 * x + m) * 128);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) to[4 + y] = *reinterpret_cast<const i32x4 *>(from + STAGE / 2 + (wi + 32 * y + m) * 128);
+        for (int y = 0; y < W; ++y) to[W + y] = *reinterpret_cast<const i32x4 *>(from + STAGE / 2 + (wi + 32 * y + m) * 128);
     };
-    auto multiply = [&](const i32x4(&g)[8], auto part) {
+    auto multiply = [&](const i32x4(&g)[2 * W], auto part) {
         constexpr int x = decltype(part)::value;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(g[x], g[4 + y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < W; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(g[x], g[W + y], acc[x][y], 0, 0, 0);
     };
-    auto slice = [&](const i32x4(&g)[8], i32x4(&next)[8], int step, int k) {  // read (step, k) under the products of g
+    auto slice = [&](const i32x4(&g)[2 * W], i32x4(&next)[2 * W], int step, int k) {  // read (step, k) under the products of g
         read(next, step, k);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(g, p0), multiply(g, p1), multiply(g, p2), multiply(g, p3);
+        each([&](auto x) { multiply(g, x); });
         __builtin_amdgcn_sched_barrier(0);
     };
-    fill_all(0);
+    each([&](auto q) { fill(0, q); });
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (steps > 1) fill_all(1);
+    if (steps > 1) each([&](auto q) { fill(1, q); });
     read(f0, 0, 0);
     for (int st = 0; st < steps; ++st) {
         slice(f0, f1, st, 1);
@@ -513,64 +450,61 @@ __global__ __launch_bounds__(256, 1) void score_i8_wide_kernel(const ScoreArgs a
         read(f0, st + 1, 0);
         __builtin_amdgcn_sched_barrier(0);
         const bool more = st + 2 < steps;
-        multiply(f1, p0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) fill(st + 2, p0);
-        multiply(f1, p1);
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) fill(st + 2, p1);
-        multiply(f1, p2);
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) fill(st + 2, p2);
-        multiply(f1, p3);
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) fill(st + 2, p3);
+        each([&](auto x) {
+            multiply(f1, x);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) fill(st + 2, x);
+        });
     }
     __syncthreads();
     // the wave's tile through its quarter of the LDS, a strip of 32 users at a time, and out in rows
-    constexpr int E = 16 / (int)sizeof(TO), L = 128 / E;
+    constexpr int COLS = 32 * W, E = 16 / (int)sizeof(TO), L = COLS / E;
     TO *strip = reinterpret_cast<TO *>(lds + w * (STAGE / 2));
     TO *S = (TO *)a.S;
-    const bool wide = (reinterpret_cast<uintptr_t>(S) | (uintptr_t)(a.lds * (int64_t)sizeof(TO))) % 16 == 0;
-    float si[4];
+    const bool inside = j0 + SIDE <= a.n;  // (else the items end in this tile)
+    float si[W];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) si[y] = a.si[min<int64_t>(j0 + wi + 32 * y + m, a.n - 1)];
+    for (int y = 0; y < W; ++y) si[y] = a.si[min<int64_t>(j0 + wi + 32 * y + m, a.n - 1)];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < W; ++x) {
         const int64_t bx = b0 + wu + 32 * x;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = (r & 3) + 8 * (r >> 2) + 4 * h;
             const float su = a.su[min<int64_t>(bx + row, a.B - 1)];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) strip[row * 128 + 32 * y + m] = from_f32<TO>((float)acc[x][y][r] * su * si[y]);
+            for (int y = 0; y < W; ++y) strip[row * COLS + 32 * y + m] = from_f32<TO>((float)acc[x][y][r] * su * si[y]);
         }
-        if (wide) {
+        if (inside) {
 #pragma unroll
             for (int q = 0; q < 32 * L / 64; ++q) {
                 const int row = q * (64 / L) + lane / L, c = lane % L * E;
-                const int64_t j = j0 + wi + c;
-                if (bx + row < a.B) {
-                    TO *to = S + (bx + row) * a.lds + j;
-                    const TO *from = strip + row * 128 + c;
-                    if (j + E <= a.n) {
-                        *reinterpret_cast<i32x4 *>(to) = *reinterpret_cast<const i32x4 *>(from);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            if (j + e < a.n) to[e] = from[e];
-                    }
-                }
+                if (bx + row < a.B) store_any(S + (bx + row) * a.lds + j0 + wi + c, *reinterpret_cast<const Vec<TO, E> *>(strip + row * COLS + c));
             }
         } else {
 #pragma unroll 4
-            for (int q = 0; q < 64; ++q) {
-                const int row = q >> 1, c = (q & 1) * 64 + lane;
-                const int64_t j = j0 + wi + c;
-                if (bx + row < a.B && j < a.n) S[(bx + row) * a.lds + j] = strip[row * 128 + c];
+            for (int q = 0; q < 32 * COLS / 64; ++q) {
+                const int row = q / (COLS / 64), c = q % (COLS / 64) * 64 + lane;
+                if (bx + row < a.B && j0 + wi + c < a.n) S[(bx + row) * a.lds + j0 + wi + c] = strip[row * COLS + c];
             }
         }
     }
+}
+
+template <class TO, int W>
+static int launch_tiles(const ScoreArgs &a, hipStream_t s) {
+    constexpr int64_t SIDE = 64 * W;
+    const int64_t gx = (a.n + SIDE - 1) / SIDE, all = (a.B + SIDE - 1) / SIDE, most = std::max<int64_t>(1, ((int64_t)1 << 29) / gx);
+    for (int64_t y0 = 0; y0 < all; y0 += most) {  // (tiles are numbered in 32 bits)
+        ScoreArgs p = a;
+        p.qu += y0 * SIDE * a.ldu, p.su += y0 * SIDE, p.B -= y0 * SIDE;
+        p.S = (TO *)a.S + y0 * SIDE * a.lds;
+        const int64_t gy = std::min(most, all - y0);
+        p.B = std::min(p.B, gy * SIDE);
+        hipLaunchKernelGGL((score_i8_tile_kernel<TO, W>), dim3((unsigned)(gx * gy)), dim3(256), 0, s, p, (int)gx, (int)gy);
+    }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
 }
 
 template <class TO>
@@ -578,29 +512,19 @@ static int launch_score(const ScoreArgs &a, hipStream_t s) {
     if (a.B <= 16) return launch_few<TO, void, 1>(a, s);
     if (a.kc <= 4) return launch_short<TO, 2>(a, s);
     if (a.kc <= 8) return launch_short<TO, 4>(a, s);
-    if (a.B <= 32) return launch_few<TO, void, 2>(a, s);
-    if (a.B <= 64) return launch_few<TO, void, 4>(a, s);
+    if (a.kc <= 16 && a.B * a.n * (int64_t)sizeof(TO) >= 128 << 20) return launch_short<TO, 8>(a, s);  // (4096 x 40 001 x 256: 197 us, 237 in tiles; 100 x 100 001 x 200: 40 and 22)
     const int64_t wide = ((a.n + 255) / 256) * ((a.B + 255) / 256), small = ((a.n + 127) / 128) * ((a.B + 127) / 128);
-    if (small < 128 && a.kc > 16) return launch_few<TO, void, 4>(a, s);  // (64 x 16 tiles, K over four waves: many times the workgroups)
-    // Rounds of 256 x 256 tiles (one per CU) against 128 x 128 ones, whose products cost 1.37 times as much (690 and 505 us at 4096 x
-    // 16 384 x 8192) but which waste less of the last round and of the edges.  (32-bit offsets inside a wide tile.)
-    if ((wide + 255) / 256 * 4 <= 1.37 * small / 256 && wide < (1 << 30) && a.ldu <= 1 << 23 && a.ldi <= 1 << 23) {
-        hipLaunchKernelGGL((score_i8_wide_kernel<TO>), dim3((unsigned)wide), dim3(256), 0, s, a, (int)((a.n + 255) / 256), (int)((a.B + 255) / 256));
-        RBG_HIP(hipGetLastError());
-        return RBG_OK;
-    }
-    const int64_t gy = (a.B + 127) / 128;
-    for (int64_t y0 = 0; y0 < gy; y0 += 65535) {  // (a grid's y dimension ends at 65 535)
-        ScoreArgs p = a;
-        p.qu += y0 * 128 * a.ldu, p.su += y0 * 128, p.B -= y0 * 128;
-        p.S = (TO *)a.S + y0 * 128 * a.lds;
-        const unsigned rows = (unsigned)std::min<int64_t>(65535, gy - y0);
-        hipLaunchKernelGGL((score_i8_kernel<TO>), dim3((unsigned)((a.n + 127) / 128), rows), dim3(256), 0, s, p);
-    }
-    RBG_HIP(hipGetLastError());
-    return RBG_OK;
+    // 64 x 16 tiles with K over four waves, many times the workgroups (300 x 300 x 8 192: 31 us against 51; 1 000 x 1 000 x 1 024: 19 against 16)
+    if (small <= 32 && a.kc >= 128) return launch_few<TO, void, 4>(a, s);
+    // Rounds of 256 x 256 tiles (one per CU) against 128 x 128 ones, whose products cost about 1.37 times as much but which waste less of the
+    // last round and of the edges.
+    return (wide + 255) / 256 * 4 <= 1.37 * small / 256 ? launch_tiles<TO, 4>(a, s) : launch_tiles<TO, 2>(a, s);
 }
 
+// Bytes between the rows of codes that a call makes for itself.
+static int64_t own_stride(int64_t K) { return (K + 127) / 128 * 128; }
+
+constexpr int64_t kMaxStride = 1 << 23;  // 32-bit offsets inside a tile
 constexpr int64_t kMaxK = 131071;  // 128 x 128 x K < 2^31
 
 // What both product entries ask of the items and the scores.
@@ -611,6 +535,7 @@ static int check_score(int64_t B, const int8_t *qi, int64_t ldi, const float *si
     if (ldi % 16) return fail(RBG_EINVAL, "ldi = %lld is not a multiple of 16", (long long)ldi);
     if (K > kMaxK) return fail(RBG_EUNSUPPORTED, "K = %lld: sums of more than 131071 products may pass 32 bits", (long long)K);
     if (n > 0x7fffffffll || B > 0x7fffffffll) return fail(RBG_EUNSUPPORTED, "rows beyond 2^31");
+    if (ldi > kMaxStride) return fail(RBG_EUNSUPPORTED, "ldi = %lld: at most 2^23 bytes between rows of codes", (long long)ldi);
     if (B && n && (!qi || !si || !S)) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(qi) || reinterpret_cast<uintptr_t>(S) % elem_size(out_dtype)) return fail(RBG_EINVAL, "codes need 16-byte alignment, scores that of their type");
     return RBG_OK;
@@ -643,6 +568,7 @@ int rbg_score_i8(const int8_t *qu, int64_t ldu, const float *su, int64_t B, cons
     if (int rc = check_score(B, qi, ldi, si, n, K, S, lds, out_dtype)) return rc;
     if (ldu < K) return fail(RBG_ESHAPE, "K = %lld, ldu = %lld", (long long)K, (long long)ldu);
     if (ldu % 128) return fail(RBG_EINVAL, "ldu = %lld is not a multiple of 128", (long long)ldu);
+    if (ldu > kMaxStride) return fail(RBG_EUNSUPPORTED, "ldu = %lld: at most 2^23 bytes between rows of codes", (long long)ldu);
     if (B == 0 || n == 0) return RBG_OK;
     if (!qu || !su) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(qu)) return fail(RBG_EINVAL, "codes need 16-byte alignment");
@@ -654,7 +580,7 @@ int rbg_score_rows_i8_workspace(int64_t B, int64_t K, int64_t *bytes) {
     clear_error();
     if (!bytes) return fail(RBG_EINVAL, "bytes is NULL");
     if (B < 0 || K <= 0) return fail(RBG_ESHAPE, "B = %lld, K = %lld", (long long)B, (long long)K);
-    const int64_t ldc = (K + 127) / 128 * 128;
+    const int64_t ldc = own_stride(K);
     *bytes = B * ldc + (4 * B + 15) / 16 * 16;
     return RBG_OK;
 }
@@ -668,7 +594,7 @@ int rbg_score_rows_i8(const void *u, int64_t ldu, int dtype, int64_t B, const in
     if (B == 0 || n == 0) return RBG_OK;
     if (!u || !workspace) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(workspace) || reinterpret_cast<uintptr_t>(u) % elem_size(dtype)) return fail(RBG_EINVAL, "workspace is not 16-byte aligned, or rows not to their type");
-    const int64_t ldc = (K + 127) / 128 * 128;
+    const int64_t ldc = own_stride(K);
     int8_t *qu = (int8_t *)workspace;
     float *su = (float *)(qu + B * ldc);
     if (B <= 16 && B * K <= kOwnCodes) {

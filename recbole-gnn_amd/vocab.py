@@ -338,7 +338,7 @@ def _codes(codes, k):
     if (k == 1 or codes.stride(1) == 1) and codes.data_ptr() % 16 == 0:
         ld = codes.stride(0) if n > 1 else need
         room = codes.untyped_storage().nbytes() - codes.storage_offset()
-        if ld % 16 == 0 and ld >= need and (n - 1) * ld + need <= room:
+        if ld % 16 == 0 and need <= ld <= 1 << 23 and (n - 1) * ld + need <= room:
             return codes, ld
     padded = codes.new_zeros((n, need))
     padded[:, :k] = codes

@@ -518,7 +518,7 @@ def test_score_int8(rbg, cuda, b, n, k, dtype, out_dtype):
 
 
 @pytest.mark.parametrize("b,n,k,out_dtype", [(3500, 3600, 129, F32), (4096, 4096, 1024, BF16), (2050, 8003, 300, F32), (1025, 10241, 257, F16), (256, 49153, 2048, BF16),
-                                             (70, 49000, 64, F32), (2048, 40982, 64, F32), (333, 9001, 100, BF16), (40, 70003, 33, F16)])
+                                             (70, 49000, 64, F32), (1100, 40001, 250, F32), (2000, 40003, 129, BF16), (100, 1000, 2050, F32), (900, 1100, 1030, BF16), (2048, 40982, 64, F32), (333, 9001, 100, BF16), (40, 70003, 33, F16)])
 def test_score_int8_many(rbg, cuda, b, n, k, out_dtype):
     """Sizes that fill the chip with large tiles or with long walks; every score against the same in 64 bits (here on the GPU), and nothing
     written outside the scores."""

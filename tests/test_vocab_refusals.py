@@ -59,7 +59,7 @@ REFUSED = [
     (preference, dict(ref=None), EINVAL), (preference, dict(grad=None), EINVAL), (preference, dict(grad=P((1 << 20) - 32)), EINVAL),
     (quantize, dict(ldc=24), EINVAL), (quantize, dict(ldc=0), ESHAPE), (quantize, dict(codes=P(8)), EINVAL), (quantize, dict(k=0), ESHAPE),
     (quantize, dict(x=P(2)), EINVAL), (quantize, dict(scale=None), EINVAL),
-    (score, dict(ldu=64), EINVAL), (score, dict(ldi=24), EINVAL), (score, dict(k=131072, ldu=131072, ldi=131072), EUNSUPPORTED), (score, dict(lds=2), ESHAPE),
+    (score, dict(ldu=64), EINVAL), (score, dict(ldi=24), EINVAL), (score, dict(k=131072, ldu=131072, ldi=131072), EUNSUPPORTED), (score, dict(lds=2), ESHAPE), (score, dict(ldi=(1 << 23) + 16), EUNSUPPORTED), (score, dict(ldu=(1 << 23) + 128), EUNSUPPORTED),
     (score, dict(qi=P(8)), EINVAL), (score, dict(out=3), EINVAL), (score, dict(k=0), ESHAPE), (score, dict(su=None), EINVAL),
     (score_rows, dict(dtype=3), EINVAL), (score_rows, dict(out=-1), EINVAL), (score_rows, dict(ldu=7), ESHAPE), (score_rows, dict(work=None), EINVAL),
     (score_rows, dict(work=P(8)), EINVAL), (score_rows, dict(u=P(2)), EINVAL), (score_rows, dict(k=131072, ldu=131072, ldi=131072), EUNSUPPORTED),
