@@ -488,20 +488,20 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     if (!first && sub == 0 && blockIdx.y == 0) a.list[atomicAdd(a.count, 1u)] = (uint32_t)c;  // (the list's order changes no sum)
 }
 
-// Few places (n <= kFewPlaces): one launch, no sorted list.  A workgroup owns 256 rows (and a piece of their columns), finds the places that
+// Few places (n <= kFewPlaces): one launch, no sorted list.  A workgroup owns `stripe` rows (and a piece of their columns), finds the places that
 // refer to them, ranks those by (row, place) by counting, and sums a run per lane-group; its other rows are zeroed.
 constexpr int kFewPlaces = 256;
 
 template <class TI, class TO, int VEC, int G>
-__global__ __launch_bounds__(256) void few_places_kernel(const RunArgs a, const int64_t *__restrict__ ids, int64_t padding) {
-    constexpr int U = 8;  // rows in flight per lane-group
+__global__ __launch_bounds__(256) void few_places_kernel(const RunArgs a, const int64_t *__restrict__ ids, int64_t padding, int stripe) {
+    constexpr int U = 16;  // rows in flight per lane-group (a row that all places refer to is one group's: 256 of them in 16 turns)
     __shared__ __align__(16) uint32_t row_of[kFewPlaces];  // of a place, from the workgroup's first row; 256: another's
     __shared__ uint32_t run_of[kFewPlaces + 1], place_of[kFewPlaces];
     __shared__ uint32_t used[256];
     __shared__ uint32_t found;
     const int n = (int)a.n, i = threadIdx.x;
-    const int64_t r0 = (int64_t)blockIdx.x * 256;
-    const int rows = (int)min<int64_t>(256, a.n_rows - r0);
+    const int64_t r0 = (int64_t)blockIdx.x * stripe;
+    const int rows = (int)min<int64_t>(stripe, a.n_rows - r0);
     uint32_t mine = 256;
     if (i < n) {
         const int64_t id = ids[i];
@@ -642,8 +642,10 @@ template <class TI, class TO, int VEC, int G>
 static void launch_runs(const RunArgs &a0, const int64_t *ids, int64_t padding, hipStream_t s) {
     RunArgs a = a0;
     if (a.n <= kFewPlaces) {
-        hipLaunchKernelGGL((few_places_kernel<TI, TO, VEC, G>), dim3((unsigned)((a.n_rows + 255) / 256), (unsigned)((a.d + G * VEC - 1) / (G * VEC))), dim3(256),
-                           0, s, a, ids, padding);
+        int stripe = 256;  // fewer rows where there are few, for more workgroups
+        while (stripe > 8 && a.n_rows < stripe * 256) stripe /= 2;
+        hipLaunchKernelGGL((few_places_kernel<TI, TO, VEC, G>), dim3((unsigned)((a.n_rows + stripe - 1) / stripe), (unsigned)((a.d + G * VEC - 1) / (G * VEC))),
+                           dim3(256), 0, s, a, ids, padding, stripe);
         return;
     }
     a.run_blocks = (a.chunks + 256 / G - 1) / (256 / G);
@@ -690,6 +692,7 @@ int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dty
     if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
     if (n < 0 || n_rows < 0 || d <= 0 || ldt < d || ldo < d)
         return fail(RBG_ESHAPE, "n = %lld, n_rows = %lld, d = %d, ldt = %lld, ldo = %lld", (long long)n, (long long)n_rows, d, (long long)ldt, (long long)ldo);
+    if (n > (int64_t)1 << 34) return fail(RBG_EUNSUPPORTED, "n = %lld: at most 2^34 ids", (long long)n);
     if (n == 0) return RBG_OK;
     if ((n_rows && !table) || !ids || !out) return fail(RBG_EINVAL, "NULL pointer");
     const int size = elem_size(dtype);

@@ -45,7 +45,7 @@ def score_rows(lib, u=A, ldu=8, dtype=0, b=2, qi=C, ldi=16, si=B, n=3, k=8, s=D,
 
 REFUSED = [
     (embedding, dict(dtype=3), EINVAL), (embedding, dict(d=0), ESHAPE), (embedding, dict(ldt=7), ESHAPE), (embedding, dict(ldo=7), ESHAPE),
-    (embedding, dict(n=-1), ESHAPE), (embedding, dict(ids=None), EINVAL), (embedding, dict(table=None), EINVAL), (embedding, dict(out=P(2)), EINVAL),
+    (embedding, dict(n=-1), ESHAPE), (embedding, dict(ids=None), EINVAL), (embedding, dict(table=None), EINVAL), (embedding, dict(out=P(2)), EINVAL), (embedding, dict(n=(1 << 34) + 1), EUNSUPPORTED),
     (embedding_grad, dict(out_dtype=2), EINVAL), (embedding_grad, dict(ldg=7), ESHAPE), (embedding_grad, dict(rows=0x7fffffff), EUNSUPPORTED),
     (embedding_grad, dict(n=0x7fff0000), EUNSUPPORTED), (embedding_grad, dict(d=(1 << 20) + 1, ldg=1 << 21), EUNSUPPORTED), (embedding_grad, dict(work=P(8)), EINVAL),
     (embedding_grad, dict(work=None, n=1000), EINVAL), (embedding_grad, dict(grad=P(1)), EINVAL),
