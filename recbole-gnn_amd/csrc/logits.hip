@@ -315,7 +315,7 @@ __device__ __forceinline__ void fix_entries(const DistillArgs &a, T *g, const Ro
     }
 }
 
-// The loss alone: one workgroup streams a row.
+// The loss alone: one workgroup streams a row.  Bound by the reads: 4 096 x 91 600 fp32, 1.5 GB in 253 us = 5.9 TB/s.
 template <class T, int TH>
 __global__ __launch_bounds__(TH) void distill_eval_kernel(const DistillArgs a) {
     __shared__ Entries sh;
@@ -343,7 +343,8 @@ __device__ __forceinline__ Vec<T, E> as_elems(const u32x4 &v) {
 
 // Value and gradient of a row that fits the registers of its workgroup: NC chunks of 16 bytes per thread.  The teacher's entries are set
 // right behind the row's stores and a barrier.  (Finding each thread's entries on a list in LDS before its stores instead: 82 us
-// against 74 at 2048 x 40 982 bf16 — the lists' making delays every store of the row, the second look only its last ones.)
+// against 74 at 2048 x 40 982 bf16 — the lists' making delays every store of the row, the second look only its last ones.)  Bound by
+// memory: at that size 336 MB in 60 us = 5.6 TB/s behind another call of itself, 73 us with other work between.
 template <class T, int TH, int NC>
 __global__ __launch_bounds__(TH, NC <= 12 ? 5 : 4) void distill_row_kernel(const DistillArgs a) {
     constexpr int E = RowShape<T>::E;
@@ -509,7 +510,8 @@ __device__ __forceinline__ void store_logp(const LogpArgs &a, int64_t row, bool 
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// One workgroup per row and part; a row without a target is not read.
+// One workgroup per row and part; a row without a target is not read.  Bound by the reads: 252 MB (4 096 x 40 982 bf16, a quarter
+// without a target) in 43 us = 5.9 TB/s, 1.18 GB (6 001 x 131 072 fp16) in 196 = 6.0.
 template <class T, int TH, bool PARTS>
 __global__ __launch_bounds__(TH) void logp_kernel(const LogpArgs a) {
     __shared__ MaxSum red[TH / kWave];
@@ -565,7 +567,9 @@ __device__ __forceinline__ void clear_row(const void *zv, int64_t ldz, int V, in
     zero_row<T, TH>((T *)gv + row * ldg, rs, 0, rs.nb, true);
 }
 
-// One workgroup per row and part; row = the last one first: what the pass before read last is what the caches still hold.
+// One workgroup per row and part; row = the last one first: what the pass before read last is what the caches still hold.  Bound by
+// memory: at the sizes above 252 MB read and 336 MB written in 84 us = 7.0 TB/s, much of the reads out of the caches, and 1.18 + 1.57 GB
+// in 485 = 5.7.
 template <class T, int TH>
 __global__ __launch_bounds__(TH) void logp_grad_kernel(const void *z, int64_t ldz, int V, const int64_t *targets, const float *stats,
                                                        const float *row_g, void *g, int64_t ldg) {
@@ -593,7 +597,8 @@ __device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_
     hi = hi < lo ? lo : hi > m ? m : hi;
 }
 
-// One workgroup per pair: both sums in 64 bits, the loss, and (COEF) the tokens' gradients of pair_w loss.
+// One workgroup per pair: both sums in 64 bits, the loss, and (COEF) the tokens' gradients of pair_w loss.  Bound by latency (4 096
+// tokens of 32 pairs 5 us, 6 001 of two 10).
 template <class L, bool COEF>
 __global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, const int64_t *offsets, const float *ref, float beta,
                                                    float smoothing, const float *pair_w, float *loss, float *margin, float *coef) {
@@ -623,7 +628,8 @@ __global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, con
 }
 
 // Small calls in one launch: a workgroup per pair, a wave per row.  Both sums meet in LDS, and the rows, read a second time for their
-// gradient, are still in the caches.  (m, S) of a row stays with the wave that goes on to write it.
+// gradient, are still in the caches.  (m, S) of a row stays with the wave that goes on to write it.  Bound by that chain of latencies: 40
+// tokens of 1 683 fp32 logits in 10.7 us.
 template <class T>
 __global__ __launch_bounds__(1024) void pair_small_kernel(const LogpArgs a, int64_t m, const int64_t *offsets, const float *ref, float beta,
                                                           float smoothing, const float *pair_w, float *loss, float *margin, void *gv, int64_t ldg) {
