@@ -268,7 +268,8 @@ __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
     __shared__ alignas(16) int8_t own[OWN ? kOwnCodes + 16 * 80 : 16];
     __shared__ float own_su[16];
     const int pitch = (a.kc + 3) / 4 * 64 + 16;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    // (w as a scalar: it decides how many steps there are, and a matrix instruction that a mask of lanes alone guards runs all the same)
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
     const int64_t j0 = ((int64_t)blockIdx.x * (4 / KW) + w / KW) * (16 * IT), b0 = (int64_t)blockIdx.y * (16 * UT);
     const i32x4 *pu[UT], *pi[IT];
 #pragma unroll

@@ -723,3 +723,20 @@ def test_wrappers_refuse(rbg, cuda):
         (g,) = torch.autograd.grad(rbg.token_logp(leaf, torch.zeros(3, dtype=torch.int64, device=cuda)).sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError):
             g.sum().backward()
+
+
+@pytest.mark.parametrize("b,n", [(1, 500), (3, 33000), (16, 66000), (40, 200), (64, 2000)])
+def test_scores_of_every_length(rbg, cuda, b, n):
+    """Lengths that leave the waves that share a row every remainder of steps, at the sizes where 1, 2 and 4 groups of items go to a wave."""
+    few = min(n, 500)
+    at = torch.arange(n, device=cuda) % few
+    for k in (1, 63, 64, 65, 200, 257, 1000, 1023, 1025, 1100, 1281, 1500, 1537, 1800, 2049, 2200, 2310, 2600, 3200, 4100, 4200, 5000, 8193):
+        g = gen(b + k, cuda)
+        u = torch.randn(b, k, generator=g, device=cuda)
+        codes, scales = rbg.quantize_rows(torch.randn(few, k, generator=g, device=cuda))
+        wide = torch.full((n, codes.stride(0)), 5, dtype=torch.int8, device=cuda)  # (what stands behind a row's end is read and not used)
+        wide[:, :k] = codes[at]
+        qu, su = rbg.quantize_rows(u)
+        sums = qu.double() @ codes.double().t().contiguous()
+        ref = sums.float() * su[:, None] * scales  # exact sums, then the two products in the order the operator takes them
+        assert torch.equal(rbg.score_int8(u, wide[:, :k], scales[at]), ref[:, at]), (b, n, k)
