@@ -698,6 +698,7 @@ int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dty
     if (n < 0 || n_rows < 0 || d <= 0 || ldt < d || ldo < d)
         return fail(RBG_ESHAPE, "n = %lld, n_rows = %lld, d = %d, ldt = %lld, ldo = %lld", (long long)n, (long long)n_rows, d, (long long)ldt, (long long)ldo);
     if (n > (int64_t)1 << 34) return fail(RBG_EUNSUPPORTED, "n = %lld: at most 2^34 ids", (long long)n);
+    constexpr int64_t kIdsPerLaunch = 1 << 26;  // (a grid holds fewer than 2^32 threads per dimension, a workgroup of 256 at least 16 ids)
     if (n == 0) return RBG_OK;
     if ((n_rows && !table) || !ids || !out) return fail(RBG_EINVAL, "NULL pointer");
     const int size = elem_size(dtype);
@@ -708,8 +709,11 @@ int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dty
         constexpr int VEC = 16 / (int)sizeof(E);
         auto go = [&](auto kernel, int G) {
             const int64_t per = 256 / G * 4;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids, n, d, scale,
-                               (E *)out, ldo);
+            for (int64_t i0 = 0; i0 < n; i0 += kIdsPerLaunch) {
+                const int64_t cnt = std::min(kIdsPerLaunch, n - i0);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)((cnt + per - 1) / per)), dim3(256), 0, (hipStream_t)stream, (const E *)table, ldt, n_rows, ids + i0,
+                                   cnt, d, scale, (E *)out + i0 * ldo, ldo);
+            }
         };
         const int lanes = wide ? (d + VEC - 1) / VEC : d;
         if (wide) {

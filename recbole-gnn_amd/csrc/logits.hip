@@ -734,7 +734,7 @@ static int check_grad(const void *z, int64_t ldz, int dtype, int64_t n, int64_t 
 }
 
 template <class T>
-static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, hipStream_t s) {
+static int launch_distill_rows(const DistillArgs &a, int64_t n, int64_t V, hipStream_t s) {
     const int S = row_parts(n, V);
     if (S > 1) {
         hipLaunchKernelGGL((distill_part_kernel<T, 256>), dim3(S, (unsigned)n), dim3(256), 0, s, a);
@@ -760,7 +760,20 @@ static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, hipStream_
 }
 
 template <class T>
-static int launch_logp(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
+static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, hipStream_t s) {
+    for (int64_t r0 = 0; r0 < n; r0 += kRowsPerLaunch) {
+        DistillArgs p = a;
+        p.z = (const T *)a.z + r0 * a.ldz, p.idx += r0 * a.k, p.val += r0 * a.k, p.loss += r0;
+        if (a.row_w) p.row_w += r0;
+        if (a.stats) p.stats += 2 * r0;
+        if (a.grad) p.grad = (T *)a.grad + r0 * a.ldg;
+        if (int rc = launch_distill_rows<T>(p, std::min(kRowsPerLaunch, n - r0), V, s)) return rc;
+    }
+    return RBG_OK;
+}
+
+template <class T>
+static int launch_logp_rows(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
     const int S = row_parts(m, V);
     if (S > 1) {
         hipLaunchKernelGGL((logp_kernel<T, 256, true>), dim3(S, (unsigned)m), dim3(256), 0, s, a);
@@ -770,6 +783,30 @@ static int launch_logp(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
     } else {
         hipLaunchKernelGGL((logp_kernel<T, 256, false>), dim3((unsigned)m), dim3(256), 0, s, a);
     }
+    RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+template <class T>
+static int launch_logp(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
+    for (int64_t r0 = 0; r0 < m; r0 += kRowsPerLaunch) {
+        LogpArgs p = a;
+        p.z = (const T *)a.z + r0 * a.ldz, p.targets += r0;
+        if (a.logp) p.logp += r0;
+        if (a.logp64) p.logp64 += r0;
+        if (a.coef) p.coef += r0;
+        if (a.stats) p.stats += 2 * r0;
+        if (int rc = launch_logp_rows<T>(p, std::min(kRowsPerLaunch, m - r0), V, s)) return rc;
+    }
+    return RBG_OK;
+}
+
+template <class L, bool COEF>
+static int launch_pairs(const L *logp, int64_t m, const int64_t *offsets, int64_t pairs, const float *ref, float beta, float smoothing,
+                        const float *pair_w, float *loss, float *margin, float *coef, hipStream_t s) {
+    for (int64_t i0 = 0; i0 < pairs; i0 += kRowsPerLaunch)
+        hipLaunchKernelGGL((pair_kernel<L, COEF>), dim3((unsigned)std::min(kRowsPerLaunch, pairs - i0)), dim3(256), 0, s, logp, m, offsets + 2 * i0,
+                           ref + 2 * i0, beta, smoothing, pair_w ? pair_w + i0 : nullptr, loss + i0, margin + i0, coef);
     RBG_HIP(hipGetLastError());
     return RBG_OK;
 }
@@ -897,10 +934,7 @@ int rbg_preference_loss(const float *logp, int64_t m, const int64_t *offsets, in
     if (int rc = check_pairs(m, offsets, pairs, beta, smoothing)) return rc;
     if (pairs == 0) return RBG_OK;
     if ((m && !logp) || !ref || !loss || !margin) return fail(RBG_EINVAL, "NULL pointer");
-    hipLaunchKernelGGL((pair_kernel<float, false>), dim3((unsigned)pairs), dim3(256), 0, (hipStream_t)stream, logp, m, offsets, ref, beta,
-                       smoothing, (const float *)nullptr, loss, margin, (float *)nullptr);
-    RBG_HIP(hipGetLastError());
-    return RBG_OK;
+    return launch_pairs<float, false>(logp, m, offsets, pairs, ref, beta, smoothing, nullptr, loss, margin, nullptr, (hipStream_t)stream);
 }
 
 int rbg_preference_loss_backward(const float *margin, int64_t m, const int64_t *offsets, int64_t pairs, float beta, float smoothing,
@@ -945,7 +979,7 @@ int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_
         // device: all tokens in one pair cost 16 turns of it at most (4 756 tokens of two pairs would take 560 us), and a wave
         // reads a row of 16 KB in four turns (one of 500 KB would take 80 us).
         const int64_t total = m * V * (int64_t)sizeof(E);
-        if (m && m <= 256 && m <= pairs * 64 && V * (int64_t)sizeof(E) <= 16 << 10 && total <= 1 << 20 && total <= pairs << 17) {
+        if (m && m <= 256 && m <= pairs * 64 && pairs <= kRowsPerLaunch && V * (int64_t)sizeof(E) <= 16 << 10 && total <= 1 << 20 && total <= pairs << 17) {
             const LogpArgs a{z, ldz, (int)V, targets, nullptr, nullptr, nullptr, stats, nullptr};
             hipLaunchKernelGGL((pair_small_kernel<E>), dim3((unsigned)pairs), dim3(1024), 0, s, a, m, offsets, ref, beta, smoothing, pair_w, loss, margin,
                                grad, ldg);
@@ -956,11 +990,7 @@ int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_
             const LogpArgs a{z, ldz, (int)V, targets, nullptr, logp, coef, stats, part};
             if (int rc = launch_logp<E>(a, m, V, s)) return rc;
         }
-        if (pairs) {
-            hipLaunchKernelGGL((pair_kernel<double, true>), dim3((unsigned)pairs), dim3(256), 0, s, logp, m, offsets, ref, beta, smoothing,
-                               pair_w, loss, margin, coef);
-            RBG_HIP(hipGetLastError());
-        }
+        if (int rc = launch_pairs<double, true>(logp, m, offsets, pairs, ref, beta, smoothing, pair_w, loss, margin, coef, s)) return rc;
         return m ? launch_logp_grad<E>((const E *)z, ldz, m, V, targets, stats, coef, (E *)grad, ldg, s) : (int)RBG_OK;
     });
 }

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void quantize_long_kernel(const T *__restrict_
 }
 
 template <class T>
-static int launch_quantize(const T *x, int64_t ldx, int64_t n, int64_t K, int8_t *codes, int64_t ldc, float *scale, hipStream_t s) {
+static int launch_quantize_rows(const T *x, int64_t ldx, int64_t n, int64_t K, int8_t *codes, int64_t ldc, float *scale, hipStream_t s) {
     constexpr int E = 16 / (int)sizeof(T);
     auto blocks = [&](int per) { return dim3((unsigned)((n + per - 1) / per)); };
     if (ldc <= 32 * E) hipLaunchKernelGGL((quantize_kernel<T, 32, 1>), blocks(8), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
@@ -125,6 +125,13 @@ static int launch_quantize(const T *x, int64_t ldx, int64_t n, int64_t K, int8_t
     else if (ldc <= 4096 * E) hipLaunchKernelGGL((quantize_kernel<T, 256, 16>), blocks(1), dim3(256), 0, s, x, ldx, n, (int)K, codes, (int)ldc, scale);
     else hipLaunchKernelGGL((quantize_long_kernel<T>), blocks(1), dim3(256), 0, s, x, ldx, K, codes, ldc, scale);
     RBG_HIP(hipGetLastError());
+    return RBG_OK;
+}
+
+template <class T>
+static int launch_quantize(const T *x, int64_t ldx, int64_t n, int64_t K, int8_t *codes, int64_t ldc, float *scale, hipStream_t s) {
+    for (int64_t r0 = 0; r0 < n; r0 += kRowsPerLaunch)
+        if (int rc = launch_quantize_rows<T>(x + r0 * ldx, ldx, std::min(kRowsPerLaunch, n - r0), K, codes + r0 * ldc, ldc, scale + r0, s)) return rc;
     return RBG_OK;
 }
 
@@ -500,8 +507,8 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void score_i8_tile_kernel(cons
 template <class TO, int W>
 static int launch_tiles(const ScoreArgs &a, hipStream_t s) {
     constexpr int64_t SIDE = 64 * W;
-    const int64_t gx = (a.n + SIDE - 1) / SIDE, all = (a.B + SIDE - 1) / SIDE, most = std::max<int64_t>(1, ((int64_t)1 << 29) / gx);
-    for (int64_t y0 = 0; y0 < all; y0 += most) {  // (tiles are numbered in 32 bits)
+    const int64_t gx = (a.n + SIDE - 1) / SIDE, all = (a.B + SIDE - 1) / SIDE, most = std::max<int64_t>(1, ((int64_t)1 << 23) / gx);
+    for (int64_t y0 = 0; y0 < all; y0 += most) {  // (a grid holds fewer than 2^32 threads)
         ScoreArgs p = a;
         p.qu += y0 * SIDE * a.ldu, p.su += y0 * SIDE, p.B -= y0 * SIDE;
         p.S = (TO *)a.S + y0 * SIDE * a.lds;
@@ -513,8 +520,10 @@ static int launch_tiles(const ScoreArgs &a, hipStream_t s) {
     return RBG_OK;
 }
 
-template <class TO>
-static int launch_score(const ScoreArgs &a, hipStream_t s) {
+// TU: as in score_i8_few_kernel.
+template <class TO, class TU>
+static int launch_score_items(const ScoreArgs &a, hipStream_t s) {
+    if constexpr (!std::is_void_v<TU>) return launch_few<TO, TU, 1>(a, s);
     if (a.B <= 16) return launch_few<TO, void, 1>(a, s);
     if (a.kc <= 4) return launch_short<TO, 2>(a, s);
     if (a.kc <= 8) return launch_short<TO, 4>(a, s);
@@ -525,6 +534,17 @@ static int launch_score(const ScoreArgs &a, hipStream_t s) {
     // Rounds of 256 x 256 tiles (one per CU) against 128 x 128 ones, whose products cost about 1.37 times as much but which waste less of the
     // last round and of the edges.
     return (wide + 255) / 256 * 4 <= 1.37 * small / 256 ? launch_tiles<TO, 4>(a, s) : launch_tiles<TO, 2>(a, s);
+}
+
+template <class TO, class TU>
+static int launch_score(const ScoreArgs &a, hipStream_t s) {
+    constexpr int64_t kItemsPerLaunch = 1 << 24;  // (a grid holds fewer than 2^32 threads per dimension)
+    for (int64_t j0 = 0; j0 < a.n; j0 += kItemsPerLaunch) {
+        ScoreArgs p = a;
+        p.qi += j0 * a.ldi, p.si += j0, p.S = (TO *)a.S + j0, p.n = std::min(kItemsPerLaunch, a.n - j0);
+        if (int rc = launch_score_items<TO, TU>(p, s)) return rc;
+    }
+    return RBG_OK;
 }
 
 // Bytes between the rows of codes that a call makes for itself.
@@ -579,7 +599,7 @@ int rbg_score_i8(const int8_t *qu, int64_t ldu, const float *su, int64_t B, cons
     if (!qu || !su) return fail(RBG_EINVAL, "NULL pointer");
     if (!on_16(qu)) return fail(RBG_EINVAL, "codes need 16-byte alignment");
     const ScoreArgs a{qu, qi, ldu, ldi, su, si, B, n, (int)((K + 15) / 16), S, lds, nullptr, (int)K};
-    return with_elem(out_dtype, [&](auto t) { return launch_score<decltype(t)>(a, (hipStream_t)stream); });
+    return with_elem(out_dtype, [&](auto t) { return launch_score<decltype(t), void>(a, (hipStream_t)stream); });
 }
 
 int rbg_score_rows_i8_workspace(int64_t B, int64_t K, int64_t *bytes) {
@@ -606,7 +626,7 @@ int rbg_score_rows_i8(const void *u, int64_t ldu, int dtype, int64_t B, const in
     if (B <= 16 && B * K <= kOwnCodes) {
         const ScoreArgs a{nullptr, qi, ldu, ldi, nullptr, si, B, n, (int)((K + 15) / 16), S, lds, u, (int)K};
         return with_elem(out_dtype, [&](auto o) {
-            return with_elem(dtype, [&](auto t) { return launch_few<decltype(o), decltype(t), 1>(a, (hipStream_t)stream); });
+            return with_elem(dtype, [&](auto t) { return launch_score<decltype(o), decltype(t)>(a, (hipStream_t)stream); });
         });
     }
     if (int rc = rbg_quantize_rows_i8(u, ldu, dtype, B, K, qu, ldc, su, stream)) return rc;

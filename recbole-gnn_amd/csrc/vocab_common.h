@@ -42,6 +42,10 @@ __device__ __forceinline__ T from_f32(float x) { return (T)x; }
 
 constexpr int kWave = 64;
 
+// A grid holds fewer than 2^32 threads per dimension: operators with a workgroup of up to 1 024 threads per row launch for this many rows
+// at a time.
+constexpr int64_t kRowsPerLaunch = 1 << 21;
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);

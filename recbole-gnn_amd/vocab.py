@@ -96,9 +96,17 @@ def _embedding(table, ids, scale):
     return out
 
 
+def _padding(padding_idx, n_rows):
+    if padding_idx is None:
+        return -1
+    if not -n_rows <= padding_idx < n_rows:
+        raise ValueError(f"padding_idx = {padding_idx} is not a row of {n_rows}")
+    return int(padding_idx) % n_rows
+
+
 def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=None):
     """The gradient of :func:`embedding`'s table: ``out[v] = scale * sum of grad[i] over ids[i] == v`` as a dense [n_rows, d] tensor of
-    ``out_dtype`` (``grad``'s type, the default, or float32), zeros where no id refers to a row and in row ``padding_idx``.  The
+    ``out_dtype`` (``grad``'s type, the default, or float32), zeros where no id refers to a row and in row ``padding_idx`` (counted from the end when negative).  The
     places are sorted by id and summed in ascending order in 32 bits: the same bits from run to run."""
     if not grad.is_cuda:
         raise RuntimeError("grad must live on the GPU (the HIP engine has no CPU path)")
@@ -107,6 +115,7 @@ def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=Non
     d = grad.shape[-1]
     grad = _rows(grad.reshape(ids.numel(), d) if grad.dim() != 2 else grad, "grad")
     ids = _like(ids, grad, "ids", tuple(ids.shape), torch.int64)
+    padding_idx = _padding(padding_idx, n_rows)
     out_dtype = out_dtype or grad.dtype
     if out_dtype not in (grad.dtype, torch.float32):
         raise TypeError(f"out_dtype must be {grad.dtype} or float32, got {out_dtype}")
@@ -115,7 +124,7 @@ def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=Non
         n = ids.numel()
         work = _workspace(grad, "rbg_embedding_grad_workspace", n, n_rows, d)
         _call(lib.rbg_embedding_grad, grad, grad.data_ptr(), _ld(grad), _DTYPES[grad.dtype], ids.data_ptr(), n, n_rows, d, float(scale),
-              -1 if padding_idx is None else int(padding_idx), out.data_ptr(), _DTYPES[out_dtype], _ptr(work))
+              padding_idx, out.data_ptr(), _DTYPES[out_dtype], _ptr(work))
     return out
 
 
@@ -139,6 +148,7 @@ def embedding(table, ids, scale=1.0, padding_idx=None):
     ``nn.Embedding``.  The wide-type, scaled form of :func:`ops.gather_rows` (lightgcn.py:60-68,128)."""
     table = _rows(table, "table")
     ids = _like(ids, table, "ids", tuple(ids.shape), torch.int64)
+    _padding(padding_idx, table.shape[0])
     if table.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(table, ids, float(scale), padding_idx)
     return _embedding(table, ids, float(scale))

@@ -740,3 +740,84 @@ def test_scores_of_every_length(rbg, cuda, b, n):
         sums = qu.double() @ codes.double().t().contiguous()
         ref = sums.float() * su[:, None] * scales  # exact sums, then the two products in the order the operator takes them
         assert torch.equal(rbg.score_int8(u, wide[:, :k], scales[at]), ref[:, at]), (b, n, k)
+
+
+# ---- more rows than one launch takes -------------------------------------------------------------------------------------
+
+MANY = (1 << 21) + 3
+
+
+def test_many_ids(rbg, cuda):
+    n = (1 << 26) + 5
+    table = torch.randn(97, 1, generator=gen(1, cuda), device=cuda).to(F16)
+    ids = torch.arange(n, device=cuda) % 97
+    out = rbg.embedding(table, ids)
+    assert torch.equal(out[:, 0], table[:, 0].repeat(n // 97 + 1)[:n])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_distilled_rows(rbg, cuda, dtype):
+    """The rows repeat with a period, so that every launch's rows can be held against the first ones'."""
+    few = 1000
+    z, idx, val, w = distill_inputs(3, few, 5, 2, dtype, cuda)
+    at = torch.arange(MANY, device=cuda) % few
+    loss, grad = rbg.distill_topk_grad(z[at], idx[at], val[at], row_weight=w[at])
+    one, one_grad = rbg.distill_topk_grad(z, idx, val, row_weight=w)
+    assert torch.equal(loss, one[at]) and torch.equal(grad, one_grad[at])
+    leaf = z[at].requires_grad_()
+    rbg.distill_topk(leaf, idx[at], val[at]).backward(w[at])
+    few_leaf = z.clone().requires_grad_()
+    rbg.distill_topk(few_leaf, idx, val).backward(w)
+    assert torch.equal(leaf.grad, few_leaf.grad[at])
+
+
+def test_many_pairs(rbg, cuda):
+    """Pairs of one token each whose logits say which pair they belong to."""
+    few = 1000
+    g = gen(4, cuda)
+    z, y = torch.randn(2 * few, 3, generator=g, device=cuda), torch.randint(0, 3, (2 * few,), generator=g, device=cuda)
+    ref, w = torch.randn(2 * few, generator=g, device=cuda), torch.rand(few, generator=g, device=cuda)
+    tok, pair = torch.arange(2 * MANY, device=cuda) % (2 * few), torch.arange(MANY, device=cuda) % few
+    loss, margin, grad = rbg.preference_grad(z[tok], y[tok], torch.arange(2 * MANY + 1, device=cuda), ref[tok], beta=0.5, pair_weight=w[pair])
+    l1, m1, g1 = rbg.preference_grad(z, y, torch.arange(2 * few + 1, device=cuda), ref, beta=0.5, pair_weight=w)
+    assert torch.equal(loss, l1[pair]) and torch.equal(margin, m1[pair]) and torch.equal(grad, g1[tok])
+    logp = rbg.token_logp(z[tok], y[tok])
+    assert torch.equal(logp, rbg.token_logp(z, y)[tok])
+    l2, m2 = rbg.preference_loss(logp, torch.arange(2 * MANY + 1, device=cuda), ref[tok], beta=0.5)
+    l3, m3 = rbg.preference_loss(logp[:2 * few], torch.arange(2 * few + 1, device=cuda), ref, beta=0.5)
+    assert torch.equal(l2, l3[pair]) and torch.equal(m2, m3[pair])
+
+
+def test_many_quantized_rows(rbg, cuda):
+    x = torch.randn(1000, 3, generator=gen(5, cuda), device=cuda)
+    at = torch.arange(MANY, device=cuda) % 1000
+    codes, scales = rbg.quantize_rows(x[at])
+    c1, s1 = rbg.quantize_rows(x)
+    assert torch.equal(codes, c1[at]) and torch.equal(scales, s1[at])
+
+
+@pytest.mark.parametrize("b,k", [(1, 5), (2, 1100), (20, 5)])
+def test_many_items(rbg, cuda, b, k):
+    n = (1 << 24) + 5
+    g = gen(b + k, cuda)
+    u, items = torch.randn(b, k, generator=g, device=cuda), torch.randn(1000, k, generator=g, device=cuda)
+    codes, scales = rbg.quantize_rows(items)
+    at = torch.arange(n, device=cuda) % 1000
+    wide = torch.empty(n, codes.stride(0), dtype=torch.int8, device=cuda)
+    wide[:, :k] = codes[at]
+    out = rbg.score_int8(u, wide[:, :k], scales[at])
+    one = rbg.score_int8(u, codes, scales)  # exact sums: the same bits whatever the form
+    assert all(torch.equal(out[r], one[r][at]) for r in range(b))
+
+
+@pytest.mark.parametrize("n", [50, 3000])
+def test_padding_row_counted_from_the_end(rbg, cuda, n):
+    g = gen(n, cuda)
+    grad, ids = torch.randn(n, 24, generator=g, device=cuda), torch.randint(0, 30, (n,), generator=g, device=cuda)
+    got = rbg.embedding_grad(grad, ids, 30, padding_idx=-2)
+    assert torch.equal(got, rbg.embedding_grad(grad, ids, 30, padding_idx=28)) and torch.all(got[28] == 0) and torch.any(got[27] != 0)
+    for wrong in (30, -31):
+        with pytest.raises(ValueError):
+            rbg.embedding_grad(grad, ids, 30, padding_idx=wrong)
+        with pytest.raises(ValueError):
+            rbg.embedding(torch.zeros(30, 4, device=cuda), ids, padding_idx=wrong)
