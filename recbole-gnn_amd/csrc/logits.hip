@@ -598,21 +598,36 @@ __device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_
 }
 
 // One workgroup per pair: both sums in 64 bits, the loss, and (COEF) the tokens' gradients of pair_w loss.  Bound by latency (4 096
-// tokens of 32 pairs 5 us, 6 001 of two 10).
+// tokens of 32 pairs 5 us, 6 001 of two 8).
 template <class L, bool COEF>
 __global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, const int64_t *offsets, const float *ref, float beta,
                                                    float smoothing, const float *pair_w, float *loss, float *margin, float *coef) {
     __shared__ double red[2][4];
     const int64_t i = blockIdx.x;
     int64_t lo[2], hi[2];
+    seq_of(offsets, 2 * i, m, lo[0], hi[0]);
+    seq_of(offsets, 2 * i + 1, m, lo[1], hi[1]);
+    // both sequences as one list of tokens, 1 024 in flight
+    const int64_t first = hi[0] - lo[0], all = first + hi[1] - lo[1], skip = lo[1] - first;
+    double v[2] = {0.0, 0.0};
+    for (int64_t u0 = threadIdx.x; u0 < all; u0 += 1024) {
+        double l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t u = u0 + 256 * q;
+            l[q] = u < all ? (double)logp[u + (u < first ? lo[0] : skip)] : 0.0;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const bool second = u0 + 256 * q >= first;
+            v[0] += second ? 0.0 : l[q], v[1] += second ? l[q] : 0.0;
+        }
+    }
     double sum[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        seq_of(offsets, 2 * i + k, m, lo[k], hi[k]);
-        double v = 0.0;
-        for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) v += (double)logp[t];
-        v = wave_sum(v);
-        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = v;
+        const double w = wave_sum(v[k]);
+        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = w;
     }
     __syncthreads();
 #pragma unroll
@@ -621,9 +636,7 @@ __global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, con
     if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
     if constexpr (COEF) {
         const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) coef[t] = k ? -d : d;
+        for (int64_t u = threadIdx.x; u < all; u += 256) coef[u + (u < first ? lo[0] : skip)] = u < first ? d : -d;
     }
 }
 
