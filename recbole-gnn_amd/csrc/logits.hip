@@ -597,47 +597,97 @@ __device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_
     hi = hi < lo ? lo : hi > m ? m : hi;
 }
 
-// One workgroup per pair: both sums in 64 bits, the loss, and (COEF) the tokens' gradients of pair_w loss.  Bound by latency (4 096
-// tokens of 32 pairs 5 us, 6 001 of two 8).
-template <class L, bool COEF>
-__global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, const int64_t *offsets, const float *ref, float beta,
-                                                   float smoothing, const float *pair_w, float *loss, float *margin, float *coef) {
-    __shared__ double red[2][4];
-    const int64_t i = blockIdx.x;
-    int64_t lo[2], hi[2];
+// The margin of a pair, by the TH threads of a workgroup: both sequences as one list of tokens, 4 TH in flight, both sums in 64 bits.
+template <class L, int TH>
+__device__ __forceinline__ float pair_margin(const L *logp, int64_t m, const int64_t *offsets, const float *ref, int64_t i, float beta,
+                                             int64_t (&lo)[2], int64_t (&hi)[2], double (&red)[2][TH / kWave]) {
     seq_of(offsets, 2 * i, m, lo[0], hi[0]);
     seq_of(offsets, 2 * i + 1, m, lo[1], hi[1]);
-    // both sequences as one list of tokens, 1 024 in flight
+    const float r0 = ref[2 * i], r1 = ref[2 * i + 1];
     const int64_t first = hi[0] - lo[0], all = first + hi[1] - lo[1], skip = lo[1] - first;
     double v[2] = {0.0, 0.0};
-    for (int64_t u0 = threadIdx.x; u0 < all; u0 += 1024) {
+    for (int64_t u0 = threadIdx.x; u0 < all; u0 += 4 * TH) {
         double l[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int64_t u = u0 + 256 * q;
+            const int64_t u = u0 + TH * q;
             l[q] = u < all ? (double)logp[u + (u < first ? lo[0] : skip)] : 0.0;
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const bool second = u0 + 256 * q >= first;
+            const bool second = u0 + TH * q >= first;
             v[0] += second ? 0.0 : l[q], v[1] += second ? l[q] : 0.0;
         }
     }
     double sum[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const double w = wave_sum(v[k]);
-        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = w;
+        sum[k] = wave_sum(v[k]);
+        if constexpr (TH > kWave)
+            if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = sum[k];
     }
-    __syncthreads();
+    if constexpr (TH > kWave) {
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) sum[k] = ((red[k][0] + red[k][1]) + (red[k][2] + red[k][3])) - (double)ref[2 * i + k];
-    const float h = (float)((double)beta * (sum[0] - sum[1]));
+        for (int k = 0; k < 2; ++k) {
+            sum[k] = red[k][0];
+#pragma unroll
+            for (int q = 1; q < TH / kWave; ++q) sum[k] += red[k][q];
+        }
+    }
+    return (float)((double)beta * ((sum[0] - (double)r0) - (sum[1] - (double)r1)));
+}
+
+// One workgroup per pair: the loss, and (COEF) the tokens' gradients of pair_w loss.  Bound by latency (4 096 tokens of 32 pairs 5 us,
+// 6 001 of two 8).
+template <class L, bool COEF>
+__global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, const int64_t *offsets, const float *ref, float beta,
+                                                   float smoothing, const float *pair_w, float *loss, float *margin, float *coef) {
+    __shared__ double red[2][4];
+    const int64_t i = blockIdx.x;
+    int64_t lo[2], hi[2];
+    const float h = pair_margin<L, 256>(logp, m, offsets, ref, i, beta, lo, hi, red);
     if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
     if constexpr (COEF) {
         const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
-        for (int64_t u = threadIdx.x; u < all; u += 256) coef[u + (u < first ? lo[0] : skip)] = u < first ? d : -d;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) coef[t] = k ? -d : d;
     }
+}
+
+// Pairs and gradients in one launch, for few tokens: the workgroups of a row find its sequence (the last one that begins at or before it)
+// and form their pair's margin for themselves, which reads kFusedTokens log-probabilities at most; one workgroup per pair behind the
+// rows' (blockIdx.y >= m, part 0) writes its loss.
+constexpr int64_t kFusedTokens = 1024, kFusedPairs = 256;
+
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void pair_rows_kernel(const LogpArgs a, int64_t m, const int64_t *offsets, int64_t pairs, const float *ref,
+                                                       float beta, float smoothing, const float *pair_w, float *loss, float *margin, void *gv,
+                                                       int64_t ldg) {
+    __shared__ double red[2][TH / kWave];
+    int64_t lo[2], hi[2];
+    if (blockIdx.y >= m) {
+        if (blockIdx.x) return;
+        const int64_t i = blockIdx.y - m;
+        const float h = pair_margin<double, TH>(a.logp64, m, offsets, ref, i, beta, lo, hi, red);
+        if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
+        return;
+    }
+    const int64_t row = blockIdx.y, t = a.targets[row];
+    float w = 0.f;
+    if (t >= 0 && t < a.V) {
+        int before = 0;  // offsets at or before the row
+        for (int64_t c = threadIdx.x & 63; c - (threadIdx.x & 63) <= 2 * pairs; c += 64)
+            before += __popcll(__ballot(c <= 2 * pairs && offsets[min(c, 2 * pairs)] <= row));
+        if (before > 0 && before <= 2 * pairs) {
+            const int64_t i = (before - 1) >> 1;
+            const float h = pair_margin<double, TH>(a.logp64, m, offsets, ref, i, beta, lo, hi, red);
+            const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
+            w = (before - 1) & 1 ? -d : d;
+        }
+    }
+    grad_row<T, TH>(a.z, a.ldz, a.V, a.targets, a.stats, row, w, gv, ldg, blockIdx.x, gridDim.x);
 }
 
 // Small calls in one launch: a workgroup per pair, a wave per row.  Both sums meet in LDS, and the rows, read a second time for their
@@ -999,9 +1049,22 @@ int rbg_preference_grad(const void *z, int64_t ldz, int dtype, int64_t m, int64_
             RBG_HIP(hipGetLastError());
             return (int)RBG_OK;
         }
+        // Pairs and gradients in one launch: 870 x 135 bf16, 40 pairs, 16.1 us a call against 18.4; 883 x 5 178 fp32, 10 pairs, 16.3 against
+        // 18.3; but 1 000 x 40 000 bf16, 200 pairs (80 MB), 41.3 against 39.4, and 1 024 x 131 072 fp32, one pair, 252 against 228.
+        const bool fused = m && m <= kFusedTokens && pairs <= kFusedPairs && total <= 32 << 20;
         if (m) {
-            const LogpArgs a{z, ldz, (int)V, targets, nullptr, logp, coef, stats, part};
+            const LogpArgs a{z, ldz, (int)V, targets, nullptr, logp, fused ? nullptr : coef, stats, part};
             if (int rc = launch_logp<E>(a, m, V, s)) return rc;
+        }
+        if (fused) {
+            const LogpArgs a{z, ldz, (int)V, targets, nullptr, logp, nullptr, stats, nullptr};
+            const dim3 grid(grad_parts(V, sizeof(E)), (unsigned)(m + pairs));
+            if (V * (int64_t)sizeof(E) <= 4096)
+                hipLaunchKernelGGL((pair_rows_kernel<E, 64>), grid, dim3(64), 0, s, a, m, offsets, pairs, ref, beta, smoothing, pair_w, loss, margin, grad, ldg);
+            else
+                hipLaunchKernelGGL((pair_rows_kernel<E, 256>), grid, dim3(256), 0, s, a, m, offsets, pairs, ref, beta, smoothing, pair_w, loss, margin, grad, ldg);
+            RBG_HIP(hipGetLastError());
+            return (int)RBG_OK;
         }
         if (int rc = launch_pairs<double, true>(logp, m, offsets, pairs, ref, beta, smoothing, pair_w, loss, margin, coef, s)) return rc;
         return m ? launch_logp_grad<E>((const E *)z, ldz, m, V, targets, stats, coef, (E *)grad, ldg, s) : (int)RBG_OK;

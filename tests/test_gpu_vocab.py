@@ -821,3 +821,43 @@ def test_padding_row_counted_from_the_end(rbg, cuda, n):
             rbg.embedding_grad(grad, ids, 30, padding_idx=wrong)
         with pytest.raises(ValueError):
             rbg.embedding(torch.zeros(30, 4, device=cuda), ids, padding_idx=wrong)
+
+
+# one launch for pairs and gradients up to 1 024 tokens, 256 pairs and 32 MB of logits; three beyond
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("m,v,pairs", [(1024, 33, 256), (1024, 33, 257), (1025, 33, 256), (300, 1500, 1), (1000, 4097, 3), (1024, 8192, 2), (1023, 20000, 40)])
+def test_preference_forms(rbg, cuda, dtype, m, v, pairs):
+    """A log-probability is off by its row's S and its own z - m in 32 bits; a margin by those of its tokens, summed in 64 bits, and its own
+    rounding; the sigmoid passes a margin's error on by at most a quarter of it."""
+    g = gen(m + pairs, cuda)
+    z = torch.randn(m, v, generator=g, device=cuda).to(dtype)
+    y = torch.randint(-1, v, (m,), generator=g, device=cuda)
+    offsets = torch.sort(torch.randint(0, m + 1, (2 * pairs + 1,), generator=g, device=cuda)).values
+    weight = torch.rand(pairs, generator=g, device=cuda) + 0.5
+    lp = torch.log_softmax(z.double(), 1)
+    lp = torch.where(y >= 0, lp.gather(1, y.clamp(min=0)[:, None])[:, 0], 0.0)
+    sums = torch.cat([lp.new_zeros(1), lp.cumsum(0)])[offsets]
+    seq = sums[1:] - sums[:-1]
+    ref = (seq + torch.randn(2 * pairs, generator=g, device=cuda)).float()
+    beta = 0.5
+    loss, margin, grad = rbg.preference_grad(z, y, offsets, ref, beta=beta, pair_weight=weight)
+    want = beta * ((seq[0::2] - ref[0::2].double()) - (seq[1::2] - ref[1::2].double()))
+    # a log-probability in the call: its row's S and its own z - m in 32 bits, as in the head of this file
+    spread = (z.double().amax(1) - z.double().amin(1)).max().item() / math.log(2)
+    one = (4 + 3 * spread + 2 * (v / 64 + 96)) * U
+    count = (offsets[1:] - offsets[:-1]).double()
+    tol = beta * (count[0::2] + count[1::2]) * one + 4 * U * want.abs() + 1e-12 * seq.abs().max()
+    within(margin, want, tol)
+    dl = -torch.sigmoid(-want)
+    where = torch.bucketize(torch.arange(m, device=cuda), offsets, right=True) - 1
+    inside = (where >= 0) & (where < 2 * pairs) & (y >= 0)
+    pair = where.clamp(0, 2 * pairs - 1) // 2
+    w = torch.where(inside, beta * (dl * weight.double())[pair] * (1 - 2 * (where % 2)), 0.0)
+    q = torch.softmax(z.double(), 1)
+    hot = torch.zeros_like(q)
+    hot[torch.arange(m, device=cuda)[y >= 0], y[y >= 0]] = 1.0
+    want_grad = w[:, None] * (hot - q)
+    # w: the sigmoid's 8 u and a quarter of the margin's error; q: its error; the difference and the product one u each
+    bound = want_grad.abs() * (12 * U) + beta * weight.max() * (tol[pair] / 4)[:, None] * inside[:, None] * (hot + q) + w.abs()[:, None] * q * one
+    within(grad, want_grad, bound + stored(want_grad, dtype) + stored(bound, dtype))
+    assert torch.all(grad[~inside] == 0)
