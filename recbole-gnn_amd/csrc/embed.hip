@@ -65,7 +65,8 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table
 
 // ---- sort ----------------------------------------------------------------------------------------------------------------
 
-constexpr int kRankMax = 16384;  // places ranked by counting
+// Places ranked by counting (15 565 places of 4 221 rows: 41 us a call this way, 38 by digits; 12 200: 34 and 35.5; 9 000: 29 and 33.5).
+constexpr int kRankMax = 12288;
 constexpr int kMaxBits = 9;
 
 // A place's sort key: its row, or n_rows for one that adds to nothing (such places end behind every row).
@@ -360,7 +361,8 @@ struct RunArgs {
     void *out;
     float *part;               // [chunks][2][d]: sums of the chunk's first run and of its last, where they cross a border
     uint32_t *list, *count;    // chunks whose last run starts there and goes on
-    int64_t run_blocks;        // the launch's workgroups that sum; the rest zero rows
+    int64_t run_blocks;        // the launch's workgroups that sum; the rest zero rows,
+    int stripe;                // this many each
 };
 
 template <class T, int VEC>
@@ -386,7 +388,8 @@ __device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t
     return lo;
 }
 
-constexpr int kStripe = 256;  // rows that one workgroup zeroes
+constexpr int kFewRows = 16;
+constexpr int kStripe = 256;  // rows that one workgroup zeroes, at most
 
 // G lanes x VEC elements cover a piece of a row (blockIdx.y: which piece); 256 / G chunks per workgroup.  Bound by reading rows in sorted,
 // that is random, order: 65 536 gradient rows of 2 KB (bf16, d = 1 024) and 131 072 rows written, 403 MB in 89 us = 4.5 TB/s; the join
@@ -402,8 +405,8 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     if (blockIdx.x >= a.run_blocks) {  // zero the rows of a stripe that no place refers to
         __shared__ uint32_t used[kStripe];
         __shared__ int64_t bounds[2];
-        const int64_t r0 = (int64_t)(blockIdx.x - a.run_blocks) * kStripe;
-        const int rows = (int)min<int64_t>(kStripe, a.n_rows - r0);
+        const int64_t r0 = (int64_t)(blockIdx.x - a.run_blocks) * a.stripe;
+        const int rows = (int)min<int64_t>(a.stripe, a.n_rows - r0);
         if (threadIdx.x < kStripe) used[threadIdx.x] = 0;
         if (threadIdx.x < 128) {
             const int w = threadIdx.x >> 6;
@@ -413,7 +416,12 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
         __syncthreads();
         if (bounds[1] - bounds[0] <= 4096) {
             for (int64_t p = bounds[0] + threadIdx.x; p < bounds[1]; p += 256) used[a.keys[p] - (uint32_t)r0] = 1;
-        } else if ((int)threadIdx.x < rows) {  // long runs: each row looks for itself
+        } else if (rows <= kFewRows) {  // long runs: a wave looks for each row
+            for (int q = threadIdx.x >> 6; q < rows; q += 4) {
+                const int64_t at = bounds[0] + first_not_below(a.keys + bounds[0], bounds[1] - bounds[0], (uint32_t)(r0 + q));
+                if ((threadIdx.x & 63) == 0) used[q] = at < bounds[1] && a.keys[at] == (uint32_t)(r0 + q);
+            }
+        } else if ((int)threadIdx.x < rows) {  // each row looks for itself
             int64_t lo = bounds[0], hi = bounds[1];
             const uint32_t key = (uint32_t)(r0 + threadIdx.x);
             while (lo < hi) {
@@ -655,10 +663,13 @@ static void launch_runs(const RunArgs &a0, const int64_t *ids, int64_t padding, 
     }
     a.run_blocks = (a.chunks + 256 / G - 1) / (256 / G);
     const unsigned pieces = (unsigned)((a.d + G * VEC - 1) / (G * VEC));
-    const int64_t zero_blocks = (a.n_rows + kStripe - 1) / kStripe;
+    // rows of about 1 024 places, which a workgroup takes its rows' marks from at once
+    a.stripe = kStripe;
+    while (a.stripe > 8 && a.n * a.stripe > 1024 * a.n_rows) a.stripe /= 2;
+    const int64_t zero_blocks = (a.n_rows + a.stripe - 1) / a.stripe;
     hipLaunchKernelGGL((run_sum_kernel<TI, TO, VEC, G>), dim3((unsigned)(a.run_blocks + zero_blocks), pieces), dim3(256), 0, s, a);
     if (a.chunks > 1)
-        hipLaunchKernelGGL((run_join_kernel<TO, VEC, G>), dim3((unsigned)std::min<int64_t>(a.chunks, 1024), pieces), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((run_join_kernel<TO, VEC, G>), dim3((unsigned)std::min<int64_t>(a.chunks, 4096), pieces), dim3(256), 0, s, a);
 }
 
 template <class TI, class TO>
@@ -788,7 +799,7 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
         }
     }
     RBG_HIP(hipGetLastError());
-    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0};
+    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0, 0};
     const bool wide = d * size >= 16;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;

@@ -861,3 +861,18 @@ def test_preference_forms(rbg, cuda, dtype, m, v, pairs):
     bound = want_grad.abs() * (12 * U) + beta * weight.max() * (tol[pair] / 4)[:, None] * inside[:, None] * (hot + q) + w.abs()[:, None] * q * one
     within(grad, want_grad, bound + stored(want_grad, dtype) + stored(bound, dtype))
     assert torch.all(grad[~inside] == 0)
+
+
+@pytest.mark.parametrize("n,rows,d", [(12288, 40, 24), (12289, 40, 24), (13000, 17, 9), (13000, 260000, 8), (20000, 3, 8), (40000, 200, 33), (60000, 3001, 8), (65536, 9, 4),
+                                      (70000, 1000, 16), (300000, 33, 4)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_embedding_grad_rows_between_long_runs(rbg, cuda, dtype, n, rows, d):
+    """Only every third row is used and the last used one has half of the places: what lies between long runs is zeroed."""
+    g = gen(n + rows, cuda)
+    grad = torch.randn(n, d, generator=g, device=cuda).to(dtype)
+    ids = torch.randint(0, (rows + 2) // 3, (n,), generator=g, device=cuda) * 3
+    ids[torch.rand(n, generator=g, device=cuda) < 0.5] = (rows - 1) // 3 * 3
+    got = rbg.embedding_grad(grad, ids, rows)
+    ref, mag, cnt = runs_reference(grad, ids, rows, 1.0, -1)
+    within(got, ref, stored(ref, dtype) + mag * U * (cnt + 4))  # cnt additions in some order
+    assert torch.all(got[cnt[:, 0] == 0] == 0)
