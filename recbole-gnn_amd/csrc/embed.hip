@@ -65,7 +65,8 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table
 
 // ---- sort ----------------------------------------------------------------------------------------------------------------
 
-// Places ranked by counting (15 565 places of 4 221 rows: 41 us a call this way, 38 by digits; 12 200: 34 and 35.5; 9 000: 29 and 33.5).
+// Places ranked by counting (15 565 places of 4 221 rows with their lookup: 41 us this way, 38 by digits; 12 200: 34 and 35.5; 9 000: 29
+// and 33.5).
 constexpr int kRankMax = 12288;
 constexpr int kMaxBits = 9;
 
@@ -82,14 +83,13 @@ __device__ __forceinline__ uint32_t key_of(const int64_t *ids, int64_t i, int64_
 // compares: 6 144 places in 7.7 us; one launch where radix passes would be four.
 template <int Q>
 __global__ __launch_bounds__(1024) void rank_kernel(const int64_t *__restrict__ ids, int n, int64_t n_rows, int64_t padding,
-                                                    uint32_t *__restrict__ keys, uint32_t *__restrict__ places, uint32_t *count) {
+                                                    uint32_t *__restrict__ keys, uint32_t *__restrict__ places) {
     constexpr int U = 8;  // steps in flight
     __shared__ uint32_t all[kRankMax];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n64 = (n + 63) & ~63;
 #pragma unroll 8
     for (int j = threadIdx.x; j < n64; j += 1024) all[j] = j < n ? key_of(ids, j, n_rows, padding) : 0xffffffffu;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
     const int i0 = (blockIdx.x * 16 + w) * Q;
     if (i0 >= n) return;
@@ -179,10 +179,9 @@ constexpr int kMoveTiles = kMoveMax / kMoveTile;
 
 // The first pass's counts; the later passes' are cleared.
 __global__ __launch_bounds__(512) void move_count_kernel(const int64_t *ids, int n, int64_t n_rows, int64_t padding, int bits, int passes,
-                                                         uint32_t *counts, uint32_t *count) {
+                                                         uint32_t *counts) {
     __shared__ uint32_t h[kBins];
     h[threadIdx.x] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < kMoveTile / 512; ++u) {
@@ -262,11 +261,10 @@ __global__ __launch_bounds__(512) void move_kernel(const int64_t *ids, const uin
 // Three launches per pass (beyond kMoveMax places).  First: how often each digit occurs in each tile -> hist[digit][tile].  (ids: the first pass.)
 constexpr int kTile = 2048;
 __global__ __launch_bounds__(256) void digit_count_kernel(const int64_t *ids, const uint32_t *keys, int64_t n, int64_t n_rows, int64_t padding,
-                                                          int shift, int bits, uint32_t *hist, uint32_t *count) {
+                                                          int shift, int bits, uint32_t *hist) {
     __shared__ uint32_t h[1 << kMaxBits];
     const int bins = 1 << bits;
     for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
     __syncthreads();
     const int64_t i0 = (int64_t)blockIdx.x * kTile;
 #pragma unroll
@@ -360,7 +358,6 @@ struct RunArgs {
     float scale;
     void *out;
     float *part;               // [chunks][2][d]: sums of the chunk's first run and of its last, where they cross a border
-    uint32_t *list, *count;    // chunks whose last run starts there and goes on
     int64_t run_blocks;        // the launch's workgroups that sum; the rest zero rows,
     int stripe;                // this many each
 };
@@ -388,12 +385,11 @@ __device__ __forceinline__ int64_t first_not_below(const uint32_t *keys, int64_t
     return lo;
 }
 
-constexpr int kFewRows = 16;
 constexpr int kStripe = 256;  // rows that one workgroup zeroes, at most
 
 // G lanes x VEC elements cover a piece of a row (blockIdx.y: which piece); 256 / G chunks per workgroup.  Bound by reading rows in sorted,
-// that is random, order: 65 536 gradient rows of 2 KB (bf16, d = 1 024) and 131 072 rows written, 403 MB in 89 us = 4.5 TB/s; the join
-// behind it 6.
+// that is random, order: 65 536 gradient rows of 2 KB (bf16, d = 1 024) and 131 072 rows written, 403 MB in 86 us = 4.7 TB/s; the join
+// behind it 7.
 template <class TI, class TO, int VEC, int G>
 __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
     constexpr int U = G < 8 ? G : 8;  // rows in flight per lane-group
@@ -416,7 +412,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
         __syncthreads();
         if (bounds[1] - bounds[0] <= 4096) {
             for (int64_t p = bounds[0] + threadIdx.x; p < bounds[1]; p += 256) used[a.keys[p] - (uint32_t)r0] = 1;
-        } else if (rows <= kFewRows) {  // long runs: a wave looks for each row
+        } else if (rows <= 16) {  // long runs: a wave looks for each row
             for (int q = threadIdx.x >> 6; q < rows; q += 4) {
                 const int64_t at = bounds[0] + first_not_below(a.keys + bounds[0], bounds[1] - bounds[0], (uint32_t)(r0 + q));
                 if ((threadIdx.x & 63) == 0) used[q] = at < bounds[1] && a.keys[at] == (uint32_t)(r0 + q);
@@ -497,7 +493,6 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const RunArgs a) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) to[e] = acc[e];
     }
-    if (!first && sub == 0 && blockIdx.y == 0) a.list[atomicAdd(a.count, 1u)] = (uint32_t)c;  // (the list's order changes no sum)
 }
 
 // Few places (n <= kFewPlaces): one launch, no sorted list.  A workgroup owns `stripe` rows (and a piece of their columns), finds the places that
@@ -569,7 +564,9 @@ __global__ __launch_bounds__(256) void few_places_kernel(const RunArgs a, const 
         if (!used[q]) store_row<TO, VEC>(out + (r0 + q) * a.d + col, zero, 1.f);
 }
 
-// Runs over several chunks: the last sum of the chunk they start in, then the first sums of the chunks they reach into.
+// Runs over several chunks: the last sum of the chunk they start in, then the first sums of the chunks they reach into.  A workgroup finds
+// out for itself whether a run starts in its chunk and goes on (a list of such chunks cost the launch before it an atomic each at one
+// address: 5 us for 3 000 of them).
 template <class TO, int VEC, int G>
 __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
     constexpr int N = 256 / G;
@@ -577,10 +574,10 @@ __global__ __launch_bounds__(256) void run_join_kernel(const RunArgs a) {
     const int sub = threadIdx.x % G, grp = threadIdx.x / G;
     const int piece = (blockIdx.y * G + sub) * VEC, col = vector_at<VEC>(piece, a.d);
     const bool on = piece < a.d;
-    const uint32_t todo = *a.count;
-    for (uint32_t t = blockIdx.x; t < todo; t += gridDim.x) {
-        const int64_t c = a.list[t];
-        const uint32_t key = a.keys[(c + 1) * a.chunk];
+    for (int64_t c = blockIdx.x; c + 1 < a.chunks; c += gridDim.x) {
+        const int64_t p0 = c * a.chunk, p1 = p0 + a.chunk;
+        const uint32_t key = a.keys[p1], own = a.keys[p1 - 1], ahead = p0 > 0 ? a.keys[p0 - 1] : 0xffffffffu;
+        if (key != own || key == ahead || key == (uint32_t)a.n_rows) continue;  // no run, or none of a row, starts in chunk c and goes on
         // the last chunk that starts with the run's key
         const int64_t last = c + first_not_below(a.keys + (c + 1) * a.chunk, a.chunks - c - 1, key + 1u, a.chunk);
         // parts c, c + 1, .., last: an equal piece for each lane-group, the pieces joined in order
@@ -621,7 +618,7 @@ static int chunk_of(int64_t n, int d) {
 }
 
 struct Layout {
-    int64_t keys, places, keys2, places2, hist, total, part, list, count, bytes;
+    int64_t keys, places, keys2, places2, hist, total, part, bytes;
     int chunk, tiles;
     int64_t chunks;
 };
@@ -638,14 +635,12 @@ static Layout layout_of(int64_t n, int d) {
         return r;
     };
     if (n <= kFewPlaces) return l;
-    l.count = take(16);
     l.keys = take(4 * n), l.places = take(4 * n);
     if (n > kRankMax) {
         l.keys2 = take(4 * n), l.places2 = take(4 * n);
         l.hist = take(4ll * kBins * l.tiles * (n <= kMoveMax ? kMaxPasses : 1));
         l.total = take(4 * kBins);
     }
-    l.list = take(4 * l.chunks);
     l.part = take(4ll * 2 * l.chunks * d);
     l.bytes = at;
     return l;
@@ -669,7 +664,7 @@ static void launch_runs(const RunArgs &a0, const int64_t *ids, int64_t padding, 
     const int64_t zero_blocks = (a.n_rows + a.stripe - 1) / a.stripe;
     hipLaunchKernelGGL((run_sum_kernel<TI, TO, VEC, G>), dim3((unsigned)(a.run_blocks + zero_blocks), pieces), dim3(256), 0, s, a);
     if (a.chunks > 1)
-        hipLaunchKernelGGL((run_join_kernel<TO, VEC, G>), dim3((unsigned)std::min<int64_t>(a.chunks, 4096), pieces), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((run_join_kernel<TO, VEC, G>), dim3((unsigned)std::min<int64_t>(a.chunks, 16384), pieces), dim3(256), 0, s, a);
 }
 
 template <class TI, class TO>
@@ -761,13 +756,12 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
     hipStream_t s = (hipStream_t)stream;
     const Layout l = layout_of(n, d);
     char *w = (char *)workspace;
-    uint32_t *count = (uint32_t *)(w + l.count);
     uint32_t *keys = (uint32_t *)(w + l.keys), *places = (uint32_t *)(w + l.places);
     if (n > kFewPlaces && n <= kRankMax) {
         // places per wave: few where there are few, so that every CU has a workgroup
-        if (n <= 4096) hipLaunchKernelGGL((rank_kernel<1>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
-        else if (n <= 8192) hipLaunchKernelGGL((rank_kernel<2>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
-        else hipLaunchKernelGGL((rank_kernel<4>), dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places, count);
+        if (n <= 4096) hipLaunchKernelGGL((rank_kernel<1>), dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places);
+        else if (n <= 8192) hipLaunchKernelGGL((rank_kernel<2>), dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places);
+        else hipLaunchKernelGGL((rank_kernel<4>), dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s, ids, (int)n, n_rows, padding_idx, keys, places);
     } else if (n > kRankMax) {
         int bits = 1;
         while (((int64_t)1 << bits) <= n_rows) ++bits;  // keys 0 .. n_rows
@@ -775,7 +769,7 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
         uint32_t *k2 = (uint32_t *)(w + l.keys2), *p2 = (uint32_t *)(w + l.places2);
         uint32_t *hist = (uint32_t *)(w + l.hist), *total = (uint32_t *)(w + l.total);
         const uint32_t *from_k = nullptr, *from_p = nullptr;
-        if (n <= kMoveMax) hipLaunchKernelGGL(move_count_kernel, dim3(l.tiles), dim3(512), 0, s, ids, (int)n, n_rows, padding_idx, width, passes, hist, count);
+        if (n <= kMoveMax) hipLaunchKernelGGL(move_count_kernel, dim3(l.tiles), dim3(512), 0, s, ids, (int)n, n_rows, padding_idx, width, passes, hist);
         // the last pass ends in (keys, places)
         uint32_t *to_k = passes & 1 ? keys : k2, *to_p = passes & 1 ? places : p2;
         for (int q = 0; q < passes; ++q) {
@@ -789,7 +783,7 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
                     hipLaunchKernelGGL((move_kernel<false>), dim3(l.tiles), dim3(512), 0, s, src, from_k, from_p, (int)n, n_rows, padding_idx, q * width, width,
                                        counts, nullptr, to_k, to_p);
             } else {
-                hipLaunchKernelGGL(digit_count_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist, count);
+                hipLaunchKernelGGL(digit_count_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, n, n_rows, padding_idx, q * width, width, hist);
                 hipLaunchKernelGGL(digit_prefix_kernel, dim3(1u << width), dim3(256), 0, s, hist, l.tiles, total);
                 hipLaunchKernelGGL(digit_scatter_kernel, dim3(l.tiles), dim3(256), 0, s, src, from_k, from_p, n, n_rows, padding_idx, q * width, width,
                                    hist, total, to_k, to_p);
@@ -799,7 +793,7 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
         }
     }
     RBG_HIP(hipGetLastError());
-    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), (uint32_t *)(w + l.list), count, 0, 0};
+    const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), 0, 0};
     const bool wide = d * size >= 16;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
