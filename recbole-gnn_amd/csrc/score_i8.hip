@@ -149,13 +149,52 @@ struct ScoreArgs {
     int K;
 };
 
+// The codes of a row that two lanes share, h the even 16-byte chunks or the odd ones, from its K values; its scale.
+template <class TU, int KS>
+__device__ __forceinline__ float own_codes(const TU *x, int K, int h, i32x4 (&codes)[KS]) {
+    constexpr int E = 16 / (int)sizeof(TU);
+    TU v[KS][16];
+    float mag = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        const int c = 16 * (2 * k + h);
+        if (c + 16 <= K) {
+#pragma unroll
+            for (int q = 0; q < 16 / E; ++q) {
+                const Vec<TU, E> t = load_any<TU, E>(x + c + q * E);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[k][q * E + e] = t.v[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[k][e] = c + e < K ? x[c + e] : from_f32<TU>(0.f);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mag = fmaxf(mag, magnitude(to_f32(v[k][e])));
+    const RowScale s = row_scale(fmaxf(mag, __shfl_xor(mag, 32)));
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w = 0;
+            if (s.s != 0.f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w |= code_of(to_f32(v[k][4 * q + e]), s.s) << (8 * e);
+            codes[k][q] = (int)w;
+        }
+    return s.out;
+}
+
 // Short rows (K <= 32 KS): the scores are written at the rate of the stores and everything else has to hide behind them.  A workgroup
 // keeps 32 users' codes in registers and walks item tiles of TB bytes of scores per row: each wave multiplies 32 items' codes at a time,
 // taken straight from the table, and puts its scores into LDS, every row shifted by its distance from a 128-byte line.  Whole lines then
 // leave as 16-byte stores of consecutive lanes (1 KB of a row per wave and store at TB = 2048), whatever the row stride; what a tile leaves
 // over of a row's last line (less than LINE scores) moves to the front of the row for the next tile.  4 096 x 40 982 x 64 into fp32:
 // 672 MB in 135 us = 5.0 TB/s, which is the rate of bare whole-line stores into rows of that stride (131 to 138).
-template <class TO, int KS, int TB>
+template <class TO, class TU, int KS, int TB>
 __global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel(const ScoreArgs a, int tiles_per_walk) {
     constexpr int E = 16 / (int)sizeof(TO), TILE = TB / (int)sizeof(TO), LINE = 128 / (int)sizeof(TO), PITCH = TILE + LINE;
     __shared__ alignas(16) TO buf[32 * PITCH];
@@ -168,15 +207,21 @@ __global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel
     // row r starts (off0 + r step) mod LINE scores behind a line, and so does every tile of it (TILE is whole lines)
     const unsigned off0 = (unsigned)((reinterpret_cast<uintptr_t>(S) / sizeof(TO)) % LINE), step = (unsigned)(a.lds % LINE);
     i32x4 fu[KS];
-    const i32x4 *pu = reinterpret_cast<const i32x4 *>(a.qu + min(b0 + m, a.B - 1) * a.ldu) + h;
+    float own_su = 0.f;
+    if constexpr (std::is_void_v<TU>) {
+        const i32x4 *pu = reinterpret_cast<const i32x4 *>(a.qu + min(b0 + m, a.B - 1) * a.ldu) + h;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) fu[k] = pu[2 * k];
+        for (int k = 0; k < KS; ++k) fu[k] = pu[2 * k];
+    } else {
+        own_su = own_codes<TU, KS>((const TU *)a.u + min(b0 + m, a.B - 1) * a.ldu, a.K, h, fu);
+    }
     float su[16];
     unsigned at[16];  // where this lane's item of sub-tile 0 goes, for each of its 16 rows
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const unsigned row = (r & 3) + 8 * (r >> 2) + 4 * h;
-        su[r] = a.su[min<int64_t>(b0 + row, a.B - 1)];
+        if constexpr (std::is_void_v<TU>) su[r] = a.su[min<int64_t>(b0 + row, a.B - 1)];
+        else su[r] = __shfl(own_su, row);
         at[r] = row * PITCH + ((off0 + row * step) & (LINE - 1)) + w * 32 + m;
     }
     i32x4 fi[KS];
@@ -233,7 +278,7 @@ __global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel
     }
 }
 
-template <class TO, int KS, int TB>
+template <class TO, class TU, int KS, int TB>
 static int launch_short(const ScoreArgs &a, int64_t resident, hipStream_t s) {
     constexpr int TILE = TB / (int)sizeof(TO);
     const int64_t tiles = (a.n + TILE - 1) / TILE, panels = (a.B + 31) / 32;
@@ -243,19 +288,21 @@ static int launch_short(const ScoreArgs &a, int64_t resident, hipStream_t s) {
     walks = (tiles + per - 1) / per;
     for (int64_t y0 = 0; y0 < panels; y0 += 65535) {  // (a grid's y dimension ends at 65 535)
         ScoreArgs p = a;
-        p.qu += y0 * 32 * a.ldu, p.su += y0 * 32, p.B -= y0 * 32;
+        if constexpr (std::is_void_v<TU>) p.qu += y0 * 32 * a.ldu, p.su += y0 * 32;
+        else p.u = (const TU *)a.u + y0 * 32 * a.ldu;
+        p.B -= y0 * 32;
         p.S = (TO *)a.S + y0 * 32 * a.lds;
-        hipLaunchKernelGGL((score_i8_short_kernel<TO, KS, TB>), dim3((unsigned)walks, (unsigned)std::min<int64_t>(65535, panels - y0)), dim3(256), 0, s, p, per);
+        hipLaunchKernelGGL((score_i8_short_kernel<TO, TU, KS, TB>), dim3((unsigned)walks, (unsigned)std::min<int64_t>(65535, panels - y0)), dim3(256), 0, s, p, per);
     }
     RBG_HIP(hipGetLastError());
     return RBG_OK;
 }
 
 // 2 KB of a row per tile where that leaves every CU work; else 512 bytes: four times the workgroups.
-template <class TO, int KS>
+template <class TO, class TU, int KS>
 static int launch_short(const ScoreArgs &a, hipStream_t s) {
     const int64_t panels = (a.B + 31) / 32, lines = (a.n * (int64_t)sizeof(TO) + 2047) / 2048;
-    return panels * lines >= 1024 ? launch_short<TO, KS, 2048>(a, 512, s) : launch_short<TO, KS, 512>(a, 1024, s);
+    return panels * lines >= 1024 ? launch_short<TO, TU, KS, 2048>(a, 512, s) : launch_short<TO, TU, KS, 512>(a, 1024, s);
 }
 
 // Few users (B <= 16 UT), or too few scores for the tiles below: 16 x 16 tiles straight from the rows, no staging: a wave's load touches
@@ -520,14 +567,13 @@ static int launch_tiles(const ScoreArgs &a, hipStream_t s) {
     return RBG_OK;
 }
 
-// TU: as in score_i8_few_kernel.
+// TU other than void: rows of users to be made into codes on the way, few ones or short ones.
 template <class TO, class TU>
 static int launch_score_items(const ScoreArgs &a, hipStream_t s) {
-    if constexpr (!std::is_void_v<TU>) return launch_few<TO, TU, 1>(a, s);
-    if (a.B <= 16) return launch_few<TO, void, 1>(a, s);
-    if (a.kc <= 4) return launch_short<TO, 2>(a, s);
-    if (a.kc <= 8) return launch_short<TO, 4>(a, s);
-    if (a.kc <= 16 && a.B * a.n * (int64_t)sizeof(TO) >= 128 << 20) return launch_short<TO, 8>(a, s);  // (4096 x 40 001 x 256: 197 us, 237 in tiles; 100 x 100 001 x 200: 40 and 22)
+    if (a.B <= 16) return launch_few<TO, TU, 1>(a, s);
+    if (a.kc <= 4) return launch_short<TO, TU, 2>(a, s);
+    if (a.kc <= 8 || !std::is_void_v<TU>) return launch_short<TO, TU, 4>(a, s);
+    if (a.kc <= 16 && a.B * a.n * (int64_t)sizeof(TO) >= 128 << 20) return launch_short<TO, void, 8>(a, s);  // (4096 x 40 001 x 256: 197 us, 237 in tiles; 100 x 100 001 x 200: 40 and 22)
     const int64_t wide = ((a.n + 255) / 256) * ((a.B + 255) / 256), small = ((a.n + 127) / 128) * ((a.B + 127) / 128);
     // 64 x 16 tiles with K over four waves, many times the workgroups (300 x 300 x 8 192: 31 us against 51; 1 000 x 1 000 x 1 024: 19 against 16)
     if (small <= 32 && a.kc >= 128) return launch_few<TO, void, 4>(a, s);
@@ -549,6 +595,14 @@ static int launch_score(const ScoreArgs &a, hipStream_t s) {
 
 // Bytes between the rows of codes that a call makes for itself.
 static int64_t own_stride(int64_t K) { return (K + 127) / 128 * 128; }
+
+// Whether the product's workgroups make the users' codes themselves, in one launch.  Up to 16 users: kOwnCodes.  Rows of up to 128 values of
+// more users, against codes made first: 100 x 1 000 x 100 fp16 9.8 us a call and 12.7, 4 096 x 40 982 x 128 bf16 112 and 118, x 64 fp32 140 and
+// 141; but x 128 fp32 148 and 144, 600 x 5 000 x 127 fp32 13.3 and 13.0: every workgroup reads its 32 rows before its first product.
+static bool makes_codes(int64_t B, int64_t n, int64_t K, int size) {
+    if (B <= 16) return B * K <= kOwnCodes;
+    return K <= 128 && (K * size <= 256 || B * n <= 1 << 21);
+}
 
 constexpr int64_t kMaxStride = 1 << 23;  // 32-bit offsets inside a tile
 constexpr int64_t kMaxK = 131071;  // 128 x 128 x K < 2^31
@@ -623,7 +677,7 @@ int rbg_score_rows_i8(const void *u, int64_t ldu, int dtype, int64_t B, const in
     const int64_t ldc = own_stride(K);
     int8_t *qu = (int8_t *)workspace;
     float *su = (float *)(qu + B * ldc);
-    if (B <= 16 && B * K <= kOwnCodes) {
+    if (makes_codes(B, n, K, elem_size(dtype))) {
         const ScoreArgs a{nullptr, qi, ldu, ldi, nullptr, si, B, n, (int)((K + 15) / 16), S, lds, u, (int)K};
         return with_elem(out_dtype, [&](auto o) {
             return with_elem(dtype, [&](auto t) { return launch_score<decltype(o), decltype(t)>(a, (hipStream_t)stream); });

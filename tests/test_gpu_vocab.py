@@ -876,3 +876,22 @@ def test_embedding_grad_rows_between_long_runs(rbg, cuda, dtype, n, rows, d):
     ref, mag, cnt = runs_reference(grad, ids, rows, 1.0, -1)
     within(got, ref, stored(ref, dtype) + mag * U * (cnt + 4))  # cnt additions in some order
     assert torch.all(got[cnt[:, 0] == 0] == 0)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("b,n", [(17, 40), (33, 1000), (100, 3000), (300, 9001), (2097153, 2)])
+def test_scores_of_short_rows(rbg, cuda, dtype, b, n):
+    """Users' rows of up to 128 values, whose codes the product makes on the way: those of quantize_rows, to the bit; a zero row scores
+    zero, one that is not finite scores NaN."""
+    for k in (1, 15, 16, 17, 32, 33, 63, 64, 65, 100, 127, 128, 129) if b < 1000 else (5,):
+        g = gen(b + k, cuda)
+        u = torch.randn(b, k + 3, generator=g, device=cuda).to(dtype)[:, :k]
+        u[1] = 0
+        u[2, k - 1], u[b - 1, 0] = math.inf, math.nan
+        codes, scales = rbg.quantize_rows(torch.randn(n, k, generator=g, device=cuda))
+        qu, su = rbg.quantize_rows(u)
+        sums = qu.double() @ codes.double().t().contiguous()
+        ref = sums.float() * su[:, None] * scales  # exact sums, then the two products in the order the operator takes them
+        assert torch.isnan(ref[2]).all() and torch.isnan(ref[b - 1]).all() and (ref[1] == 0).all()
+        got = rbg.score_int8(u, codes, scales)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.nan_to_num(), ref.nan_to_num()), k
