@@ -796,9 +796,9 @@ static int check_grad(const void *z, int64_t ldz, int dtype, int64_t n, int64_t 
     return RBG_OK;
 }
 
+// S: row_parts of the whole call, which its workspace is sized for (a call's last slice of rows may be short).
 template <class T>
-static int launch_distill_rows(const DistillArgs &a, int64_t n, int64_t V, hipStream_t s) {
-    const int S = row_parts(n, V);
+static int launch_distill_rows(const DistillArgs &a, int64_t n, int64_t V, int S, hipStream_t s) {
     if (S > 1) {
         hipLaunchKernelGGL((distill_part_kernel<T, 256>), dim3(S, (unsigned)n), dim3(256), 0, s, a);
         hipLaunchKernelGGL((distill_grad_kernel<T, 256, true>), dim3(S, (unsigned)n), dim3(256), 0, s, a);
@@ -823,21 +823,20 @@ static int launch_distill_rows(const DistillArgs &a, int64_t n, int64_t V, hipSt
 }
 
 template <class T>
-static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, hipStream_t s) {
+static int launch_distill(const DistillArgs &a, int64_t n, int64_t V, int S, hipStream_t s) {
     for (int64_t r0 = 0; r0 < n; r0 += kRowsPerLaunch) {
         DistillArgs p = a;
         p.z = (const T *)a.z + r0 * a.ldz, p.idx += r0 * a.k, p.val += r0 * a.k, p.loss += r0;
         if (a.row_w) p.row_w += r0;
         if (a.stats) p.stats += 2 * r0;
         if (a.grad) p.grad = (T *)a.grad + r0 * a.ldg;
-        if (int rc = launch_distill_rows<T>(p, std::min(kRowsPerLaunch, n - r0), V, s)) return rc;
+        if (int rc = launch_distill_rows<T>(p, std::min(kRowsPerLaunch, n - r0), V, S, s)) return rc;
     }
     return RBG_OK;
 }
 
 template <class T>
-static int launch_logp_rows(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
-    const int S = row_parts(m, V);
+static int launch_logp_rows(const LogpArgs &a, int64_t m, int64_t V, int S, hipStream_t s) {
     if (S > 1) {
         hipLaunchKernelGGL((logp_kernel<T, 256, true>), dim3(S, (unsigned)m), dim3(256), 0, s, a);
         hipLaunchKernelGGL((logp_join_kernel<T>), dim3((unsigned)m), dim3(64), 0, s, a, S);
@@ -852,6 +851,7 @@ static int launch_logp_rows(const LogpArgs &a, int64_t m, int64_t V, hipStream_t
 
 template <class T>
 static int launch_logp(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
+    const int S = row_parts(m, V);  // the whole call's, as its workspace
     for (int64_t r0 = 0; r0 < m; r0 += kRowsPerLaunch) {
         LogpArgs p = a;
         p.z = (const T *)a.z + r0 * a.ldz, p.targets += r0;
@@ -859,7 +859,7 @@ static int launch_logp(const LogpArgs &a, int64_t m, int64_t V, hipStream_t s) {
         if (a.logp64) p.logp64 += r0;
         if (a.coef) p.coef += r0;
         if (a.stats) p.stats += 2 * r0;
-        if (int rc = launch_logp_rows<T>(p, std::min(kRowsPerLaunch, m - r0), V, s)) return rc;
+        if (int rc = launch_logp_rows<T>(p, std::min(kRowsPerLaunch, m - r0), V, S, s)) return rc;
     }
     return RBG_OK;
 }
@@ -932,7 +932,7 @@ int rbg_distill_topk(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V
     const int S = row_parts(n, V);
     DistillArgs a{z, ldz, (int)V, k, idx, val, (float)(1.4426950408889634 / (double)T), T, row_w, loss, stats, grad, ldg, (MaxSum *)workspace,
                   (float *)((char *)workspace + round16(n * S * (int64_t)sizeof(MaxSum)))};
-    return with_elem(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, V, (hipStream_t)stream); });
+    return with_elem(dtype, [&](auto t) { return launch_distill<decltype(t)>(a, n, V, S, (hipStream_t)stream); });
 }
 
 int rbg_distill_topk_backward(const void *z, int64_t ldz, int dtype, int64_t n, int64_t V, const int64_t *idx, const float *val, int k,

@@ -895,3 +895,29 @@ def test_scores_of_short_rows(rbg, cuda, dtype, b, n):
         assert torch.isnan(ref[2]).all() and torch.isnan(ref[b - 1]).all() and (ref[1] == 0).all()
         got = rbg.score_int8(u, codes, scales)
         assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.nan_to_num(), ref.nan_to_num()), k
+
+
+def test_a_last_slice_of_few_long_rows(rbg, cuda):
+    """2^21 + 3 rows of 8 192 logits: the three rows that a launch of their own takes are not split as three rows alone would be (the call has
+    no workspace for that), and come out as the same rows in a call of 1 000."""
+    few, v = 1000, 8192
+    z, idx, val, w = distill_inputs(5, few, v, 4, BF16, cuda)
+    y = torch.randint(-1, v, (few,), generator=gen(6, cuda), device=cuda)
+    at = torch.arange(MANY, device=cuda) % few
+    many = z[at]  # 34 GB
+    logp = rbg.token_logp(many, y[at])
+    assert torch.equal(logp, rbg.token_logp(z, y)[at])
+    one, one_grad = rbg.distill_topk_grad(z, idx, val, row_weight=w)
+    assert torch.equal(rbg.distill_topk(many, idx[at], val[at]), one[at])
+    loss, grad = rbg.distill_topk_grad(many, idx[at], val[at], row_weight=w[at])
+    assert torch.equal(loss, one[at]) and torch.equal(grad[-5 * few:], one_grad[at[-5 * few:]]) and torch.equal(grad[:few], one_grad)
+    del grad
+    # pairs of whole blocks of `few` tokens but for the last, which holds what is left
+    cuts = torch.cat([torch.arange(0, MANY, few, device=cuda)[:2 * (MANY // (2 * few))], torch.tensor([MANY], device=cuda)])
+    sums = torch.stack([part.double().sum() for part in logp.split((cuts[1:] - cuts[:-1]).tolist())])
+    loss, margin, grad = rbg.preference_grad(many, y[at], cuts, sums.float(), beta=0.5)
+    want = 0.5 * ((sums[0::2] - sums[0::2].float().double()) - (sums[1::2] - sums[1::2].float().double()))
+    # logp is rounded to 32 bits out of the call and not in it: half a step of each, in up to 2 few + few tokens of a pair
+    step = (2 * U) * logp.abs().max().double()
+    within(margin, want, 0.5 * 3.2 * few * step / 2 + 2 * U * want.abs())
+    assert grad.shape == many.shape and bool(torch.isfinite(grad[-few:]).all()) and torch.all(grad[-few:][y[at[-few:]] < 0] == 0)
