@@ -735,8 +735,8 @@ int rbg_token_logp_backward(const void *z, int64_t ldz, int dtype, int64_t m, in
  * sums to 0); sequence 2 i is pair i's preferred one, 2 i + 1 the other; ref[s] is the reference model's sum.
  *   margin[i] = beta ((sum logp of 2 i - ref[2 i]) - (sum logp of 2 i + 1 - ref[2 i + 1]))
  *   loss[i]   = -(1 - smoothing) log sigmoid(margin[i]) - smoothing log sigmoid(-margin[i])          0 <= smoothing <= 1
- * The sums are held in 64 bits: a margin is a small difference of large sums.
- * backward: grad_logp [m] from margin and the gradients g_loss, g_margin [pairs] (either may be NULL); zeros outside the sequences.
+ * Sums, margin, loss and its derivative are held in 64 bits and rounded once each: a margin is a small difference of large sums.
+ * backward: grad_logp [m] at the margin that the forward call stored (in 32 bits) and the gradients g_loss, g_margin [pairs] (either may be NULL); zeros outside the sequences.
  * Offsets outside [0, m] are clamped. */
 int rbg_preference_loss(const float *logp, int64_t m, const int64_t *offsets, int64_t pairs, const float *ref, float beta, float smoothing,
                         float *loss, float *margin, void *stream);

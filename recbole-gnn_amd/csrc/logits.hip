@@ -577,18 +577,22 @@ __global__ __launch_bounds__(TH) void logp_grad_kernel(const void *z, int64_t ld
     grad_row<T, TH>(z, ldz, V, targets, stats, row, row_g[row], g, ldg, blockIdx.x, gridDim.x);
 }
 
-__device__ __forceinline__ float sigmoid_d(float h, float smoothing) {  // d loss / d margin
-    return smoothing / (1.f + expf(-h)) - (1.f - smoothing) / (1.f + expf(h));
+// A pair's margin h, its loss and d loss / d h are held in 64 bits and rounded once each: they are few, and a margin rounded to 32 bits costs
+// a loss of exp(-h) |h| steps.  With t = exp(-|h|): sigmoid(|h|) = 1 / (1 + t), sigmoid(-|h|) = t / (1 + t).
+__device__ __forceinline__ double sigmoid_d(double h, double smoothing) {  // d loss / d margin
+    const double t = exp(-fabs(h)), r = 1.0 / (1.0 + t);
+    const double up = h < 0.0 ? t * r : r, down = h < 0.0 ? r : t * r;  // sigmoid(h), sigmoid(-h)
+    return smoothing * up - (1.0 - smoothing) * down;
 }
 
 // -log sigmoid(x) = max(-x, 0) + log(1 + exp(-|x|)); a term of weight 0 is left out (its value may be infinite).
-__device__ __forceinline__ void store_pair(float h, float smoothing, float *loss, float *margin) {
-    const float l = log1pf(expf(-fabsf(h)));
-    float v = 0.f;
-    if (smoothing < 1.f) v += (1.f - smoothing) * (fmaxf(-h, 0.f) + l);
-    if (smoothing > 0.f) v += smoothing * (fmaxf(h, 0.f) + l);
-    *loss = h != h ? h : v;
-    *margin = h;
+__device__ __forceinline__ void store_pair(double h, double smoothing, float *loss, float *margin) {
+    const double l = log1p(exp(-fabs(h)));
+    double v = 0.0;
+    if (smoothing < 1.0) v += (1.0 - smoothing) * (fmax(-h, 0.0) + l);
+    if (smoothing > 0.0) v += smoothing * (fmax(h, 0.0) + l);
+    *loss = (float)(h != h ? h : v);
+    *margin = (float)h;
 }
 
 __device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_t m, int64_t &lo, int64_t &hi) {
@@ -599,7 +603,7 @@ __device__ __forceinline__ void seq_of(const int64_t *offsets, int64_t s, int64_
 
 // The margin of a pair, by the TH threads of a workgroup: both sequences as one list of tokens, 4 TH in flight, both sums in 64 bits.
 template <class L, int TH>
-__device__ __forceinline__ float pair_margin(const L *logp, int64_t m, const int64_t *offsets, const float *ref, int64_t i, float beta,
+__device__ __forceinline__ double pair_margin(const L *logp, int64_t m, const int64_t *offsets, const float *ref, int64_t i, float beta,
                                              int64_t (&lo)[2], int64_t (&hi)[2], double (&red)[2][TH / kWave]) {
     seq_of(offsets, 2 * i, m, lo[0], hi[0]);
     seq_of(offsets, 2 * i + 1, m, lo[1], hi[1]);
@@ -635,7 +639,7 @@ __device__ __forceinline__ float pair_margin(const L *logp, int64_t m, const int
             for (int q = 1; q < TH / kWave; ++q) sum[k] += red[k][q];
         }
     }
-    return (float)((double)beta * ((sum[0] - (double)r0) - (sum[1] - (double)r1)));
+    return (double)beta * ((sum[0] - (double)r0) - (sum[1] - (double)r1));
 }
 
 // One workgroup per pair: the loss, and (COEF) the tokens' gradients of pair_w loss.  Bound by latency (4 096 tokens of 32 pairs 5 us,
@@ -646,10 +650,10 @@ __global__ __launch_bounds__(256) void pair_kernel(const L *logp, int64_t m, con
     __shared__ double red[2][4];
     const int64_t i = blockIdx.x;
     int64_t lo[2], hi[2];
-    const float h = pair_margin<L, 256>(logp, m, offsets, ref, i, beta, lo, hi, red);
+    const double h = pair_margin<L, 256>(logp, m, offsets, ref, i, beta, lo, hi, red);
     if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
     if constexpr (COEF) {
-        const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
+        const float d = (float)((double)beta * sigmoid_d(h, smoothing) * (pair_w ? (double)pair_w[i] : 1.0));
 #pragma unroll
         for (int k = 0; k < 2; ++k)
             for (int64_t t = lo[k] + threadIdx.x; t < hi[k]; t += 256) coef[t] = k ? -d : d;
@@ -670,7 +674,7 @@ __global__ __launch_bounds__(TH) void pair_rows_kernel(const LogpArgs a, int64_t
     if (blockIdx.y >= m) {
         if (blockIdx.x) return;
         const int64_t i = blockIdx.y - m;
-        const float h = pair_margin<double, TH>(a.logp64, m, offsets, ref, i, beta, lo, hi, red);
+        const double h = pair_margin<double, TH>(a.logp64, m, offsets, ref, i, beta, lo, hi, red);
         if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
         return;
     }
@@ -682,8 +686,8 @@ __global__ __launch_bounds__(TH) void pair_rows_kernel(const LogpArgs a, int64_t
             before += __popcll(__ballot(c <= 2 * pairs && offsets[min(c, 2 * pairs)] <= row));
         if (before > 0 && before <= 2 * pairs) {
             const int64_t i = (before - 1) >> 1;
-            const float h = pair_margin<double, TH>(a.logp64, m, offsets, ref, i, beta, lo, hi, red);
-            const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
+            const double h = pair_margin<double, TH>(a.logp64, m, offsets, ref, i, beta, lo, hi, red);
+            const float d = (float)((double)beta * sigmoid_d(h, smoothing) * (pair_w ? (double)pair_w[i] : 1.0));
             w = (before - 1) & 1 ? -d : d;
         }
     }
@@ -725,9 +729,9 @@ __global__ __launch_bounds__(1024) void pair_small_kernel(const LogpArgs a, int6
         for (int q = 0; q < 16; ++q) sum[k] += red[k][q];
         sum[k] -= (double)ref[2 * i + k];
     }
-    const float h = (float)((double)beta * (sum[0] - sum[1]));
+    const double h = (double)beta * (sum[0] - sum[1]);
     if (threadIdx.x == 0) store_pair(h, smoothing, loss + i, margin + i);
-    const float d = beta * sigmoid_d(h, smoothing) * (pair_w ? pair_w[i] : 1.f);
+    const float d = (float)((double)beta * sigmoid_d(h, smoothing) * (pair_w ? (double)pair_w[i] : 1.0));
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         for (int64_t row = lo[k] + w; row < hi[k]; row += 16)
@@ -746,7 +750,7 @@ __global__ __launch_bounds__(256) void pair_grad_kernel(const float *margin, int
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= m) return;
     int64_t lo = 0, hi = 2 * pairs;  // offsets[lo] <= t < offsets[hi], if t is in a sequence
-    float v = 0.f;
+    double v = 0.0;
     if (offsets[0] <= t && t < offsets[hi]) {
         while (hi - lo > 1) {
             const int64_t mid = (lo + hi) >> 1;
@@ -754,11 +758,11 @@ __global__ __launch_bounds__(256) void pair_grad_kernel(const float *margin, int
             else hi = mid;
         }
         const int64_t i = lo >> 1;
-        if (g_loss) v += g_loss[i] * sigmoid_d(margin[i], smoothing);
-        if (g_margin) v += g_margin[i];
-        v *= lo & 1 ? -beta : beta;
+        if (g_loss) v += (double)g_loss[i] * sigmoid_d(margin[i], smoothing);
+        if (g_margin) v += (double)g_margin[i];
+        v *= lo & 1 ? -(double)beta : (double)beta;
     }
-    grad[t] = v;
+    grad[t] = (float)v;
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------

@@ -921,3 +921,42 @@ def test_a_last_slice_of_few_long_rows(rbg, cuda):
     step = (2 * U) * logp.abs().max().double()
     within(margin, want, 0.5 * 3.2 * few * step / 2 + 2 * U * want.abs())
     assert grad.shape == many.shape and bool(torch.isfinite(grad[-few:]).all()) and torch.all(grad[-few:][y[at[-few:]] < 0] == 0)
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.3, 1.0])
+@pytest.mark.parametrize("pairs,each", [(4, 1), (32, 4), (100, 5), (300, 2)])
+def test_preference_is_rounded_once(rbg, cuda, smoothing, pairs, each):
+    """Rows of two equal logits: a token's log-probability is -log 2 in 64 bits, its softmax 1/2 exactly, and its gradient half the pair's
+    coefficient.  Margin, loss and coefficient then show their own rounding alone, half a step (and what 64 bits lose, below 2^-40):
+    in the one launch of few tokens, in the pairs that the rows' workgroups form, and in the pairs' own launch."""
+    g = gen(pairs, cuda)
+    m = 2 * pairs * each
+    beta, e = 0.75, float(torch.tensor(smoothing, dtype=F32))  # (the operator takes 32 bits)
+    h = torch.linspace(-30, 30, pairs, device=cuda)
+    ref = torch.stack([-h / beta, torch.rand(pairs, generator=g, device=cuda)], 1).view(-1)
+    weight = torch.rand(pairs, generator=g, device=cuda) + 0.5
+    h = beta * (ref[1::2].double() - ref[0::2].double())  # (both sequences of a pair sum to the same)
+    offsets = torch.arange(2 * pairs + 1, device=cuda) * each
+    y = torch.zeros(m, dtype=torch.int64, device=cuda)
+    want = (1 - e) * (-h).clamp(min=0) + e * h.clamp(min=0) + torch.exp(-h.abs()).log1p()
+    d = e * torch.sigmoid(h) - (1 - e) * torch.sigmoid(-h)
+    once = U + 2.0 ** -40
+    loss, margin, grad = rbg.preference_grad(torch.zeros(m, 2, device=cuda), y, offsets, ref, beta=beta, label_smoothing=smoothing, pair_weight=weight)
+    within(margin, h, once * h.abs())
+    within(loss, want, once * want)
+    coef = (beta * d * weight.double())[:, None, None] * torch.tensor([1.0, -1.0], device=cuda)[None, :, None]
+    half = coef.expand(pairs, 2, each).reshape(m) / 2
+    # e sigma(h) - (1 - e) sigma(-h) cancels near a margin of log((1 - e) / e): off by 64 bits' rounding of its terms
+    tol = once * half.abs() + 2.0 ** -48
+    within(grad[:, 0], half, tol)
+    within(grad[:, 1], -half, tol)
+    # from given log-probabilities; backward from the margin that came out
+    logp = torch.zeros(m, device=cuda, requires_grad=True)
+    loss, margin = rbg.preference_loss(logp, offsets, ref, beta=beta, label_smoothing=smoothing)
+    within(margin.detach(), h, once * h.abs())
+    within(loss.detach(), want, once * want)
+    loss.backward(weight)
+    h = margin.detach().double()
+    d = e * torch.sigmoid(h) - (1 - e) * torch.sigmoid(-h)
+    coef = (beta * d * weight.double())[:, None, None] * torch.tensor([1.0, -1.0], device=cuda)[None, :, None]
+    within(logp.grad, coef.expand(pairs, 2, each).reshape(m), once * coef.abs().expand(pairs, 2, each).reshape(m) + 2.0 ** -47)
