@@ -4,6 +4,9 @@ arithmetic is in 32 bits and an output is rounded once.  GPU tensors only; calls
 
 An id, target or list entry outside its range (-1 is the usual "none") reads nothing and adds to nothing: the library cannot raise
 for values that live on the device.
+
+Gradients are those of reverse mode, once: gradients of gradients and forward mode raise.  The calls that return a gradient, and those in
+8 bits, take their inputs as constants.
 """
 from __future__ import annotations
 
@@ -11,6 +14,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -67,6 +71,12 @@ def _like(t, of, name, shape, dtype):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _differentiated(t):
+    """Whether a call on ``t`` goes through its autograd function: a gradient may be asked for, or forward mode is on, where a tensor with a
+    tangent is refused there (the functions have no forward-mode formula) instead of losing it."""
+    return t.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -107,7 +117,7 @@ def _padding(padding_idx, n_rows):
 def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=None):
     """The gradient of :func:`embedding`'s table: ``out[v] = scale * sum of grad[i] over ids[i] == v`` as a dense [n_rows, d] tensor of
     ``out_dtype`` (``grad``'s type, the default, or float32), zeros where no id refers to a row and in row ``padding_idx`` (counted from the end when negative).  The
-    places are sorted by id and summed in ascending order in 32 bits: the same bits from run to run."""
+    places are sorted by id and summed in ascending order in 32 bits: the same bits from run to run.  Not differentiable itself."""
     if not grad.is_cuda:
         raise RuntimeError("grad must live on the GPU (the HIP engine has no CPU path)")
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
@@ -149,7 +159,7 @@ def embedding(table, ids, scale=1.0, padding_idx=None):
     table = _rows(table, "table")
     ids = _like(ids, table, "ids", tuple(ids.shape), torch.int64)
     _padding(padding_idx, table.shape[0])
-    if table.requires_grad and torch.is_grad_enabled():
+    if _differentiated(table):
         return _Embedding.apply(table, ids, float(scale), padding_idx)
     return _embedding(table, ids, float(scale))
 
@@ -204,7 +214,7 @@ def distill_topk(logits, teacher_idx, teacher_val, temperature=1.0):
     k <= 256."""
     logits = _rows(logits, "logits")
     idx, val = _teacher(logits, teacher_idx, teacher_val)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _differentiated(logits):
         return _DistillTopk.apply(logits, idx, val, float(temperature))
     return _distill(logits, idx, val, float(temperature), None, False, False)[0]
 
@@ -333,7 +343,8 @@ def _quantize(x, pad):
 def quantize_rows(x):
     """``(codes [n, K] int8, scale [n] float32)`` of the rows of ``x``: ``scale = max|row| / 127``, ``codes = round(row / scale)`` in
     [-127, 127].  A zero row has scale 0; one that holds an infinity or NaN has scale NaN (and its scores are NaN).  The codes
-    are a view of rows padded with zeros to a multiple of 64 bytes, the layout :func:`score_int8` reads without a copy."""
+    are a view of rows padded with zeros to a multiple of 64 bytes, the layout :func:`score_int8` reads without a copy.  No gradient
+    flows through it."""
     x = _rows(x, "x")
     if x.shape[1] == 0:
         raise ValueError("rows must have at least one column")
@@ -358,7 +369,7 @@ def _codes(codes, k):
 def score_int8(u, codes, scales, out_dtype=torch.float32):
     """Scores [B, n] of the rows ``u`` [B, K] (float32, bfloat16 or float16) against a table in 8 bits (``codes`` [n, K], ``scales`` [n], as
     :func:`quantize_rows` makes them once): ``u`` is quantized row by row in the call, the products are summed exactly in 32-bit integers,
-    and ``out_dtype`` is rounded to once.  The 8-bit form of :func:`ops.score` (lightgcn.py:131).  K <= 131071."""
+    and ``out_dtype`` is rounded to once.  No gradient flows through it.  The 8-bit form of :func:`ops.score` (lightgcn.py:131).  K <= 131071."""
     u = _rows(u.detach(), "u")
     b, k = u.shape
     if codes.dim() != 2 or codes.dtype != torch.int8:

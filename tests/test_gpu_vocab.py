@@ -960,3 +960,22 @@ def test_preference_is_rounded_once(rbg, cuda, smoothing, pairs, each):
     d = e * torch.sigmoid(h) - (1 - e) * torch.sigmoid(-h)
     coef = (beta * d * weight.double())[:, None, None] * torch.tensor([1.0, -1.0], device=cuda)[None, :, None]
     within(logp.grad, coef.expand(pairs, 2, each).reshape(m), once * coef.abs().expand(pairs, 2, each).reshape(m) + 2.0 ** -47)
+
+
+def test_forward_mode_is_refused(rbg, cuda):
+    """A tangent is refused by every differentiable operator, never dropped; values inside a forward-mode level are what they are outside."""
+    from torch.autograd import forward_ad
+    g = gen(3, cuda)
+    t, dt = torch.randn(6, 8, generator=g, device=cuda), torch.randn(6, 8, generator=g, device=cuda)
+    ids, offsets, ref = torch.arange(6, device=cuda), torch.tensor([0, 3, 6], device=cuda), torch.zeros(2, device=cuda)
+    calls = [lambda x: rbg.embedding(x, ids, scale=2.0), lambda x: rbg.distill_topk(x, ids[:, None], t[:, :1]), lambda x: rbg.token_logp(x, ids),
+             lambda x: rbg.preference_loss(x[:, 0].contiguous(), offsets, ref)[0]]
+    want = [call(t) for call in calls]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t, dt)
+        for call, value in zip(calls, want):
+            assert torch.equal(call(t), value)
+            for grad_mode in (True, False):
+                with torch.set_grad_enabled(grad_mode), pytest.raises((RuntimeError, NotImplementedError)):
+                    call(dual)
+    assert all(torch.equal(call(t), value) for call, value in zip(calls, want))
