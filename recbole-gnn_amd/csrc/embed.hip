@@ -56,8 +56,9 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T *__restrict__ table
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (i0 + r >= n) break;
+            const float s = id[r] >= 0 && id[r] < n_rows ? scale : 0.f;  // (zeros stay zeros whatever the scale)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[r].v[e] = from_f32<T>(scale * to_f32(v[r].v[e]));
+            for (int e = 0; e < VEC; ++e) v[r].v[e] = from_f32<T>(s * to_f32(v[r].v[e]));
             store_any(out + (i0 + r) * ldo + c, v[r]);
         }
     }

@@ -979,3 +979,15 @@ def test_forward_mode_is_refused(rbg, cuda):
                 with torch.set_grad_enabled(grad_mode), pytest.raises((RuntimeError, NotImplementedError)):
                     call(dual)
     assert all(torch.equal(call(t), value) for call, value in zip(calls, want))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("d", [3, 64, 520])
+def test_embedding_of_no_row_is_zero_at_any_scale(rbg, cuda, dtype, d):
+    """1e39 and more are infinite in the operator's 32 bits: rows are scaled to infinities, places without a row stay zero."""
+    ids = torch.tensor([0, -1, 4, 5, 1 << 40, 2], device=cuda)
+    there = torch.tensor([True, False, True, False, False, True], device=cuda)
+    for scale in (1e39, -math.inf, math.nan, -1.0):
+        out = rbg.embedding(torch.ones(5, d, dtype=dtype, device=cuda), ids, scale=scale)
+        assert torch.all(out[~there] == 0)
+        assert bool(out[there].isnan().all()) if math.isnan(scale) else torch.all(out[there] == scale)
