@@ -149,6 +149,30 @@ struct ScoreArgs {
     int K;
 };
 
+// acc su si in 32 bits.  acc < 2^31, so acc su may pass the type's end, where the score need not, for su > 2^96 alone: such a scale goes in two
+// parts (powers of two: the same roundings).  FAR: some scale of the wave's users is one.  (Two parts for every user: 110 -> 118 us at
+// 4 096 x 40 982 x 128 bf16; chosen by wave 110.)
+constexpr float kFarScale = 0x1p96f;
+template <bool FAR>
+__device__ __forceinline__ float score_of(int acc, float su, float si) {
+    if constexpr (!FAR) return (float)acc * su * si;
+    asm volatile("" : "+v"(su));  // (or the parts of every row's scale are made ahead and kept in registers)
+    const bool far = su > kFarScale;
+    return (float)acc * (far ? su * 0x1p-64f : su) * si * (far ? 0x1p64f : 1.f);
+}
+template <int N>
+__device__ __forceinline__ bool any_far(const float (&su)[N]) {  // on any lane of the wave
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) far |= su[i] > kFarScale;
+    return __ballot(far) != 0;
+}
+template <class F>
+__device__ __forceinline__ void by_far(bool far, F f) {
+    if (far) f(std::true_type{});
+    else f(std::false_type{});
+}
+
 // The codes of a row that two lanes share, h the even 16-byte chunks or the odd ones, from its K values; its scale.
 template <class TU, int KS>
 __device__ __forceinline__ float own_codes(const TU *x, int K, int h, i32x4 (&codes)[KS]) {
@@ -236,6 +260,7 @@ __global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel
     // the scores of a row's last piece of a line: LINE of them from (threadIdx.x / (LINE / KEEP)), KEEP for each thread
     constexpr int KEEP = 32 * LINE / 256;
     const unsigned krow = threadIdx.x / (LINE / KEEP), kcol = threadIdx.x % (LINE / KEEP) * KEEP;
+    const bool far = any_far(su);  // (the same rows in all four waves)
     fetch(t0 * (TILE / 128));
     for (int64_t t = t0; t < t1; ++t) {
 #pragma unroll
@@ -246,7 +271,11 @@ __global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel
             const float sj = si;
             if (u + 1 < TILE / 128 || t + 1 < t1) fetch(t * (TILE / 128) + u + 1);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) buf[at[r] + u * 128] = from_f32<TO>((float)acc[r] * su[r] * sj);
+            for (int r = 0; r < 16; ++r) buf[at[r] + u * 128] = from_f32<TO>(score_of<false>(acc[r], su[r], sj));
+            if (__builtin_expect(far, 0)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) buf[at[r] + u * 128] = from_f32<TO>(score_of<true>(acc[r], su[r], sj));
+            }
         }
         __syncthreads();
         const bool first = t == t0, last = t + 1 == t1;
@@ -385,19 +414,24 @@ __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
                 for (int y = 0; y < IT; ++y) acc[x][y] += part[w + q][x * IT + y][lane];
     }
     TO *S = (TO *)a.S;
+    float sb[UT * 4];
 #pragma unroll
-    for (int y = 0; y < IT; ++y) {
-        const int64_t j = j0 + 16 * y + m;
-        if (j >= a.n) continue;
-        const float si = a.si[j];
+    for (int i = 0; i < UT * 4; ++i) sb[i] = su[min<int64_t>(b0 + 16 * (i / 4) + 4 * g + i % 4, a.B - 1)];
+    by_far(any_far(sb), [&](auto far) {
 #pragma unroll
-        for (int x = 0; x < UT; ++x)
+        for (int y = 0; y < IT; ++y) {
+            const int64_t j = j0 + 16 * y + m;
+            if (j >= a.n) continue;
+            const float si = a.si[j];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t b = b0 + 16 * x + 4 * g + r;
-                if (b < a.B) S[b * a.lds + j] = from_f32<TO>((float)acc[x][y][r] * su[b] * si);
-            }
-    }
+            for (int x = 0; x < UT; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t b = b0 + 16 * x + 4 * g + r;
+                    if (b < a.B) S[b * a.lds + j] = from_f32<TO>(score_of<decltype(far)::value>(acc[x][y][r], sb[4 * x + r], si));
+                }
+        }
+    });
 }
 
 template <class TO, class TU, int UT>
@@ -496,6 +530,10 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void score_i8_tile_kernel(cons
         each([&](auto x) { multiply(g, x); });
         __builtin_amdgcn_sched_barrier(0);
     };
+    float wave_su[(W + 1) / 2];  // of the wave's users, one or two for each lane
+#pragma unroll
+    for (int i = 0; i < (W + 1) / 2; ++i) wave_su[i] = a.su[min<int64_t>(b0 + wu + 64 * i + lane, a.B - 1)];
+    const bool far_users = any_far(wave_su);
     each([&](auto q) { fill(0, q); });
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (steps > 1) each([&](auto q) { fill(1, q); });
@@ -528,13 +566,15 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void score_i8_tile_kernel(cons
 #pragma unroll
     for (int x = 0; x < W; ++x) {
         const int64_t bx = b0 + wu + 32 * x;
+        by_far(far_users, [&](auto far) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = (r & 3) + 8 * (r >> 2) + 4 * h;
-            const float su = a.su[min<int64_t>(bx + row, a.B - 1)];
+            for (int r = 0; r < 16; ++r) {
+                const int row = (r & 3) + 8 * (r >> 2) + 4 * h;
+                const float su = a.su[min<int64_t>(bx + row, a.B - 1)];
 #pragma unroll
-            for (int y = 0; y < W; ++y) strip[row * COLS + 32 * y + m] = from_f32<TO>((float)acc[x][y][r] * su * si[y]);
-        }
+                for (int y = 0; y < W; ++y) strip[row * COLS + 32 * y + m] = from_f32<TO>(score_of<decltype(far)::value>(acc[x][y][r], su, si[y]));
+            }
+        });
         if (inside) {
 #pragma unroll
             for (int q = 0; q < 32 * L / 64; ++q) {

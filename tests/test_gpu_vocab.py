@@ -991,3 +991,21 @@ def test_embedding_of_no_row_is_zero_at_any_scale(rbg, cuda, dtype, d):
         out = rbg.embedding(torch.ones(5, d, dtype=dtype, device=cuda), ids, scale=scale)
         assert torch.all(out[~there] == 0)
         assert bool(out[there].isnan().all()) if math.isnan(scale) else torch.all(out[there] == scale)
+
+
+@pytest.mark.parametrize("b,n,k", [(1, 100, 128), (2, 333, 1100), (16, 40000, 2100), (40, 300, 64), (200, 3000, 100), (100, 500, 128), (33, 300, 300), (300, 300, 8192), (600, 1000, 300),
+                                   (3000, 4200, 200), (4096, 4096, 260)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scores_of_large_users_and_small_items(rbg, cuda, dtype, b, n, k):
+    """Scores that 32 bits hold although a user's scale times the sum passes them (1e36 / 127 times up to 127 x 127 x K): finite in every form."""
+    g = gen(b + n, cuda)
+    u = torch.randn(b, k, generator=g, device=cuda)
+    u[::3] *= 1e36 / u[::3].abs().amax(1, keepdim=True)
+    u[1::3] *= 1e-30
+    u = u.to(dtype)
+    codes, scales = rbg.quantize_rows(torch.randn(n, k, generator=g, device=cuda) * 10.0 ** torch.randint(-30, -5, (n, 1), generator=g, device=cuda))
+    q, s = codes_reference(u)
+    sums = torch.matmul(q.to(cuda), codes.double().t().contiguous())
+    ref = sums * s.to(cuda)[:, None] * scales.double()[None]
+    assert float((sums * s.to(cuda)[:, None]).abs().max()) > torch.finfo(F32).max > float(ref.abs().max()) * 100
+    within(rbg.score_int8(u, codes, scales), ref, 3.1 * U * ref.abs() + stored(ref, F32) + 2.0 ** -148)
