@@ -696,7 +696,7 @@ int rbg_mean_f32(const float *const *srcs, int n_srcs, int64_t n_floats, float s
  * replayed side by side) need one each.  No call allocates or synchronizes; every call can be captured.
  * ------------------------------------------------------------------------------------------- */
 
-/* out[i, :] = scale * table[ids[i], :]   (zeros where ids[i] is outside [0, n_rows)).  Rows of d elements; ldt, ldo >= d; n <= 2^34.
+/* out[i, :] = scale * table[ids[i], :]   (zeros where ids[i] is outside [0, n_rows)).  Rows of d <= 2^30 elements; ldt, ldo >= d; n <= 2^34.
  * The row gather of lightgcn.py:60-68,128 for any element type; out must not overlap table. */
 int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dtype, const int64_t *ids, int64_t n, float scale, void *out,
                   int64_t ldo, void *stream);

@@ -704,13 +704,14 @@ int rbg_embedding(const void *table, int64_t ldt, int64_t n_rows, int d, int dty
     if (!elem_ok(dtype)) return fail(RBG_EINVAL, "dtype = %d", dtype);
     if (n < 0 || n_rows < 0 || d <= 0 || ldt < d || ldo < d)
         return fail(RBG_ESHAPE, "n = %lld, n_rows = %lld, d = %d, ldt = %lld, ldo = %lld", (long long)n, (long long)n_rows, d, (long long)ldt, (long long)ldo);
+    if (d > 1 << 30) return fail(RBG_EUNSUPPORTED, "d = %d: at most 2^30 columns", d);
     if (n > (int64_t)1 << 34) return fail(RBG_EUNSUPPORTED, "n = %lld: at most 2^34 ids", (long long)n);
     constexpr int64_t kIdsPerLaunch = 1 << 26;  // (a grid holds fewer than 2^32 threads per dimension, a workgroup of 256 at least 16 ids)
     if (n == 0) return RBG_OK;
     if ((n_rows && !table) || !ids || !out) return fail(RBG_EINVAL, "NULL pointer");
     const int size = elem_size(dtype);
     if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) % size) return fail(RBG_EINVAL, "a table is not aligned to its type");
-    const bool wide = d * size >= 16;
+    const bool wide = (int64_t)d * size >= 16;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
         constexpr int VEC = 16 / (int)sizeof(E);
@@ -795,7 +796,7 @@ int rbg_embedding_grad(const void *grad, int64_t ldg, int dtype, const int64_t *
     }
     RBG_HIP(hipGetLastError());
     const RunArgs a{grad, ldg, n, n_rows, d, l.chunk, l.chunks, keys, places, scale, out, (float *)(w + l.part), 0, 0};
-    const bool wide = d * size >= 16;
+    const bool wide = (int64_t)d * size >= 16;
     return with_elem(dtype, [&](auto t) {
         typedef decltype(t) E;
         return out_dtype == dtype ? launch_runs_of<E, E>(a, ids, padding_idx, wide, s) : launch_runs_of<E, float>(a, ids, padding_idx, wide, s);

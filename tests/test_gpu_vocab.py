@@ -1009,3 +1009,10 @@ def test_scores_of_large_users_and_small_items(rbg, cuda, dtype, b, n, k):
     ref = sums * s.to(cuda)[:, None] * scales.double()[None]
     assert float((sums * s.to(cuda)[:, None]).abs().max()) > torch.finfo(F32).max > float(ref.abs().max()) * 100
     within(rbg.score_int8(u, codes, scales), ref, 3.1 * U * ref.abs() + stored(ref, F32) + 2.0 ** -148)
+
+
+def test_columns_whose_bytes_pass_31_bits(rbg, cuda):
+    d = (1 << 29) + 3
+    table = (torch.arange(d, device=cuda) % 251).float()[None].repeat(2, 1)
+    out = rbg.embedding(table, torch.tensor([1, -1], device=cuda), scale=2.0)
+    assert torch.equal(out[0], 2 * table[1]) and torch.all(out[1] == 0)

@@ -100,3 +100,9 @@ def test_wrappers_refuse_the_cpu(rbg):
                  lambda: rbg.preference_grad(f, i, i, f[0]), lambda: rbg.quantize_rows(f), lambda: rbg.score_int8(f, i, i)):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+@pytest.mark.parametrize("d", [(1 << 30) + 1, (1 << 31) - 1])
+def test_lookup_refuses_columns_that_its_steps_would_pass(rbg, d):
+    """A kernel's column steps past d by up to 512 elements in 32 bits."""
+    assert embedding(rbg._lib.lib, d=d, ldt=d, ldo=d) == EUNSUPPORTED
