@@ -77,6 +77,13 @@ def _differentiated(t):
     return t.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0
 
 
+def _c_int(n, name):
+    """A size that the C entry takes in 32 bits: ctypes would pass its lower half alone."""
+    if n > 0x7fffffff:
+        raise ValueError(f"{name} = {n} is beyond 2^31 - 1")
+    return n
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -98,7 +105,7 @@ def _workspace(of, fn, *sizes):
 # table rows and their gradient
 # ---------------------------------------------------------------------------------------------------------------------
 def _embedding(table, ids, scale):
-    n, d = ids.numel(), table.shape[1]
+    n, d = ids.numel(), _c_int(table.shape[1], "columns of table")
     out = table.new_empty((*ids.shape, d), dtype=table.dtype)
     if n and d:
         _call(lib.rbg_embedding, table, table.data_ptr(), _ld(table), table.shape[0], d, _DTYPES[table.dtype], ids.data_ptr(), n, scale,
@@ -122,7 +129,7 @@ def embedding_grad(grad, ids, n_rows, scale=1.0, padding_idx=None, out_dtype=Non
         raise RuntimeError("grad must live on the GPU (the HIP engine has no CPU path)")
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         raise ValueError(f"grad must be {(*ids.shape, 'd')}, got {tuple(grad.shape)}")
-    d = grad.shape[-1]
+    d = _c_int(grad.shape[-1], "columns of grad")
     grad = _rows(grad.reshape(ids.numel(), d) if grad.dim() != 2 else grad, "grad")
     ids = _like(ids, grad, "ids", tuple(ids.shape), torch.int64)
     padding_idx = _padding(padding_idx, n_rows)
@@ -171,6 +178,7 @@ def _teacher(logits, idx, val):
     n = logits.shape[0]
     if idx.dim() != 2 or idx.shape[0] != n:
         raise ValueError(f"teacher_idx must be [{n}, k], got {tuple(idx.shape)}")
+    _c_int(idx.shape[1], "k")
     return (_like(idx, logits, "teacher_idx", tuple(idx.shape), torch.int64),
             _like(val, logits, "teacher_val", tuple(idx.shape), torch.float32))
 

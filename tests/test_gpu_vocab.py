@@ -1016,3 +1016,12 @@ def test_columns_whose_bytes_pass_31_bits(rbg, cuda):
     table = (torch.arange(d, device=cuda) % 251).float()[None].repeat(2, 1)
     out = rbg.embedding(table, torch.tensor([1, -1], device=cuda), scale=2.0)
     assert torch.equal(out[0], 2 * table[1]) and torch.all(out[1] == 0)
+
+
+def test_columns_beyond_32_bits_are_refused(rbg, cuda):
+    """Widths whose lower 32 bits are a small size are not taken for it."""
+    wide = torch.empty(1, (1 << 32) + 8, dtype=BF16, device=cuda)
+    ids = torch.zeros(1, dtype=torch.int64, device=cuda)
+    for call in (lambda: rbg.embedding(wide, ids), lambda: rbg.embedding_grad(wide, ids, 2)):
+        with pytest.raises(ValueError):
+            call()

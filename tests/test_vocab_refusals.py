@@ -106,3 +106,11 @@ def test_wrappers_refuse_the_cpu(rbg):
 def test_lookup_refuses_columns_that_its_steps_would_pass(rbg, d):
     """A kernel's column steps past d by up to 512 elements in 32 bits."""
     assert embedding(rbg._lib.lib, d=d, ldt=d, ldo=d) == EUNSUPPORTED
+
+
+def test_sizes_that_32_bits_would_cut_are_refused(rbg):
+    assert rbg.vocab._c_int(0x7fffffff, "d") == 0x7fffffff
+    with pytest.raises(ValueError, match="k = 4294967297"):
+        rbg.vocab._teacher(torch.empty(1, 4), torch.zeros(1, 1, dtype=torch.int64).expand(1, (1 << 32) + 1), torch.zeros(1, 1).expand(1, (1 << 32) + 1))
+    with pytest.raises(ValueError, match="columns of table"):
+        rbg.vocab._embedding(torch.empty(1, (1 << 32) + 8, device="meta"), torch.zeros(3, dtype=torch.int64), 1.0)
