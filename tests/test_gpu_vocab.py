@@ -1025,3 +1025,45 @@ def test_columns_beyond_32_bits_are_refused(rbg, cuda):
     for call in (lambda: rbg.embedding(wide, ids), lambda: rbg.embedding_grad(wide, ids, 2)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,v", [(40, 50), (600, 700), (1500, 64)])
+@pytest.mark.parametrize("where", ["ends", "all before", "all behind"])
+def test_preference_offsets_outside_in_every_form(rbg, cuda, dtype, m, v, where):
+    """Ascending offsets that begin below 0 and end behind the last token are those offsets clamped, in the one launch of few tokens, in the
+    two of up to 1 024 and in the three beyond; every element of the gradient is written.  Bounds as in test_preference."""
+    g = gen(m, cuda)
+    z, y = torch.randn(m, v, generator=g, device=cuda).to(dtype), torch.randint(-1, v, (m,), generator=g, device=cuda)
+    offsets = {"ends": [-7, m // 5, m // 5, m // 2, m - 3, m + 1, m + 50], "all before": [-(1 << 40), -9, -4, -4, -1, 0, m // 3],
+               "all behind": [m // 3, m, m + 1, m + 1, m + 2, m + 9, 1 << 40]}[where]
+    pairs, beta = 3, 0.5
+    offsets = torch.tensor(offsets, device=cuda)
+    ref = torch.randn(2 * pairs, generator=g, device=cuda)
+    lp, tol, q, e, there = logp_reference(z, y)
+    o = offsets.clamp(0, m)
+    h, th, want_loss, tl, dh, td = preference_reference(lp, tol, o, ref, beta, 0.0)
+    c, tc = torch.zeros(m, dtype=torch.float64, device=cuda), torch.zeros(m, dtype=torch.float64, device=cuda)
+    for s in range(2 * pairs):
+        at = slice(int(o[s]), int(o[s + 1]))
+        c[at], tc[at] = (1 if s % 2 == 0 else -1) * beta * dh[s // 2], beta * (td[s // 2] + 4 * U)
+    c, tc = c * there, tc * there
+    one = torch.zeros_like(q)
+    one[torch.arange(m, device=cuda), torch.where(there, y, 0)] = 1.0
+    want = c[:, None] * (one - q)
+    bound = tc[:, None] * (q + one) + c.abs()[:, None] * (q * (e[:, None] + 4 * U) + 2 * U) + 2.0 ** -125 + stored(want, F32) + stored(want, dtype)
+    lib, b = rbg._lib.lib, ctypes.c_int64()
+    rbg._lib.check(lib.rbg_preference_grad_workspace(m, v, ctypes.byref(b)))
+    work = torch.empty(b.value, dtype=torch.uint8, device=cuda)
+    loss, margin, grad = torch.full((pairs,), 77.0, device=cuda), torch.full((pairs,), 77.0, device=cuda), torch.full((m, v + 3), 77.0, dtype=dtype, device=cuda)
+    rbg._lib.check(lib.rbg_preference_grad(z.data_ptr(), v, rbg.vocab._DTYPES[dtype], m, v, y.data_ptr(), offsets.data_ptr(), pairs, ref.data_ptr(), beta, 0.0, None,
+                                           loss.data_ptr(), margin.data_ptr(), grad.data_ptr(), v + 3, work.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    within(margin, h, th)
+    within(loss, want_loss, tl)
+    within(grad[:, :v], want, bound)
+    assert torch.all(grad[:, v:] == 77.0)
+    logp = lp.float().requires_grad_()
+    got, _ = rbg.preference_loss(logp, offsets, ref, beta=beta)
+    within(got.detach(), want_loss, tl + beta * m * U * lp.abs().max())
+    got.sum().backward()
+    within(logp.grad, torch.where(there, c, logp.grad.double()), tc + beta * beta * m * U * lp.abs().max() + 2 * U * c.abs())
