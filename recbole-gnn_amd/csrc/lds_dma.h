@@ -1,4 +1,4 @@
-// lds_dma.h — LDS-DMA (global_load_lds) helpers shared by the BiGNN forward and backward kernels.
+// lds_dma.h — LDS-DMA (global_load_lds) helpers shared by the BiGNN forward and backward kernels, the top-k's plane image and the 8-bit scores.
 //
 // A request moves 16 (or 4) bytes per lane from a per-lane global address to LDS at  M0 + 16 (4) x lane : the destination
 // is lane-linear, so any LDS layout other than "as the lanes are numbered" is made on the SOURCE side.  The kernels here
@@ -25,6 +25,20 @@ __device__ __forceinline__ void lds_dma16(const void *gsrc, unsigned lds_dst) { 
         "s_mov_b32 m0, %0"
         : "=&s"(keep)
         : "v"(gsrc), "s"(lds_dst)
+        : "memory");
+}
+
+// The same from base + off, base wave-uniform: 32 bits of address per lane.
+__device__ __forceinline__ void lds_dma16(const void *base, uint32_t off, unsigned lds_dst) {
+    unsigned keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(off), "s"(base), "s"(lds_dst)
         : "memory");
 }
 

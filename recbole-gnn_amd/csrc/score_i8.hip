@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "vocab_common.h"
 
 namespace rbg {
@@ -450,17 +451,6 @@ static int launch_few(const ScoreArgs &a, hipStream_t s) {
     return RBG_OK;
 }
 
-// 16 bytes per lane from base + off to the LDS bytes dst + 16 lane.  (m0 is this kernel's to use: nothing the compiler emits in it needs it.)
-__device__ __forceinline__ void dma16(const void *base, uint32_t off, unsigned dst) {
-    asm volatile(
-        "s_mov_b32 m0, %2\n\t"
-        "s_nop 0\n\t"
-        "global_load_lds_dwordx4 %0, %1"
-        :
-        : "v"(off), "s"(base), "s"(dst)
-        : "memory");
-}
-
 // Large products: a 64 W x 64 W tile of S per workgroup (W = 4, or 2 where that leaves CUs without one), one wave per SIMD with a quarter
 // of it (W x W accumulators of 32 x 32), K in steps of 128 bytes through two LDS stages that LDS-DMA fills.  A step is four slices of
 // 32 bytes: while a slice's W W products run, the next slice's 2 W fragments are read; the barrier that hands over a stage
@@ -499,10 +489,10 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void score_i8_tile_kernel(cons
         const uint32_t at = (uint32_t)step * 128;
         const bool end = step + 1 == steps;
         constexpr int q = 2 * decltype(part)::value;
-        dma16(bu, ou[q] + at, to + q * 1024);
-        dma16(bu, ou[q + 1] + at, to + q * 1024 + 1024);
-        dma16(bi, oi[q] + at - (end ? back[0] : 0u), to + STAGE / 2 + q * 1024);
-        dma16(bi, oi[q + 1] + at - (end ? back[1] : 0u), to + STAGE / 2 + q * 1024 + 1024);
+        lds_dma16(bu, ou[q] + at, to + q * 1024);
+        lds_dma16(bu, ou[q + 1] + at, to + q * 1024 + 1024);
+        lds_dma16(bi, oi[q] + at - (end ? back[0] : 0u), to + STAGE / 2 + q * 1024);
+        lds_dma16(bi, oi[q + 1] + at - (end ? back[1] : 0u), to + STAGE / 2 + q * 1024 + 1024);
     };
     auto each = [](auto f) {
         f(std::integral_constant<int, 0>{});
