@@ -346,7 +346,7 @@ constexpr int kOwnCodes = 2048;
 
 template <class TO, class TU, int UT, int IT, int KW>
 __global__ __launch_bounds__(256) void score_i8_few_kernel(const ScoreArgs a) {
-    constexpr int U = UT * IT >= 8 ? 2 : 4;  // steps of 64 bytes in flight
+    constexpr int U = 4;  // steps of 64 bytes in flight
     constexpr bool OWN = !std::is_void_v<TU>;
     // a row of codes: K rounded up to 64, and 16 more bytes so that the 16 rows of a fragment spread over the banks
     __shared__ alignas(16) int8_t own[OWN ? kOwnCodes + 16 * 80 : 16];
@@ -439,7 +439,9 @@ template <class TO, class TU, int UT>
 static int launch_few(const ScoreArgs &a, hipStream_t s) {
     const unsigned gy = (unsigned)((a.B + 16 * UT - 1) / (16 * UT));  // (a few)
     auto blocks = [&](int per) { return dim3((unsigned)((a.n + per - 1) / per), gy); };
-    if (a.kc >= 64) {  // 1 KB and more of a row: four waves share it
+    if constexpr (UT > 1) {  // (at most 8 192 items and groups of users: see launch_score_items)
+        hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), blocks(16), dim3(256), 0, s, a);
+    } else if (a.kc >= 64) {  // 1 KB and more of a row: four waves share it
         // more items per wave read the users' codes less often, but leave fewer waves
         if (a.n * gy <= 16 * 2048) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), blocks(16), dim3(256), 0, s, a);
         else if (a.n * gy <= 64 * 1024 || a.kc < 128) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), blocks(32), dim3(256), 0, s, a);
@@ -603,7 +605,7 @@ static int launch_score_items(const ScoreArgs &a, hipStream_t s) {
     if (a.B <= 16) return launch_few<TO, TU, 1>(a, s);
     if (a.kc <= 4) return launch_short<TO, TU, 2>(a, s);
     if (a.kc <= 8 || !std::is_void_v<TU>) return launch_short<TO, TU, 4>(a, s);
-    if (a.kc <= 16 && a.B * a.n * (int64_t)sizeof(TO) >= 128 << 20) return launch_short<TO, void, 8>(a, s);  // (4096 x 40 001 x 256: 197 us, 237 in tiles; 100 x 100 001 x 200: 40 and 22)
+    if (a.kc <= 16 && a.B * a.n * (int64_t)sizeof(TO) >= 128 << 20) return launch_short<TO, void, 8, 2048>(a, 512, s);  // (4096 x 40 001 x 256: 197 us, 237 in tiles; 100 x 100 001 x 200: 40 and 22)
     const int64_t wide = ((a.n + 255) / 256) * ((a.B + 255) / 256), small = ((a.n + 127) / 128) * ((a.B + 127) / 128);
     // 64 x 16 tiles with K over four waves, many times the workgroups (300 x 300 x 8 192: 31 us against 51; 1 000 x 1 000 x 1 024: 19 against 16)
     if (small <= 32 && a.kc >= 128) return launch_few<TO, void, 4>(a, s);
