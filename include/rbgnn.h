@@ -763,8 +763,8 @@ int rbg_quantize_rows_i8(const void *x, int64_t ldx, int dtype, int64_t n, int64
 int rbg_score_i8(const int8_t *qu, int64_t ldu, const float *su, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n,
                  int64_t K, void *S, int64_t lds, int out_dtype, void *stream);
 
-/* Both in one call: the rows u [B, K] of `dtype` are quantized (rbg_quantize_rows_i8) and scored (rbg_score_i8); for up to 16 rows of 2 048
- * values in all it is one launch.  `workspace`: rbg_score_rows_i8_workspace(B, K) bytes, 16-byte aligned. */
+/* Both in one call: the rows u [B, K] of `dtype` are quantized (rbg_quantize_rows_i8) and scored (rbg_score_i8); one launch for up to 16
+ * rows of 2 048 values in all, and for more rows of up to 128 values where these have at most 256 bytes or B n <= 2^21; else two.  `workspace`: rbg_score_rows_i8_workspace(B, K) bytes, 16-byte aligned. */
 int rbg_score_rows_i8_workspace(int64_t B, int64_t K, int64_t *bytes);
 int rbg_score_rows_i8(const void *u, int64_t ldu, int dtype, int64_t B, const int8_t *qi, int64_t ldi, const float *si, int64_t n, int64_t K,
                       void *S, int64_t lds, int out_dtype, void *workspace, void *stream);

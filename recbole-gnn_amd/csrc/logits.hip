@@ -696,7 +696,7 @@ __global__ __launch_bounds__(TH) void pair_rows_kernel(const LogpArgs a, int64_t
 
 // Small calls in one launch: a workgroup per pair, a wave per row.  Both sums meet in LDS, and the rows, read a second time for their
 // gradient, are still in the caches.  (m, S) of a row stays with the wave that goes on to write it.  Bound by that chain of latencies: 40
-// tokens of 1 683 fp32 logits in 10.7 us.
+// tokens of 1 683 fp32 logits in 10.8 us.
 template <class T>
 __global__ __launch_bounds__(1024) void pair_small_kernel(const LogpArgs a, int64_t m, const int64_t *offsets, const float *ref, float beta,
                                                           float smoothing, const float *pair_w, float *loss, float *margin, void *gv, int64_t ldg) {
@@ -811,6 +811,9 @@ static int launch_distill_rows(const DistillArgs &a, int64_t n, int64_t V, int S
         else hipLaunchKernelGGL((distill_eval_kernel<T, 256>), dim3((unsigned)n), dim3(256), 0, s, a);
     } else {
         const int64_t chunks = V * (int64_t)sizeof(T) / 16;  // at most this many whole ones
+        // The smallest that holds the row; the next one up costs (us, bf16): 4 096 x 2 048 12.5 -> 16, 4 096 x 8 192 29 -> 33, 2 048 x 16 384
+        // 28.5 -> 30, x 28 672 42 -> 44, x 40 982 62 -> 67, 1 024 x 65 536 46 -> 48, x 91 600 67 -> 84; a row read twice instead (fp32)
+        // 1 024 x 91 600 149 -> 182.
         const dim3 grid((unsigned)n);
         if (chunks <= 64 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 64, 4>), grid, dim3(64), 0, s, a);
         else if (chunks <= 256 * 4) hipLaunchKernelGGL((distill_row_kernel<T, 256, 4>), grid, dim3(256), 0, s, a);

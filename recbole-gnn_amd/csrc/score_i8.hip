@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *__restrict__ x, 
     }
 }
 
-// Longer rows: one workgroup per row, which it reads twice.
+// Longer rows (of more than 16 384 values in 32 bits, 32 768 in 16): one workgroup per row, which it reads twice and element by element.  512 rows
+// of 16 448 fp32 in 36 us where 16 384 take 11, of 32 832 bf16 in 70 where 32 768 take 19: correct at any length, not made for speed.
 template <class T>
 __global__ __launch_bounds__(256) void quantize_long_kernel(const T *__restrict__ x, int64_t ldx, int64_t K, int8_t *__restrict__ codes, int64_t ldc,
                                                            float *__restrict__ scale) {
@@ -218,7 +219,8 @@ __device__ __forceinline__ float own_codes(const TU *x, int K, int h, i32x4 (&co
 // taken straight from the table, and puts its scores into LDS, every row shifted by its distance from a 128-byte line.  Whole lines then
 // leave as 16-byte stores of consecutive lanes (1 KB of a row per wave and store at TB = 2048), whatever the row stride; what a tile leaves
 // over of a row's last line (less than LINE scores) moves to the front of the row for the next tile.  4 096 x 40 982 x 64 into fp32:
-// 672 MB in 135 us = 5.0 TB/s, which is the rate of bare whole-line stores into rows of that stride (131 to 138).
+// 672 MB in 141 to 147 us behind itself, 138 to 140 a call among other work = 4.6 to 4.9 TB/s; bare whole-line stores into rows of that
+// stride take 131 to 138.
 template <class TO, class TU, int KS, int TB>
 __global__ __launch_bounds__(256, TB == 2048 ? 2 : 4) void score_i8_short_kernel(const ScoreArgs a, int tiles_per_walk) {
     constexpr int E = 16 / (int)sizeof(TO), TILE = TB / (int)sizeof(TO), LINE = 128 / (int)sizeof(TO), PITCH = TILE + LINE;
@@ -442,11 +444,12 @@ static int launch_few(const ScoreArgs &a, hipStream_t s) {
     if constexpr (UT > 1) {  // (at most 8 192 items and groups of users: see launch_score_items)
         hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), blocks(16), dim3(256), 0, s, a);
     } else if (a.kc >= 64) {  // 1 KB and more of a row: four waves share it
-        // more items per wave read the users' codes less often, but leave fewer waves
+        // more items per wave read the users' codes less often, but leave fewer waves (16, 32 and 64 items, us: 16 x 32 768 x 2 048 20, 18, 19;
+        // 1 x 65 536 x 1 024 25, 22, 20; 1 x 65 536 x 2 048 47, 47, 36; 1 x 131 072 x 2 048 82, 79, 68; 16 x 131 072 x 2 048 70, 59, 56)
         if (a.n * gy <= 16 * 2048) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 1, 4>), blocks(16), dim3(256), 0, s, a);
         else if (a.n * gy <= 64 * 1024 || a.kc < 128) hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 4>), blocks(32), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 4, 4>), blocks(64), dim3(256), 0, s, a);
-    } else {
+    } else {  // (1 x 131 072 x 960: 27, and 32 with the row over four waves; 16 x 131 072 x 512: 19.6 and 18.4)
         hipLaunchKernelGGL((score_i8_few_kernel<TO, TU, UT, 2, 1>), blocks(128), dim3(256), 0, s, a);
     }
     RBG_HIP(hipGetLastError());
@@ -610,7 +613,8 @@ static int launch_score_items(const ScoreArgs &a, hipStream_t s) {
     // 64 x 16 tiles with K over four waves, many times the workgroups (300 x 300 x 8 192: 31 us against 51; 1 000 x 1 000 x 1 024: 19 against 16)
     if (small <= 32 && a.kc >= 128) return launch_few<TO, void, 4>(a, s);
     // Rounds of 256 x 256 tiles (one per CU) against 128 x 128 ones, whose products cost about 1.37 times as much but which waste less of the
-    // last round and of the edges.
+    // last round and of the edges.  (128 and 256 wide, us: 2 000 x 2 000 x 4 096 39 and 74; 3 000 x 3 000 x 2 048 45 and 53; 4 096 x 16 384 x
+    // 2 048 199 and 188.  Short rows are the stores' and the small tiles' again, which the rule leaves: 4 096 x 8 192 x 1 024 60 and 70.)
     return (wide + 255) / 256 * 4 <= 1.37 * small / 256 ? launch_tiles<TO, 4>(a, s) : launch_tiles<TO, 2>(a, s);
 }
 
