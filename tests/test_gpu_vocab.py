@@ -1067,3 +1067,62 @@ def test_preference_offsets_outside_in_every_form(rbg, cuda, dtype, m, v, where)
     within(got.detach(), want_loss, tl + beta * m * U * lp.abs().max())
     got.sum().backward()
     within(logp.grad, torch.where(there, c, logp.grad.double()), tc + beta * beta * m * U * lp.abs().max() + 2 * U * c.abs())
+
+
+def test_captured_forward_and_backward(rbg, cuda):
+    """A training step's forward and backward of every differentiable operator in one captured graph, replayed with new inputs and eager work
+    between the replays."""
+    g = gen(31, cuda)
+    n, v, d, k = 700, 1500, 24, 8
+    table = torch.randn(v, d, generator=g, device=cuda)
+    ids, y = torch.randint(-1, v, (n,), generator=g, device=cuda), torch.randint(-1, v, (n,), generator=g, device=cuda)
+    idx, val = torch.randint(-1, v, (n, k), generator=g, device=cuda), torch.randn(n, k, generator=g, device=cuda)
+    offsets, ref = packed(5, n, 6, cuda, 3, 4), torch.randn(12, generator=g, device=cuda)
+
+    def step():
+        leaf = table.detach().requires_grad_()
+        logits = rbg.embedding(leaf, ids, scale=0.5, padding_idx=3) @ table.t()
+        z = logits.detach().requires_grad_()
+        loss, margin = rbg.preference_loss(rbg.token_logp(z, y), offsets, ref)
+        total = rbg.distill_topk(z, idx, val, temperature=2.0).sum() + loss.sum() + margin.sum()
+        (dz,) = torch.autograd.grad(total, z)
+        (dt,) = torch.autograd.grad(logits, leaf, dz)
+        return total.detach(), dz, dt
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        table.mul_(-0.9)
+        val.add_(0.1)
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        # (the sum of the losses is torch's own: its order may differ by capture)
+        assert abs(float(out[0]) - float(eager[0])) <= 1e-4 * abs(float(eager[0])) and torch.equal(out[1], eager[1]) and torch.equal(out[2], eager[2])
+
+
+def test_nothing_to_do_through_autograd(rbg, cuda):
+    """Calls of no rows, no pairs or no tokens have outputs and gradients of those shapes."""
+    none = torch.zeros(0, dtype=torch.int64, device=cuda)
+    for z in (torch.zeros(0, 5, device=cuda, requires_grad=True),):
+        (rbg.distill_topk(z, none[:, None].expand(0, 3), torch.zeros(0, 3, device=cuda)).sum() + rbg.token_logp(z, none).sum()).backward()
+        assert z.grad.shape == (0, 5)
+    table = torch.ones(4, 3, device=cuda, requires_grad=True)
+    rbg.embedding(table, none).sum().backward()
+    assert torch.all(table.grad == 0)
+    one = torch.zeros(1, dtype=torch.int64, device=cuda)
+    for m in (0, 3, 300, 1100):
+        z, y = torch.randn(m, 7, device=cuda), torch.zeros(m, dtype=torch.int64, device=cuda)
+        loss, margin, grad = rbg.preference_grad(z, y, one, torch.zeros(0, device=cuda))  # no pairs
+        assert loss.shape == margin.shape == (0,) and grad.shape == (m, 7) and torch.all(grad == 0)
+        logp = torch.zeros(m, device=cuda, requires_grad=True)
+        rbg.preference_loss(logp, one, torch.zeros(0, device=cuda))[0].sum().backward()
+        assert torch.all(logp.grad == 0)
+        loss, margin, grad = rbg.preference_grad(z, y, one.expand(5), torch.zeros(4, device=cuda))  # pairs of no tokens
+        assert torch.all(margin == 0) and bool(torch.allclose(loss, torch.full_like(loss, math.log(2)))) and torch.all(grad == 0)
